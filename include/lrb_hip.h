@@ -532,6 +532,60 @@ int lrb_vae_encode_dev(lrb_vae *v, const float *d_data, uint64_t n_rows, float *
  * 10+i / 20+i encoder / decoder block outputs, 30 the per-slice parameter gradients). */
 int lrb_vae_debug_read(lrb_vae *v, int which, float *host, uint64_t count);
 
+/* ---- K9, K10: operators of a network's training ---------------------------- */
+/* These entry points keep nothing between calls, so they take the device and the caller's hipStream_t (NULL: the legacy
+ * default stream) instead of a context, and their workspace from the caller: calls on different streams do not share
+ * anything, and a call may be made inside a stream capture.  The calling thread's current device is left as it was.
+ * Element types (x, w, p, g, m below): */
+#define LRB_F32 0
+#define LRB_BF16 1
+#define LRB_F16 2
+
+/* K9, layer normalisation over the last axis (csrc/lrb_norm.hip):
+ *   u = x, or with slope != 1 or d_keep: u = keep * keep_scale * (x > 0 ? x : slope * x);  a dropped element (keep 0) is 0
+ *       whatever x holds
+ *   y = (u - mean) / sqrt(var + eps) * w + b
+ * x: rows x cols, the elements of a row side by side, rows x_stride elements apart; y: packed.  w, b: cols elements each or
+ * NULL (1, 0), float32 or of x's type (w_type).  keep: rows x cols bytes, packed, or NULL.  d_mean, d_rstd: float32[rows],
+ * what the backward pass needs, or both NULL.  Any number of rows and columns (below 2^29) from one on. */
+int lrb_layer_norm_fwd_dev(int device, void *stream, int x_type, int w_type, uint64_t rows, uint64_t cols, const void *d_x,
+                           int64_t x_stride, const void *d_w, const void *d_b, float eps, float slope, const uint8_t *d_keep,
+                           float keep_scale, void *d_y, float *d_mean, float *d_rstd);
+/* Its gradients for dy (x's type, rows dy_stride elements apart; 0: one row for all): dx packed, dw and db of w_type; any of
+ * the three may be NULL.  d_ws: lrb_layer_norm_bwd_ws_bytes, needed for dw or db only.  The sums over the rows are made
+ * in a fixed order. */
+uint64_t lrb_layer_norm_bwd_ws_bytes(int x_type, uint64_t rows, uint64_t cols);
+int lrb_layer_norm_bwd_dev(int device, void *stream, int x_type, int w_type, uint64_t rows, uint64_t cols, const void *d_x,
+                           int64_t x_stride, const void *d_dy, int64_t dy_stride, const void *d_w, const float *d_mean,
+                           const float *d_rstd, float slope, const uint8_t *d_keep, float keep_scale, void *d_dx, void *d_dw,
+                           void *d_db, void *d_ws, uint64_t ws_bytes);
+
+/* K10, the orthogonalised update (csrc/lrb_muon.hip), for a list of weights in shared launches.  For each of `count`
+ * matrices of an item:
+ *   m <- momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;  without m: u = g
+ *   X = u / max(|u|_F, eps);  `steps` times X <- a X + (b A + c A^2) X, A = X X^T (X^T X of a tall matrix)
+ *   p <- decay p + alpha X;  with decay = 0 p is not read
+ * Strides are in elements, of (matrix, row, column), any values; p and m must not overlap each other, g, or another item's.
+ * A matrix that holds an infinity or a NaN gives NaN throughout.  1 <= steps <= 32; a matrix below 2^31 elements with sides
+ * below 2^24.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
+typedef struct {
+    void *p;
+    const void *g;
+    void *m; /* or NULL */
+    int64_t p_stride[3], g_stride[3], m_stride[3];
+    int64_t count, rows, cols;
+    int32_t p_type, g_type, m_type;
+    float alpha, decay;
+    int32_t reserved;
+} lrb_muon_item;
+/* How large a singular value from [0, 1] may become in `steps` steps with these coefficients; LRB_ERR_ARG from lrb_muon_dev
+ * where that is more than LRB_MUON_DIVERGED (the factors' 16-bit halves are scaled by this bound). */
+#define LRB_MUON_DIVERGED 64.0
+double lrb_muon_bound(int steps, float a, float b, float c);
+uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items);
+int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items, int n_items, float momentum, int nesterov, int steps,
+                 float a, float b, float c, float eps, void *d_ws, uint64_t ws_bytes);
+
 /* ---- host side: ingest and profile text -------------------------------- */
 /* FASTA/FASTQ(.gz) reader with the record semantics of SeqReader::get_seq
  * (io_utils.h:133-165) over kseq_read (kseq.h:177-218). */

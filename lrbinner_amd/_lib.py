@@ -140,6 +140,15 @@ PROTOTYPES = {
     "lrb_vae_steps_done": (C.c_int, [vp, u64p]),
     "lrb_vae_train_dev": (C.c_int, [vp, vp, vp, C.c_uint32, C.c_uint32, C.c_int]),
     "lrb_vae_encode_dev": (C.c_int, [vp, vp, C.c_uint64, vp]),
+    "lrb_layer_norm_fwd_dev": (C.c_int, [C.c_int, vp, C.c_int, C.c_int, C.c_uint64, C.c_uint64, vp, C.c_int64, vp, vp, C.c_float,
+                                         C.c_float, vp, C.c_float, vp, vp, vp]),
+    "lrb_layer_norm_bwd_ws_bytes": (C.c_uint64, [C.c_int, C.c_uint64, C.c_uint64]),
+    "lrb_layer_norm_bwd_dev": (C.c_int, [C.c_int, vp, C.c_int, C.c_int, C.c_uint64, C.c_uint64, vp, C.c_int64, vp, C.c_int64, vp, vp,
+                                         vp, C.c_float, vp, C.c_float, vp, vp, vp, vp, C.c_uint64]),
+    "lrb_muon_bound": (C.c_double, [C.c_int, C.c_float, C.c_float, C.c_float]),
+    "lrb_muon_ws_bytes": (C.c_uint64, [vp, C.c_int]),
+    "lrb_muon_dev": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_float, C.c_int, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float, vp,
+                               C.c_uint64]),
     "lrb_vae_debug_read": (C.c_int, [vp, C.c_int, C.POINTER(C.c_float), C.c_uint64]),
     "lrb_reader_open": (C.c_int, [C.c_char_p, C.POINTER(vp)]),
     "lrb_fasta_scan": (C.c_int, [C.c_char_p, C.POINTER(vp)]),

@@ -88,6 +88,24 @@ __device__ __forceinline__ void lrb_barrier()
 }
 #endif
 
+// The calling thread's current device for the length of a call, put back at its end: for entry points that take the device
+// and the stream instead of a context.
+struct lrb_on_device {
+    int before = -1, here;
+    hipError_t err;
+    explicit lrb_on_device(int device) : here(device)
+    {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != here) err = hipSetDevice(here);
+    }
+    ~lrb_on_device()
+    {
+        if (before >= 0 && before != here) (void)hipSetDevice(before);
+    }
+    lrb_on_device(const lrb_on_device &) = delete;
+    lrb_on_device &operator=(const lrb_on_device &) = delete;
+};
+
 // hipFuncSetAttribute is per DEVICE: a launch site remembers which devices it has raised its kernel's limit on
 // (the C ABI allows contexts on several GPUs in one process).  A race between two threads sets the attribute twice.
 struct lrb_per_device_once {

@@ -1,0 +1,565 @@
+// lrb_muon.hip -- K10: the orthogonalised update of a list of weights (momentum, polynomial iteration, step), gfx950 only.
+//
+//   m <- beta m + (1 - beta) g;  u = (1 - beta) g + beta m  (nesterov), else m;  without a momentum buffer u = g
+//   X = u / max(|u|_F, eps), taken with its short side as rows: n x m, n <= m
+//   steps times:  A = X X^T,  B = b A + c A^2,  X <- a X + B X
+//   p <- decay p + alpha X
+//
+// Bound: the matrix cores (2 n^2 m + 2 n^3 + 2 n^2 m multiply-adds a step, of the two symmetric products half).  The
+// float32 matrix instructions run at 1/16 of the rate of the 16-bit ones, so every factor is held as TWO float16 numbers,
+// hi = fp16(s v) and lo = fp16(s v - hi), and a product is three: hi hi + hi lo + lo hi, added up in float32.  What is left
+// out (lo lo and the rounding of lo) is about 2^-23 of the value, i.e. the result is as exact as float32 products are:
+// the polynomial stretches small singular values by up to a^steps (485 for the usual coefficients), so a 16-bit iteration
+// would return noise where a gradient is of low rank.  s is a power of two for each matrix, step and factor, from a bound
+// on the factor's largest singular value (the Frobenius norm bounds X by 1, the polynomial's extremes bound what follows):
+// no entry can leave fp16's range whatever the coefficients or the size of u, and the entries use its upper end.
+//
+// All products are of the form C[i][j] = sum_k P[i][k] Q[j][k] with k contiguous in both: A = X X^T and A^2 = A A^T as they
+// stand, B X from X's transpose, which the epilogue writes beside X.  One workgroup a T x T tile of C; of the symmetric
+// products the tiles on and above the diagonal are computed and mirrored.  Tiles of all weights of a call share a launch.
+#include <limits.h>
+#include <math.h>
+
+#include "lrb_device.h"
+
+typedef _Float16 mu_h;
+typedef mu_h mu_h8 __attribute__((ext_vector_type(8)));
+typedef mu_h mu_h4 __attribute__((ext_vector_type(4)));
+typedef float mu_f16 __attribute__((ext_vector_type(16)));
+
+#define MU_ITEMS 16       // weights of one launch (their descriptors travel as kernel arguments)
+#define MU_STEPS 32       // longest iteration
+#define MU_COEF 5         // floats of the table for each matrix and step: kA, kB1, kB2, kX1, kX2
+#define MU_TOP 57344.0    // the largest entry that a factor is scaled to: 7/8 of fp16's largest number
+#define MU_BK 32          // k of one stage in LDS
+
+struct mu_item {
+    void *p;
+    const void *g;
+    void *m;
+    long long ps[3], gs[3], ms[3]; // element strides of (matrix, short side, long side)
+    unsigned long long off, step;  // bytes: the first matrix's planes in the workspace, from one matrix to the next
+    int n, l, np, lp, count;       // short side, long side, both padded to 64; matrices
+    int first;                     // number of the first matrix in the tables
+    int p_type, g_type, m_type;
+    float alpha, decay;
+};
+
+struct mu_args {
+    char *ws;
+    double *x0;     // [matrices] what u is multiplied by
+    float *table;   // [matrices][steps][MU_COEF]
+    double *part;   // [tiles of 64 x 64 of all matrices] sums of squares
+    int n_items, steps;
+    float beta, eps, a, b, c;
+    int nesterov;
+    int flip;       // which of the two copies of X is read
+    int step;
+    int start[MU_ITEMS + 1]; // first tile of each item in this launch
+    mu_item it[MU_ITEMS];
+};
+
+// The planes of a matrix: X and its transpose twice (read and written in turn), A, B, hi then lo in each; and X and A in
+// float32, for the terms a X and b A: hi + lo is a rounding more than float32 is, and these terms would pass it on.
+__host__ __device__ inline unsigned long long mu_plane_x(const mu_item &it) { return 2ull * (unsigned long long)it.np * it.lp; }
+__host__ __device__ inline unsigned long long mu_plane_a(const mu_item &it) { return 2ull * (unsigned long long)it.np * it.np; }
+__host__ __device__ inline unsigned long long mu_bytes(const mu_item &it) { return 10 * mu_plane_x(it) + 6 * mu_plane_a(it); }
+
+struct mu_mat {
+    mu_h *x, *xt, *x2, *xt2, *a, *b; // lo planes follow their hi planes
+    float *x32, *a32;
+};
+__device__ __forceinline__ mu_mat mu_planes(const mu_args &a, const mu_item &it, int mat)
+{
+    char *w = a.ws + it.off + (unsigned long long)mat * it.step;
+    const unsigned long long px = 2 * mu_plane_x(it), pa = 2 * mu_plane_a(it);
+    mu_mat r;
+    r.x = (mu_h *)(w + (a.flip ? 2 * px : 0));
+    r.xt = (mu_h *)(w + (a.flip ? 3 * px : px));
+    r.x2 = (mu_h *)(w + (a.flip ? 0 : 2 * px));
+    r.xt2 = (mu_h *)(w + (a.flip ? px : 3 * px));
+    r.a = (mu_h *)(w + 4 * px);
+    r.b = (mu_h *)(w + 4 * px + pa);
+    r.x32 = (float *)(w + 4 * px + 2 * pa);
+    r.a32 = (float *)(w + 5 * px + 2 * pa);
+    return r;
+}
+
+__device__ __forceinline__ float mu_load(const void *p, long long at, int type)
+{
+    return type == LRB_F32 ? ((const float *)p)[at] : type == LRB_BF16 ? (float)((const __bf16 *)p)[at] : (float)((const mu_h *)p)[at];
+}
+__device__ __forceinline__ void mu_store(void *p, long long at, int type, float v)
+{
+    if (type == LRB_F32) ((float *)p)[at] = v;
+    else if (type == LRB_BF16) ((__bf16 *)p)[at] = (__bf16)v;
+    else ((mu_h *)p)[at] = (mu_h)v;
+}
+
+// Which item a tile of the launch belongs to.
+__device__ __forceinline__ int mu_find(const mu_args &a, int tile)
+{
+    int k = 0;
+    while (k + 1 < a.n_items && tile >= a.start[k + 1]) ++k;
+    return k;
+}
+
+// u at (i, j); UPDATE also writes the momentum back (each entry by one thread)
+template <bool UPDATE> __device__ __forceinline__ float mu_u(const mu_args &a, const mu_item &it, int mat, int i, int j)
+{
+    const float g = mu_load(it.g, mat * it.gs[0] + i * it.gs[1] + j * it.gs[2], it.g_type);
+    if (!it.m) return g;
+    const long long at = mat * it.ms[0] + i * it.ms[1] + j * it.ms[2];
+    float m = mu_load(it.m, at, it.m_type);
+    if (UPDATE) {
+        m = a.beta * m + (1.0f - a.beta) * g;
+        mu_store(it.m, at, it.m_type, m);
+        m = it.m_type == LRB_F32 ? m : it.m_type == LRB_BF16 ? (float)(__bf16)m : (float)(mu_h)m; // u is made of what is kept
+    }
+    return a.nesterov ? (1.0f - a.beta) * g + a.beta * m : m;
+}
+
+// Momentum, and the sum of the squares of u over a 64 x 64 tile, in double (the squares of large float32 leave its range).
+__global__ __launch_bounds__(256) void mu_momentum_kernel(mu_args a)
+{
+    __shared__ double red[4];
+    const int k = mu_find(a, blockIdx.x);
+    const mu_item &it = a.it[k];
+    const int tj = it.lp / 64, per = (it.np / 64) * tj, local = blockIdx.x - a.start[k], mat = local / per, r = local % per;
+    const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
+    const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
+    double s = 0.0;
+#pragma unroll 4
+    for (int e = 0; e < 16; ++e) {
+        const int q = e * 256 + threadIdx.x, fast = q & 63, slow = q >> 6;
+        const int i = i0 + (along_j ? slow : fast), j = j0 + (along_j ? fast : slow);
+        if (i < it.n && j < it.l) {
+            const double u = mu_u<true>(a, it, mat, i, j);
+            s += u * u;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    lrb_barrier();
+    if (threadIdx.x == 0) a.part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__host__ __device__ double mu_largest_odd(double a, double b, double c, double r) // max |a x + b x^3 + c x^5| over [0, r]
+{
+    double best = fabs(r * (a + r * r * (b + c * r * r)));
+    const double d = 9.0 * b * b - 20.0 * a * c; // 5 c t^2 + 3 b t + a = 0, t = x^2
+    for (int s = -1; s <= 1; s += 2) {
+        const double t = c != 0.0 ? (d >= 0.0 ? (-3.0 * b + s * sqrt(d)) / (10.0 * c) : -1.0) : b != 0.0 ? -a / (3.0 * b) : -1.0;
+        if (t > 0.0 && t < r * r) best = fmax(best, fabs(sqrt(t) * (a + t * (b + c * t))));
+    }
+    return best;
+}
+
+__device__ double mu_scale(double r) // the power of two that takes entries up to r to at most MU_TOP
+{
+    return r > 0.0 && r < 1e300 ? exp2(floor(log2(MU_TOP / r))) : 1.0;
+}
+
+// The norm of every matrix, and with it the scales of its factors in every step.
+__global__ __launch_bounds__(256) void mu_table_kernel(mu_args a)
+{
+    __shared__ double red[4];
+    int k = 0;
+    while (k + 1 < a.n_items && (int)blockIdx.x >= a.it[k + 1].first) ++k;
+    const mu_item &it = a.it[k];
+    const int per = (it.np / 64) * (it.lp / 64), mat = blockIdx.x - it.first;
+    const double *part = a.part + a.start[k] + (size_t)mat * per;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < per; i += 256) s += part[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    lrb_barrier();
+    if (threadIdx.x) return;
+    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
+    const double over = fmax(norm, (double)a.eps);
+    const double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
+    double r = fmax(norm / over, 1e-60) * slack, sx = mu_scale(r);
+    // an infinity or a NaN anywhere makes the whole matrix NaN
+    a.x0[blockIdx.x] = norm < 1e300 ? (over > 0.0 ? sx / over : 0.0) : (double)NAN;
+    float *t = a.table + (size_t)blockIdx.x * a.steps * MU_COEF;
+    for (int q = 0; q < a.steps; ++q, t += MU_COEF) {
+        const double ra = r * r * slack, sa = mu_scale(ra);
+        double rb = fabs(a.b * ra + (double)a.c * ra * ra);
+        if (a.c != 0.0f && -a.b / (2.0 * a.c) > 0.0 && -a.b / (2.0 * a.c) < ra) rb = fmax(rb, (double)a.b * a.b / fabs(4.0 * a.c));
+        rb *= slack;
+        const double sb = mu_scale(rb);
+        r = mu_largest_odd(a.a, a.b, a.c, r) * slack;
+        const double sn = q + 1 < a.steps ? mu_scale(r) : 1.0;
+        t[0] = (float)(sa / (sx * sx));
+        t[1] = (float)(a.b * (sb / sa));
+        t[2] = (float)(a.c * (sb / sa) / sa);
+        t[3] = (float)(a.a * (sn / sx));
+        t[4] = (float)(sn / sb / sx);
+        sx = sn;
+    }
+}
+
+__device__ __forceinline__ void mu_split(float v, mu_h &hi, mu_h &lo)
+{
+    hi = (mu_h)v;
+    lo = (mu_h)(v - (float)hi);
+}
+
+// u, scaled and split, as X and as its transpose: a 64 x 64 tile through LDS, so that all sides are read and written in rows.
+__global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
+{
+    __shared__ float tile[64][65];
+    const int k = mu_find(a, blockIdx.x);
+    const mu_item &it = a.it[k];
+    const int tj = it.lp / 64, per = (it.np / 64) * tj, local = blockIdx.x - a.start[k], mat = local / per, r = local % per;
+    const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
+    const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
+    const double scale = a.x0[it.first + mat];
+#pragma unroll 4
+    for (int e = 0; e < 16; ++e) {
+        const int q = e * 256 + threadIdx.x, fast = q & 63, slow = q >> 6;
+        const int i = along_j ? slow : fast, j = along_j ? fast : slow;
+        tile[i][j] = i0 + i < it.n && j0 + j < it.l ? (float)(scale * mu_u<false>(a, it, mat, i0 + i, j0 + j)) : 0.0f;
+    }
+    lrb_barrier();
+    const mu_mat w = mu_planes(a, it, mat);
+    const size_t plane = (size_t)it.np * it.lp;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int q = e * 256 + threadIdx.x, row = q >> 3, c = (q & 7) * 8;
+        float v[8];
+        mu_h8 hi, lo;
+        const size_t at = (size_t)(i0 + row) * it.lp + j0 + c, at_t = (size_t)(j0 + row) * it.np + i0 + c;
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) {
+            mu_h h, l;
+            v[e8] = tile[row][c + e8];
+            mu_split(v[e8], h, l);
+            hi[e8] = h, lo[e8] = l;
+        }
+        __builtin_memcpy(w.x32 + at, v, 32);
+        *(mu_h8 *)(w.x + at) = hi;
+        *(mu_h8 *)(w.x + plane + at) = lo;
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) {
+            mu_h h, l;
+            mu_split(tile[c + e8][row], h, l);
+            hi[e8] = h, lo[e8] = l;
+        }
+        *(mu_h8 *)(w.xt + at_t) = hi;
+        *(mu_h8 *)(w.xt + plane + at_t) = lo;
+    }
+}
+
+enum { MU_GRAM = 0, MU_POLY = 1, MU_APPLY = 2, MU_LAST = 3 };
+
+__device__ __forceinline__ void mu_dma(const mu_h *src, char *dst)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+
+// One tile of a product.  LDS holds two stages of 32 k: rows of 64 bytes, P hi, P lo, Q hi, Q lo; the four 16-byte chunks of
+// a row lie at chunk ^ ((row >> 2) & 3), which spreads the 16 rows that a quarter wave reads over all 64 banks.  The loads go
+// from global memory to LDS directly, one stage ahead of the products.
+template <int T, int WM, int WN, int MODE>
+__global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
+{
+    constexpr int WAVES = WM * WN, MI = T / WM / 32, NI = T / WN / 32, LOADS = 4 * T / 16 / WAVES;
+    __shared__ __attribute__((aligned(1024))) char buf0[4 * T * 64];
+    __shared__ __attribute__((aligned(1024))) char buf1[4 * T * 64];
+    // neighbouring workgroups go to different XCDs: each of the eight takes a run of neighbouring tiles
+    const int total = a.start[a.n_items], per_xcd = (total + 7) / 8;
+    const int tile = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (tile >= total) return;
+    const int k = mu_find(a, tile);
+    const mu_item &it = a.it[k];
+    const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
+    const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
+    int i0, j0 = local % per;
+    if (MODE >= MU_APPLY) {
+        i0 = j0 / tj;
+        j0 -= i0 * tj;
+    } else { // the tiles on and above the diagonal, row by row
+        i0 = 0;
+        while (j0 >= ti - i0) j0 -= ti - i0++;
+        j0 += i0;
+    }
+    i0 *= T, j0 *= T;
+    const mu_mat w = mu_planes(a, it, mat);
+    const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
+    const mu_h *P = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.b, *Q = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.xt;
+    const size_t p_plane = (size_t)it.np * K, q_plane = (size_t)jrows * K;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / WN, wj = wave % WN;
+
+    const mu_h *src[LOADS];
+    int dst[LOADS];
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) {
+        const int r0 = (q * WAVES + wave) * 16, r = r0 + (lane >> 2); // of the 4 T rows of a stage
+        const int part = r0 / T, row = r % T, chunk = (lane & 3) ^ ((r >> 2) & 3);
+        // rows past the padding (tiles larger than 64) repeat the last one; what they give is not stored
+        const int at = part < 2 ? min(i0 + row, it.np - 1) : min(j0 + row, jrows - 1);
+        src[q] = (part < 2 ? P : Q) + (part & 1 ? (part < 2 ? p_plane : q_plane) : 0) + (size_t)at * K + chunk * 8;
+        dst[q] = r0 * 64;
+    }
+
+    mu_f16 acc[MI][NI];
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int y = 0; y < NI; ++y)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[x][y][v] = 0.0f;
+
+    const int frow = lane & 31, fchunk = lane >> 5;
+    auto stage = [&](char *buf, int k0) {
+#pragma unroll
+        for (int q = 0; q < LOADS; ++q) mu_dma(src[q] + k0, buf + dst[q]);
+        __builtin_amdgcn_sched_barrier(0); // else the compiler sinks the loads to the wait that ends the stage
+    };
+    auto products = [&](const char *buf) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            mu_h8 ph[MI], pl[MI], qh[NI], ql[NI];
+#pragma unroll
+            for (int x = 0; x < MI; ++x) {
+                const int row = (wi * MI + x) * 32 + frow, at = row * 64 + (((kk * 2 + fchunk) ^ ((row >> 2) & 3)) << 4);
+                ph[x] = *(const mu_h8 *)(buf + at);
+                pl[x] = *(const mu_h8 *)(buf + T * 64 + at);
+            }
+#pragma unroll
+            for (int y = 0; y < NI; ++y) {
+                const int row = (wj * NI + y) * 32 + frow, at = row * 64 + (((kk * 2 + fchunk) ^ ((row >> 2) & 3)) << 4);
+                qh[y] = *(const mu_h8 *)(buf + 2 * T * 64 + at);
+                ql[y] = *(const mu_h8 *)(buf + 3 * T * 64 + at);
+            }
+#pragma unroll
+            for (int x = 0; x < MI; ++x)
+#pragma unroll
+                for (int y = 0; y < NI; ++y) {
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[y], ph[x], acc[x][y], 0, 0, 0);
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[y], pl[x], acc[x][y], 0, 0, 0);
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[y], ph[x], acc[x][y], 0, 0, 0);
+                }
+        }
+    };
+    // K is a multiple of 64: two stages a turn.  A stage is written while the other is read; the barrier says that all waves
+    // have left the one that is written next, the wait before it that the wave's own loads have arrived.
+    stage(buf0, 0);
+    for (int k0 = 0; k0 < K; k0 += 2 * MU_BK) {
+        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
+        lrb_barrier();
+        stage(buf1, k0 + MU_BK);
+        products(buf0);
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        lrb_barrier();
+        if (k0 + 2 * MU_BK < K) stage(buf0, k0 + 2 * MU_BK);
+        products(buf1);
+    }
+
+    // lane -> row i of C, four neighbouring columns j in every four registers
+    const float *t = a.table + ((size_t)(it.first + mat) * a.steps + a.step) * MU_COEF;
+    const float k1 = MODE == MU_GRAM ? 0.0f : MODE == MU_POLY ? t[1] : t[3], k2 = MODE == MU_GRAM ? t[0] : MODE == MU_POLY ? t[2] : t[4];
+    const int ld = MODE >= MU_APPLY ? it.lp : it.np;
+    const size_t plane = (size_t)it.np * ld;
+    float *full = MODE <= MU_POLY ? w.a32 : w.x32;
+    mu_h *out = MODE == MU_GRAM ? w.a : MODE == MU_POLY ? w.b : w.x2, *out_t = MODE == MU_APPLY ? w.xt2 : out;
+    const bool mirror = MODE == MU_APPLY || i0 != j0;
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int y = 0; y < NI; ++y)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = i0 + (wi * MI + x) * 32 + frow, j = j0 + (wj * NI + y) * 32 + 8 * q + 4 * fchunk;
+                if (i >= it.np || j >= jrows) continue;
+                float4 v = {};
+                float4 *const old = (float4 *)(full + (size_t)i * ld + j);
+                if (MODE != MU_GRAM) v = *old;
+                v.x = k1 * v.x + k2 * acc[x][y][4 * q], v.y = k1 * v.y + k2 * acc[x][y][4 * q + 1];
+                v.z = k1 * v.z + k2 * acc[x][y][4 * q + 2], v.w = k1 * v.w + k2 * acc[x][y][4 * q + 3];
+                if (MODE == MU_LAST) {
+                    if (i >= it.n) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (j + e >= it.l) continue;
+                        const long long at = mat * it.ps[0] + i * it.ps[1] + (j + e) * it.ps[2];
+                        const float before = it.decay != 0.0f ? it.decay * mu_load(it.p, at, it.p_type) : 0.0f;
+                        mu_store(it.p, at, it.p_type, before + it.alpha * (&v.x)[e]);
+                    }
+                } else {
+                    mu_h4 h4, l4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        mu_h hi, lo;
+                        mu_split((&v.x)[e], hi, lo);
+                        h4[e] = hi, l4[e] = lo;
+                    }
+                    if (MODE != MU_POLY) *old = v; // B is a factor only
+                    *(mu_h4 *)(out + (size_t)i * ld + j) = h4;
+                    *(mu_h4 *)(out + plane + (size_t)i * ld + j) = l4;
+                    if (mirror) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            out_t[(size_t)(j + e) * it.np + i] = h4[e];
+                            out_t[plane + (size_t)(j + e) * it.np + i] = l4[e];
+                        }
+                    }
+                }
+            }
+}
+
+template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
+{
+    auto tiles = [&](int T, bool keep) {
+        long long sum = 0;
+        for (int k = 0; k < a.n_items; ++k) {
+            if (keep) a.start[k] = (int)sum;
+            const long long ti = (a.it[k].np + T - 1) / T, tj = (a.it[k].lp + T - 1) / T;
+            sum += a.it[k].count * (MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2);
+        }
+        if (keep) a.start[a.n_items] = (int)sum;
+        return sum;
+    };
+    // the largest tile that still gives most of the 256 CUs one: a larger tile loads less for each product
+    const int T = MODE != MU_LAST && tiles(256, false) >= 200 ? 256 : tiles(128, false) >= 200 ? 128 : 64;
+    const long long total = tiles(T, true);
+    const dim3 grid((unsigned)((total + 7) / 8 * 8));
+    if (T == 256) hipLaunchKernelGGL((mu_product_kernel<256, 2, 4, MODE == MU_LAST ? MU_APPLY : MODE>), grid, dim3(512), 0, st, a);
+    else if (T == 128) hipLaunchKernelGGL((mu_product_kernel<128, 2, 2, MODE>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mu_product_kernel<64, 2, 2, MODE>), grid, dim3(256), 0, st, a);
+}
+
+// A run of items (or of some matrices of one) that fits the descriptors and MU_WS_MOST bytes, and what it takes.
+#define MU_WS_MOST (4ull << 30)
+#define MU_MATS_MOST 4096
+struct mu_group {
+    mu_args a;
+    int mats;
+    long long tiles;
+    uint64_t planes;
+    uint64_t bytes() const
+    {
+        return planes + ((uint64_t)mats * 8 + 255) / 256 * 256 + ((uint64_t)tiles * 8 + 255) / 256 * 256 +
+               ((uint64_t)mats * MU_STEPS * MU_COEF * 4 + 255) / 256 * 256;
+    }
+};
+
+// Calls `go(group)` for each group of the list in turn; stops at its first non-zero answer.
+template <typename F> static int mu_each_group(const lrb_muon_item *items, int n_items, F go)
+{
+    mu_group gr = {};
+    for (int k = 0; k < n_items; ++k) {
+        const lrb_muon_item &s = items[k];
+        if (s.count <= 0 || s.rows <= 0 || s.cols <= 0) continue;
+        for (int64_t done = 0; done < s.count;) {
+            mu_item it = {};
+            const bool turned = s.rows > s.cols;
+            it.n = (int)(turned ? s.cols : s.rows), it.l = (int)(turned ? s.rows : s.cols);
+            it.np = (it.n + 63) / 64 * 64, it.lp = (it.l + 63) / 64 * 64;
+            it.step = mu_bytes(it);
+            const long long per = (long long)(it.np / 64) * (it.lp / 64);
+            uint64_t room = gr.planes < MU_WS_MOST ? (MU_WS_MOST - gr.planes) / it.step : 0;
+            if (room == 0 && gr.a.n_items == 0) room = 1;
+            if (room > (uint64_t)(MU_MATS_MOST - gr.mats)) room = MU_MATS_MOST - gr.mats;
+            if (per * (long long)room > (1 << 28) - gr.tiles && room > 1) room = ((1 << 28) - gr.tiles) / per;
+            if (room == 0 || gr.a.n_items == MU_ITEMS) {
+                if (int rc = go(gr)) return rc;
+                gr = {};
+                continue;
+            }
+            it.count = (int)(s.count - done < (int64_t)room ? s.count - done : (int64_t)room);
+            const int size_p = s.p_type == LRB_F32 ? 4 : 2, size_g = s.g_type == LRB_F32 ? 4 : 2, size_m = s.m_type == LRB_F32 ? 4 : 2;
+            it.p = (char *)s.p + done * s.p_stride[0] * size_p;
+            it.g = (const char *)s.g + done * s.g_stride[0] * size_g;
+            it.m = s.m ? (char *)s.m + done * s.m_stride[0] * size_m : nullptr;
+            for (int d = 0; d < 3; ++d) {
+                const int from = d && turned ? 3 - d : d;
+                it.ps[d] = s.p_stride[from], it.gs[d] = s.g_stride[from], it.ms[d] = s.m_stride[from];
+            }
+            it.p_type = s.p_type, it.g_type = s.g_type, it.m_type = s.m_type;
+            it.alpha = s.alpha, it.decay = s.decay;
+            it.off = gr.planes, it.first = gr.mats;
+            gr.a.start[gr.a.n_items] = (int)gr.tiles;
+            gr.a.it[gr.a.n_items++] = it;
+            gr.planes += it.step * it.count, gr.mats += it.count, gr.tiles += per * it.count;
+            gr.a.start[gr.a.n_items] = (int)gr.tiles;
+            done += it.count;
+        }
+    }
+    return gr.a.n_items ? go(gr) : LRB_OK;
+}
+
+static bool mu_items_fit(const lrb_muon_item *items, int n)
+{
+    for (int k = 0; k < n; ++k) {
+        const lrb_muon_item &s = items[k];
+        if (s.count < 0 || s.rows < 0 || s.cols < 0) return false;
+        if (s.count == 0 || s.rows == 0 || s.cols == 0) continue;
+        // a side below 2^24 and planes below 2^31 entries: the kernels' 32-bit indices hold
+        if (s.rows > (1 << 24) || s.cols > (1 << 24) || (s.rows + 63) * (s.cols + 63) > INT_MAX) return false;
+        if (!s.p || !s.g || s.p_type < LRB_F32 || s.p_type > LRB_F16 || s.g_type < LRB_F32 || s.g_type > LRB_F16) return false;
+        if (s.m && (s.m_type < LRB_F32 || s.m_type > LRB_F16)) return false;
+    }
+    return true;
+}
+
+extern "C" double lrb_muon_bound(int steps, float a, float b, float c)
+{
+    double r = 1.0, most = 1.0;
+    for (int k = 0; k < steps && k < MU_STEPS && r <= 1e9; ++k) {
+        r = mu_largest_odd(a, b, c, r);
+        most = most >= r ? most : r; // a NaN stays
+    }
+    return most;
+}
+
+extern "C" uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items)
+{
+    if (n_items <= 0 || !items || !mu_items_fit(items, n_items)) return 0;
+    uint64_t most = 0;
+    mu_each_group(items, n_items, [&](mu_group &gr) {
+        if (gr.bytes() > most) most = gr.bytes();
+        return LRB_OK;
+    });
+    return most;
+}
+
+extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items, int n_items, float momentum, int nesterov, int steps,
+                            float a, float b, float c, float eps, void *d_ws, uint64_t ws_bytes)
+{
+    ARG_TRY(n_items >= 0 && (n_items == 0 || items != nullptr));
+    ARG_TRY(steps >= 1 && steps <= MU_STEPS && eps >= 0.0f);
+    ARG_TRY(lrb_muon_bound(steps, a, b, c) <= LRB_MUON_DIVERGED);
+    ARG_TRY(mu_items_fit(items, n_items));
+    const uint64_t need = lrb_muon_ws_bytes(items, n_items);
+    if (need == 0) return LRB_OK;
+    ARG_TRY(d_ws != nullptr && ws_bytes >= need && ((uintptr_t)d_ws & 255) == 0);
+    lrb_on_device on(device);
+    HIP_TRY(on.err);
+    hipStream_t st = (hipStream_t)stream;
+    return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
+        mu_args &g = gr.a;
+        g.ws = (char *)d_ws;
+        char *at = g.ws + gr.planes;
+        g.x0 = (double *)at, at += ((uint64_t)gr.mats * 8 + 255) / 256 * 256;
+        g.part = (double *)at, at += ((uint64_t)gr.tiles * 8 + 255) / 256 * 256;
+        g.table = (float *)at;
+        g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
+        hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
+        hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
+        hipLaunchKernelGGL(mu_split_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
+        for (int s = 0; s < steps; ++s) {
+            g.step = s;
+            mu_launch_product<MU_GRAM>(g, st);
+            mu_launch_product<MU_POLY>(g, st);
+            if (s + 1 < steps) mu_launch_product<MU_APPLY>(g, st);
+            else mu_launch_product<MU_LAST>(g, st);
+            g.flip ^= 1;
+        }
+        HIP_TRY(hipGetLastError());
+        return LRB_OK;
+    });
+}

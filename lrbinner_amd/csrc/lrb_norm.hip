@@ -1,0 +1,565 @@
+// lrb_norm.hip -- K9: layer normalisation over the last axis, forward and backward, gfx950 only.
+//
+//   u   = x, or keep * keep_scale * leaky_relu(x)             (what follows a linear layer in a block)
+//   y   = hat * w + b,  hat = (u - mean) * rstd,  rstd = 1 / sqrt(mean((u - mean)^2) + eps)
+//   g   = dy * w
+//   du  = rstd * (g - mean(g) - hat * mean(g * hat)),  dx = du * du/dx
+//   dw  = sum over rows of dy * hat,  db = sum over rows of dy
+//
+// Bound: memory.  A row is read once and stays in registers between its reductions (the mean first, then the mean of the
+// squared differences: no cancellation of large squares), so a forward pass moves x and y and a backward pass x, dy and dx.
+// TPR threads take a row, each `C` chunks of 16 bytes; the same thread meets the same columns in every row it visits, so
+// w and b are loaded once per thread and the weight's gradient is summed in registers: one partial row per workgroup is
+// written and a second kernel adds the partial rows in a fixed order (no atomics: the same bits run after run).
+// Everything between load and store is float32.
+#include <limits.h>
+
+#include "lrb_device.h"
+
+#define LN_MAX_GROUPS 1024 // workgroups of a pass: four a CU; also the largest number of partial rows of dw, db
+
+template <typename T> struct ln_vec {
+    static constexpr int V = 16 / (int)sizeof(T);
+};
+
+struct ln_args {
+    const void *x, *w, *b, *dy;
+    const uint8_t *keep;
+    void *y, *dx;
+    float *mean, *rstd; // written by the forward pass where not null, read by the backward pass
+    float *part;        // [groups][2][cols]
+    long long x_stride, dy_stride;
+    long long rows;
+    int cols;
+    int w_f32; // w, b (and dw, db) are float32, else of x's type
+    float eps, slope, keep_scale;
+};
+
+// V elements from column `col` on as float; columns past the end read as 0.  Rows need only their element's alignment:
+// global loads of this target take any address.
+template <typename T, int V> __device__ __forceinline__ void ln_load(const T *__restrict__ p, int col, int cols, float (&o)[V])
+{
+    if (col + V <= cols) {
+        T t[V];
+        __builtin_memcpy(t, p + col, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = (float)t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = col + i < cols ? (float)p[col + i] : 0.0f;
+    }
+}
+
+template <typename T, int V> __device__ __forceinline__ void ln_store(T *__restrict__ p, int col, int cols, const float (&o)[V])
+{
+    if (col + V <= cols) {
+        T t[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = (T)o[i];
+        __builtin_memcpy(p + col, t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (col + i < cols) p[col + i] = (T)o[i];
+    }
+}
+
+template <typename T, int V> __device__ __forceinline__ void ln_load_w(const void *w, int w_f32, int col, int cols, float dflt, float (&o)[V])
+{
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = dflt;
+    } else if (w_f32) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = col + i < cols ? ((const float *)w)[col + i] : 0.0f;
+    } else {
+        ln_load<T, V>((const T *)w, col, cols, o);
+    }
+}
+
+// keep_scale where an element is kept, 0 where it is dropped (its value then never enters, whatever it is)
+template <int V> __device__ __forceinline__ void ln_load_keep(const uint8_t *__restrict__ p, int col, int cols, float scale, float (&o)[V])
+{
+    uint8_t t[V];
+    if (col + V <= cols) {
+        __builtin_memcpy(t, p + col, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = col + i < cols ? p[col + i] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = t[i] ? scale : 0.0f;
+}
+
+// u of the block's activation; k: keep_scale or 0
+__device__ __forceinline__ float ln_act(float x, float slope, float k) { return k == 0.0f ? 0.0f : x * (x > 0.0f ? k : slope * k); }
+
+// The sum over the TPR threads of a row, in every one of them.  `red`: 2 x (TPR / 64) floats of the workgroup, used in turn
+// (`flip`) so that one barrier a reduction is enough.
+template <int TPR> __device__ __forceinline__ float ln_sum(float v, float *red, int &flip)
+{
+    constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        float *r = red + flip * NW;
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+        lrb_barrier();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) v += r[i];
+    }
+    return v;
+}
+
+// two sums behind one barrier; `red`: 4 x (TPR / 64) floats
+template <int TPR> __device__ __forceinline__ void ln_sum2(float &v, float &w, float *red, int &flip)
+{
+    constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+        v += __shfl_xor(v, o, 64);
+        w += __shfl_xor(w, o, 64);
+    }
+    if (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        float *r = red + flip * 2 * NW;
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0) {
+            r[threadIdx.x >> 6] = v;
+            r[NW + (threadIdx.x >> 6)] = w;
+        }
+        lrb_barrier();
+        v = w = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            v += r[i];
+            w += r[NW + i];
+        }
+    }
+}
+
+template <typename T, int TPR, int C, bool ACT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_fwd_kernel(ln_args a)
+{
+    constexpr int V = ln_vec<T>::V, THREADS = TPR < 256 ? 256 : TPR, RPG = THREADS / TPR;
+    __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
+    int flip = 0;
+    const int lane = threadIdx.x % TPR, cols = a.cols;
+    const float inv = 1.0f / (float)cols;
+    float w[C][V], b[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        ln_load_w<T, V>(a.w, a.w_f32, (c * TPR + lane) * V, cols, 1.0f, w[c]);
+        ln_load_w<T, V>(a.b, a.w_f32, (c * TPR + lane) * V, cols, 0.0f, b[c]);
+    }
+    // every thread of a workgroup makes the same number of turns (the reductions hold barriers); rows past the end are
+    // taken as row `rows - 1` and not written
+    const long long turns = (a.rows + RPG - 1) / RPG;
+    for (long long t = blockIdx.x; t < turns; t += gridDim.x) {
+        long long row = t * RPG + threadIdx.x / TPR;
+        const bool live = row < a.rows;
+        if (!live) row = a.rows - 1;
+        const T *x = (const T *)a.x + row * a.x_stride;
+        float u[C][V];
+        float s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) ln_load<T, V>(x, (c * TPR + lane) * V, cols, u[c]);
+        if (ACT) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float k[V];
+                if (a.keep) {
+                    ln_load_keep<V>(a.keep + row * cols, (c * TPR + lane) * V, cols, a.keep_scale, k);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) k[i] = a.keep_scale;
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) u[c][i] = ln_act(u[c][i], a.slope, k[i]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += u[c][i];
+        const float mean = ln_sum<TPR>(s, red, flip) * inv;
+        s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float e = u[c][i] - mean;
+                s += (c * TPR + lane) * V + i < cols ? e * e : 0.0f;
+            }
+        const float rstd = 1.0f / sqrtf(ln_sum<TPR>(s, red, flip) * inv + a.eps);
+        if (!live) continue;
+        if (a.mean && lane == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        T *y = (T *)a.y + row * cols;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = (u[c][i] - mean) * rstd * w[c][i] + b[c][i];
+            ln_store<T, V>(y, (c * TPR + lane) * V, cols, o);
+        }
+    }
+}
+
+template <typename T, int TPR, int C, bool ACT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_bwd_kernel(ln_args a)
+{
+    constexpr int V = ln_vec<T>::V, THREADS = TPR < 256 ? 256 : TPR, RPG = THREADS / TPR;
+    __shared__ float red[4 * (TPR > 64 ? TPR / 64 : 1)];
+    int flip = 0;
+    const int lane = threadIdx.x % TPR, cols = a.cols;
+    const float inv = 1.0f / (float)cols;
+    float w[C][V], dw[C][V], db[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        ln_load_w<T, V>(a.w, a.w_f32, (c * TPR + lane) * V, cols, 1.0f, w[c]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[c][i] = db[c][i] = 0.0f;
+    }
+    const long long turns = (a.rows + RPG - 1) / RPG;
+    for (long long t = blockIdx.x; t < turns; t += gridDim.x) {
+        long long row = t * RPG + threadIdx.x / TPR;
+        const bool live = row < a.rows;
+        if (!live) row = a.rows - 1;
+        const T *x = (const T *)a.x + row * a.x_stride, *dy = (const T *)a.dy + row * a.dy_stride;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float hat[C][V], g[C][V];
+        uint32_t kept = 0, above = 0; // a bit an element: kept, and above 0
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            ln_load<T, V>(x, (c * TPR + lane) * V, cols, hat[c]);
+            ln_load<T, V>(dy, (c * TPR + lane) * V, cols, g[c]);
+        }
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float k[V];
+            if (ACT) {
+                if (a.keep) {
+                    ln_load_keep<V>(a.keep + row * cols, (c * TPR + lane) * V, cols, a.keep_scale, k);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) k[i] = a.keep_scale;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                // dy is 0 past the end, so nothing there enters a sum
+                if (ACT) {
+                    kept |= (uint32_t)(k[i] != 0.0f) << (c * V + i);
+                    above |= (uint32_t)(hat[c][i] > 0.0f) << (c * V + i);
+                    hat[c][i] = ln_act(hat[c][i], a.slope, k[i]);
+                }
+                hat[c][i] = (hat[c][i] - mean) * rstd;
+                if (live) {
+                    dw[c][i] += g[c][i] * hat[c][i];
+                    db[c][i] += g[c][i];
+                }
+                g[c][i] *= w[c][i];
+                s1 += g[c][i];
+                s2 += g[c][i] * hat[c][i];
+            }
+        }
+        if (!a.dx) continue;
+        ln_sum2<TPR>(s1, s2, red, flip);
+        s1 *= inv, s2 *= inv;
+        if (!live) continue;
+        T *dx = (T *)a.dx + row * cols;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                o[i] = (g[c][i] - s1 - hat[c][i] * s2) * rstd;
+                if (ACT)
+                    o[i] = !(kept >> (c * V + i) & 1) ? 0.0f : o[i] * (above >> (c * V + i) & 1 ? a.keep_scale : a.slope * a.keep_scale);
+            }
+            ln_store<T, V>(dx, (c * TPR + lane) * V, cols, o);
+        }
+    }
+    if (!a.part) return;
+    float *part = a.part + (size_t)blockIdx.x * 2 * cols;
+    if (RPG == 1) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            ln_store<float, V>(part, (c * TPR + lane) * V, cols, dw[c]);
+            ln_store<float, V>(part + cols, (c * TPR + lane) * V, cols, db[c]);
+        }
+    } else {
+        // the rows that the workgroup's teams took side by side are added up in LDS, team 0 first
+        __shared__ float acc[RPG > 1 ? RPG * TPR * C * V : 1];
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            lrb_barrier();
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    acc[(threadIdx.x / TPR) * (TPR * C * V) + (c * TPR + lane) * V + i] = which ? db[c][i] : dw[c][i];
+            lrb_barrier();
+            for (int col = threadIdx.x; col < cols; col += THREADS) {
+                float s = 0.0f;
+#pragma unroll
+                for (int r = 0; r < RPG; ++r) s += acc[r * (TPR * C * V) + col];
+                part[(size_t)which * cols + col] = s;
+            }
+        }
+    }
+}
+
+// Rows too long for the registers of a workgroup: the row is read again for each of its passes (it fits the L2).
+template <typename T, bool ACT> __device__ __forceinline__ float ln_at(const ln_args &a, const T *x, long long row, int col, float &f)
+{
+    const float v = (float)x[col];
+    if (!ACT) return v;
+    const float k = a.keep ? (a.keep[row * a.cols + col] ? a.keep_scale : 0.0f) : a.keep_scale;
+    f = v > 0.0f ? k : a.slope * k; // du/dx
+    return ln_act(v, a.slope, k);
+}
+
+__device__ __forceinline__ float ln_w_at(const void *w, int w_f32, int col, float dflt, const float *) { return w ? ((const float *)w)[col] : dflt; }
+template <typename T> __device__ __forceinline__ float ln_w_at(const void *w, int w_f32, int col, float dflt, const T *)
+{
+    return !w ? dflt : w_f32 ? ((const float *)w)[col] : (float)((const T *)w)[col];
+}
+
+template <typename T, bool ACT> __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(ln_args a)
+{
+    __shared__ float red[32];
+    int flip = 0;
+    const float inv = 1.0f / (float)a.cols;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.x_stride;
+        float s = 0.0f, f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) s += ln_at<T, ACT>(a, x, row, c, f);
+        const float mean = ln_sum<1024>(s, red, flip) * inv;
+        s = 0.0f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float e = ln_at<T, ACT>(a, x, row, c, f) - mean;
+            s += e * e;
+        }
+        const float rstd = 1.0f / sqrtf(ln_sum<1024>(s, red, flip) * inv + a.eps);
+        if (a.mean && threadIdx.x == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        T *y = (T *)a.y + row * a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += 1024)
+            y[c] = (T)((ln_at<T, ACT>(a, x, row, c, f) - mean) * rstd * ln_w_at(a.w, a.w_f32, c, 1.0f, (const T *)nullptr) +
+                       ln_w_at(a.b, a.w_f32, c, 0.0f, (const T *)nullptr));
+    }
+}
+
+template <typename T, bool ACT> __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(ln_args a)
+{
+    __shared__ float red[64];
+    int flip = 0;
+    const float inv = 1.0f / (float)a.cols;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.x_stride, *dy = (const T *)a.dy + row * a.dy_stride;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s1 = 0.0f, s2 = 0.0f, f = 1.0f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float g = (float)dy[c] * ln_w_at(a.w, a.w_f32, c, 1.0f, (const T *)nullptr);
+            s1 += g;
+            s2 += g * ((ln_at<T, ACT>(a, x, row, c, f) - mean) * rstd);
+        }
+        ln_sum2<1024>(s1, s2, red, flip);
+        s1 *= inv, s2 *= inv;
+        T *dx = (T *)a.dx + row * a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float g = (float)dy[c] * ln_w_at(a.w, a.w_f32, c, 1.0f, (const T *)nullptr);
+            const float hat = (ln_at<T, ACT>(a, x, row, c, f) - mean) * rstd;
+            float o = (g - s1 - hat * s2) * rstd;
+            if (ACT) o = f == 0.0f ? 0.0f : o * f;
+            dx[c] = (T)o;
+        }
+    }
+}
+
+// dw, db partial rows of long rows: a thread a column, blockIdx.y a slice of the rows
+template <typename T, bool ACT> __global__ __launch_bounds__(256) void ln_cols_long_kernel(ln_args a)
+{
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.cols) return;
+    float dw = 0.0f, db = 0.0f, f;
+    for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const float d = (float)((const T *)a.dy)[row * a.dy_stride + c];
+        dw += d * ((ln_at<T, ACT>(a, (const T *)a.x + row * a.x_stride, row, c, f) - a.mean[row]) * a.rstd[row]);
+        db += d;
+    }
+    a.part[(size_t)blockIdx.y * 2 * a.cols + c] = dw;
+    a.part[(size_t)blockIdx.y * 2 * a.cols + a.cols + c] = db;
+}
+
+// dw[col], db[col] = the partial rows' sums: 32 columns a workgroup, 32 slices of the partial rows side by side
+template <typename W> __global__ __launch_bounds__(1024) void ln_join_kernel(const float *__restrict__ part, int groups, int cols, W *__restrict__ dw, W *__restrict__ db)
+{
+    __shared__ float acc[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, col = blockIdx.x * 32 + x;
+    W *out = blockIdx.y ? db : dw;
+    if (!out) return;
+    float s = 0.0f;
+    if (col < cols)
+        for (int g = y; g < groups; g += 32) s += part[((size_t)g * 2 + blockIdx.y) * cols + col];
+    acc[y][x] = s;
+    lrb_barrier();
+    if (y == 0 && col < cols) {
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += acc[i][x];
+        out[col] = (W)s;
+    }
+}
+
+// How a row is laid over threads: 16, 64, 256 or 1024 of them by its length, at most 16 elements each (registers: a backward
+// pass holds five float32 for each, and 1024 threads have 128 registers each).  Rows longer than 16,384, or than 8,192 in a
+// backward pass with an activation (its bits would spill): the _long_ kernels.
+static int ln_threads(long long cols, int V)
+{
+    return cols <= 16 * 2 * V ? 16 : cols <= 64 * 16 ? 64 : cols <= 256 * 16 ? 256 : 1024;
+}
+
+static bool ln_is_long(long long cols, bool act_bwd) { return cols > 1024 * (act_bwd ? 8 : 16); }
+
+static int ln_groups(long long rows, long long cols, int V, bool act_bwd)
+{
+    if (ln_is_long(cols, act_bwd)) return (int)(rows < 64 ? (rows ? rows : 1) : 64);
+    const int tpr = ln_threads(cols, V), rpg = tpr < 256 ? 256 / tpr : 1;
+    const long long turns = (rows + rpg - 1) / rpg;
+    return (int)(turns < LN_MAX_GROUPS ? (turns ? turns : 1) : LN_MAX_GROUPS);
+}
+
+template <typename T, bool ACT> static void ln_launch_fwd(const ln_args &a, hipStream_t st)
+{
+    constexpr int V = ln_vec<T>::V;
+    if (ln_is_long(a.cols, false)) {
+        hipLaunchKernelGGL((ln_fwd_long_kernel<T, ACT>), dim3((unsigned)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
+        return;
+    }
+    const int tpr = ln_threads(a.cols, V), c = (a.cols + tpr * V - 1) / (tpr * V);
+    const dim3 grid(ln_groups(a.rows, a.cols, V, false));
+#define LN_GO(TPR, C) hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, C, ACT>), grid, dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+#define LN_BY_C(TPR)              \
+    if (c == 1) LN_GO(TPR, 1);    \
+    else if (c == 2) LN_GO(TPR, 2); \
+    else LN_GO(TPR, (V == 4 ? 4 : 2))
+    if (tpr == 16) {
+        if (c == 1) LN_GO(16, 1);
+        else LN_GO(16, 2);
+    } else if (tpr == 64) {
+        LN_BY_C(64);
+    } else if (tpr == 256) {
+        LN_BY_C(256);
+    } else {
+        LN_BY_C(1024);
+    }
+#undef LN_BY_C
+#undef LN_GO
+}
+
+template <typename T, bool ACT> static void ln_launch_bwd(const ln_args &a, hipStream_t st)
+{
+    constexpr int V = ln_vec<T>::V;
+    if (ln_is_long(a.cols, ACT)) {
+        if (a.dx && a.rows) hipLaunchKernelGGL((ln_bwd_long_kernel<T, ACT>), dim3((unsigned)(a.rows < 2048 ? a.rows : 2048)), dim3(1024), 0, st, a);
+        if (a.part)
+            hipLaunchKernelGGL((ln_cols_long_kernel<T, ACT>), dim3((a.cols + 255) / 256, ln_groups(a.rows, a.cols, V, ACT)), dim3(256), 0, st, a);
+        return;
+    }
+    const int tpr = ln_threads(a.cols, V), c = (a.cols + tpr * V - 1) / (tpr * V);
+    const dim3 grid(ln_groups(a.rows, a.cols, V, ACT));
+#define LN_GO(TPR, C) hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, C, ACT>), grid, dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+#define LN_BY_C(TPR)              \
+    if (c == 1) LN_GO(TPR, 1);    \
+    else if (c == 2) LN_GO(TPR, 2); \
+    else LN_GO(TPR, (V == 4 ? 4 : 2))
+    if (tpr == 16) {
+        if (c == 1) LN_GO(16, 1);
+        else LN_GO(16, 2);
+    } else if (tpr == 64) {
+        LN_BY_C(64);
+    } else if (tpr == 256) {
+        LN_BY_C(256);
+    } else {
+        constexpr int MOST = (ACT ? 8 : 16) / V, HALF = MOST > 1 ? MOST / 2 : 1;
+        if (c <= HALF) LN_GO(1024, HALF);
+        else LN_GO(1024, MOST);
+    }
+#undef LN_BY_C
+#undef LN_GO
+}
+
+extern "C" int lrb_layer_norm_fwd_dev(int device, void *stream, int x_type, int w_type, uint64_t rows, uint64_t cols, const void *d_x,
+                                      int64_t x_stride, const void *d_w, const void *d_b, float eps, float slope, const uint8_t *d_keep,
+                                      float keep_scale, void *d_y, float *d_mean, float *d_rstd)
+{
+    ARG_TRY(x_type >= LRB_F32 && x_type <= LRB_F16 && (w_type == LRB_F32 || w_type == x_type));
+    ARG_TRY(cols >= 1 && cols <= INT_MAX / 4 && rows <= (1ull << 40));
+    ARG_TRY((d_mean == nullptr) == (d_rstd == nullptr));
+    if (rows == 0) return LRB_OK;
+    ARG_TRY(d_x != nullptr && d_y != nullptr);
+    lrb_on_device on(device);
+    HIP_TRY(on.err);
+    ln_args a = {};
+    a.x = d_x, a.w = d_w, a.b = d_b, a.keep = d_keep, a.y = d_y, a.mean = d_mean, a.rstd = d_rstd;
+    a.x_stride = x_stride, a.rows = (long long)rows, a.cols = (int)cols, a.w_f32 = w_type == LRB_F32;
+    a.eps = eps, a.slope = slope, a.keep_scale = d_keep ? keep_scale : 1.0f;
+    const bool act = d_keep || slope != 1.0f;
+    hipStream_t st = (hipStream_t)stream;
+    if (x_type == LRB_F32) act ? ln_launch_fwd<float, true>(a, st) : ln_launch_fwd<float, false>(a, st);
+    else if (x_type == LRB_BF16) act ? ln_launch_fwd<__bf16, true>(a, st) : ln_launch_fwd<__bf16, false>(a, st);
+    else act ? ln_launch_fwd<_Float16, true>(a, st) : ln_launch_fwd<_Float16, false>(a, st);
+    HIP_TRY(hipGetLastError());
+    return LRB_OK;
+}
+
+extern "C" uint64_t lrb_layer_norm_bwd_ws_bytes(int x_type, uint64_t rows, uint64_t cols)
+{
+    if (x_type < LRB_F32 || x_type > LRB_F16 || cols > INT_MAX / 4 || rows > (1ull << 40)) return 0;
+    return (uint64_t)ln_groups((long long)rows, (long long)cols, x_type == LRB_F32 ? 4 : 8, false) * 2 * cols * sizeof(float);
+}
+
+extern "C" int lrb_layer_norm_bwd_dev(int device, void *stream, int x_type, int w_type, uint64_t rows, uint64_t cols, const void *d_x,
+                                      int64_t x_stride, const void *d_dy, int64_t dy_stride, const void *d_w, const float *d_mean,
+                                      const float *d_rstd, float slope, const uint8_t *d_keep, float keep_scale, void *d_dx, void *d_dw,
+                                      void *d_db, void *d_ws, uint64_t ws_bytes)
+{
+    ARG_TRY(x_type >= LRB_F32 && x_type <= LRB_F16 && (w_type == LRB_F32 || w_type == x_type));
+    ARG_TRY(cols >= 1 && cols <= INT_MAX / 4 && rows <= (1ull << 40));
+    const bool sums = d_dw || d_db;
+    ARG_TRY(!sums || (d_ws != nullptr && ws_bytes >= lrb_layer_norm_bwd_ws_bytes(x_type, rows, cols)));
+    ARG_TRY(rows == 0 || (d_x != nullptr && d_dy != nullptr && d_mean != nullptr && d_rstd != nullptr));
+    if (!sums && (!d_dx || rows == 0)) return LRB_OK;
+    lrb_on_device on(device);
+    HIP_TRY(on.err);
+    ln_args a = {};
+    a.x = d_x, a.dy = d_dy, a.w = d_w, a.keep = d_keep, a.dx = d_dx, a.mean = (float *)d_mean, a.rstd = (float *)d_rstd;
+    a.part = sums ? (float *)d_ws : nullptr;
+    a.x_stride = x_stride, a.dy_stride = dy_stride, a.rows = (long long)rows, a.cols = (int)cols, a.w_f32 = w_type == LRB_F32;
+    a.slope = slope, a.keep_scale = d_keep ? keep_scale : 1.0f;
+    const bool act = d_keep || slope != 1.0f;
+    hipStream_t st = (hipStream_t)stream;
+    if (x_type == LRB_F32) act ? ln_launch_bwd<float, true>(a, st) : ln_launch_bwd<float, false>(a, st);
+    else if (x_type == LRB_BF16) act ? ln_launch_bwd<__bf16, true>(a, st) : ln_launch_bwd<__bf16, false>(a, st);
+    else act ? ln_launch_bwd<_Float16, true>(a, st) : ln_launch_bwd<_Float16, false>(a, st);
+    if (sums) {
+        const int groups = ln_groups(a.rows, a.cols, x_type == LRB_F32 ? 4 : 8, act);
+        const dim3 grid((a.cols + 31) / 32, 2);
+        if (w_type == LRB_F32) hipLaunchKernelGGL((ln_join_kernel<float>), grid, dim3(1024), 0, st, (const float *)d_ws, groups, a.cols, (float *)d_dw, (float *)d_db);
+        else if (w_type == LRB_BF16) hipLaunchKernelGGL((ln_join_kernel<__bf16>), grid, dim3(1024), 0, st, (const float *)d_ws, groups, a.cols, (__bf16 *)d_dw, (__bf16 *)d_db);
+        else hipLaunchKernelGGL((ln_join_kernel<_Float16>), grid, dim3(1024), 0, st, (const float *)d_ws, groups, a.cols, (_Float16 *)d_dw, (_Float16 *)d_db);
+    }
+    HIP_TRY(hipGetLastError());
+    return LRB_OK;
+}

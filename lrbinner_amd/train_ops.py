@@ -1,0 +1,385 @@
+"""Operators of a network's training on torch tensors: layer normalisation (K9) and the orthogonalised update (K10).
+
+``layer_norm`` / ``LayerNorm`` normalise the rows of a tensor, with the LeakyReLU and the dropout that stand before a norm
+in this package's blocks folded in, and give the gradients of input, weight and bias.  ``orthogonalize`` moves the
+singular values of a matrix towards 1 by a polynomial iteration, ``muon_step`` takes an optimiser's step with it for a list
+of weights (momentum, iteration and update in shared launches), and ``Muon`` is that as a ``torch.optim.Optimizer``.
+
+On the GPU the arithmetic is csrc/lrb_norm.hip and csrc/lrb_muon.hip behind the C ABI of include/lrb_hip.h; calls go to
+torch's current stream of the tensors' device, their workspace comes from torch's allocator (so calls may be captured in a
+HIP graph), and there is no fallback where the library is missing.  On CPU tensors the same definitions run as torch
+operations, as the network itself does without ``--cuda``.
+
+Float32, bfloat16 and float16; what is summed is summed in float32 or more, and results are rounded once."""
+import ctypes as C
+import math
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import call, check
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # LRB_F32, LRB_BF16, LRB_F16
+#: of the odd quintic a x + b x^3 + c x^5 that ``orthogonalize`` iterates on the singular values
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _known_type(t, name):
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name}: float32, bfloat16 or float16 is wanted, not {t.dtype}")
+
+
+# ---- layer normalisation ----------------------------------------------------------------------
+
+def _rows(t, cols):
+    """t as rows x cols with the elements of a row side by side (a copy only where its strides allow no such view)."""
+    t = t.reshape(-1, cols)
+    return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, stats):
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        both = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean, rstd = both[0], both[1]
+    if rows:
+        x2 = _rows(x, cols)
+        ref = weight if weight is not None else bias
+        weight = weight if weight is None else weight.contiguous()
+        bias = bias if bias is None else bias.contiguous()
+        keep = keep if keep is None else keep.contiguous()
+        check("lrb_layer_norm_fwd_dev", _lib.lib().lrb_layer_norm_fwd_dev(
+            x.device.index, _stream(x.device), _TYPES[x.dtype], 0 if ref is None else _TYPES[ref.dtype], rows, cols,
+            x2.data_ptr(), x2.stride(0), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+            eps, slope, None if keep is None else keep.data_ptr(), keep_scale, y.data_ptr(),
+            mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None))
+    return y, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, keep, eps, slope, keep_scale):
+        y, mean, rstd = _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, True)
+        ctx.save_for_backward(x, weight, keep, mean, rstd)
+        ctx.bias_type = None if bias is None else bias.dtype
+        ctx.slope, ctx.keep_scale = slope, keep_scale
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, keep, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        cols = x.shape[-1]
+        rows = x.numel() // cols
+        w_type = weight.dtype if weight is not None else ctx.bias_type
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty(cols, dtype=w_type, device=x.device) if need_w else None
+        db = torch.empty(cols, dtype=w_type, device=x.device) if need_b else None
+        lib = _lib.lib()
+        ws, ws_bytes = None, 0
+        if need_w or need_b:
+            ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(_TYPES[x.dtype], rows, cols)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        x2, dy2 = _rows(x, cols), _rows(dy, cols)
+        weight = weight if weight is None else weight.contiguous()
+        keep = keep if keep is None else keep.contiguous()
+        check("lrb_layer_norm_bwd_dev", lib.lrb_layer_norm_bwd_dev(
+            x.device.index, _stream(x.device), _TYPES[x.dtype], 0 if w_type is None else _TYPES[w_type], rows, cols,
+            x2.data_ptr() if rows else None, x2.stride(0), dy2.data_ptr() if rows else None, dy2.stride(0),
+            None if weight is None else weight.data_ptr(), mean.data_ptr() if rows else None, rstd.data_ptr() if rows else None,
+            ctx.slope, None if keep is None or not rows else keep.data_ptr(), ctx.keep_scale,
+            dx.data_ptr() if need_x and rows else None, dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None,
+            None if ws is None else ws.data_ptr(), ws_bytes))
+        return dx, dw, db, None, None, None, None
+
+
+def _ln_plain(x, weight, bias, keep, eps, slope, keep_scale):
+    u = x.float()
+    if keep is not None or slope != 1.0:
+        u = torch.where(u > 0, u, slope * u)
+        if keep is not None:
+            u = torch.where(keep.bool(), u * keep_scale, torch.zeros_like(u))
+    centred = u - u.mean(-1, keepdim=True)
+    y = centred / torch.sqrt((centred * centred).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.float()
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(x.dtype)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, *, slope=1.0, keep=None, keep_scale=1.0):
+    """(u - mean(u)) / sqrt(var(u) + eps) * weight + bias over the last axis, in x's type, with gradients of x, weight and bias.
+
+    u is x, or with ``slope`` (of a LeakyReLU; 0 a ReLU) or ``keep`` (bool or uint8, of x's shape, a dropout's draw)
+    keep * keep_scale * leaky_relu(x); what is dropped counts as 0 whatever it holds.  ``weight`` and ``bias``: one element a
+    column, float32 or of x's type (both alike), or None.  x may have any leading axes and strides; a copy is made only
+    where the elements of a row are not side by side, or the rows not evenly spaced.  The statistics are float32."""
+    _known_type(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x: at least one column is wanted, not shape {tuple(x.shape)}")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps: {eps}")
+    if not (math.isfinite(slope) and math.isfinite(keep_scale)):
+        raise ValueError(f"slope {slope}, keep_scale {keep_scale}: finite numbers are wanted")
+    cols = x.shape[-1]
+    grad = x.requires_grad
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != cols:
+            raise ValueError(f"{name}: shape ({cols},) is wanted, not {tuple(t.shape)}")
+        if t.dtype != torch.float32 and t.dtype != x.dtype:
+            raise TypeError(f"{name}: float32 or {x.dtype} is wanted, not {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        grad = grad or t.requires_grad
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias: one type is wanted, not {weight.dtype} and {bias.dtype}")
+    if keep is not None:
+        if keep.shape != x.shape:
+            raise ValueError(f"keep: shape {tuple(x.shape)} is wanted, not {tuple(keep.shape)}")
+        if keep.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f"keep: bool or uint8 is wanted, not {keep.dtype}")
+        if keep.device != x.device:
+            raise ValueError(f"keep is on {keep.device}, x on {x.device}")
+    else:
+        keep_scale = 1.0
+    if not x.is_cuda:
+        return _ln_plain(x, weight, bias, keep, eps, slope, keep_scale)
+    if grad and torch.is_grad_enabled():
+        return _LayerNorm.apply(x, weight, bias, keep, eps, slope, keep_scale)
+    return _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, False)[0]
+
+
+class LayerNorm(torch.nn.Module):
+    """``layer_norm`` with a weight (ones) and a bias (zeros) of its own; ``slope``: of the LeakyReLU that stands before it."""
+
+    def __init__(self, cols, eps=1e-5, *, slope=1.0, device=None, dtype=None):
+        super().__init__()
+        self.eps, self.slope = eps, slope
+        self.weight = torch.nn.Parameter(torch.ones(cols, device=device, dtype=dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(cols, device=device, dtype=dtype))
+
+    def forward(self, x, keep=None, keep_scale=1.0):
+        return layer_norm(x, self.weight, self.bias, self.eps, slope=self.slope, keep=keep, keep_scale=keep_scale)
+
+    def extra_repr(self):
+        return f"{self.weight.numel()}, eps={self.eps}, slope={self.slope}"
+
+
+# ---- the orthogonalised update ------------------------------------------------------------------
+
+_ITEM = struct.Struct("=3Q9q3q3i2fi")  # lrb_muon_item
+_DIVERGED = 64.0                       # LRB_MUON_DIVERGED
+
+
+def _stack(t, name):
+    """t as matrices x rows x columns, without a copy."""
+    if t.dim() == 2:
+        return t.unsqueeze(0)
+    if t.dim() == 3:
+        return t
+    try:
+        return t.view(-1, t.shape[-2], t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{name}: the leading axes of shape {tuple(t.shape)}, strides {t.stride()} are not evenly spaced") from None
+
+
+def _written(t, name):
+    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} is written, but several of its elements share their memory (strides {t.stride()})")
+
+
+def _check_iteration(steps, coefficients, eps):
+    if int(steps) != steps or not 1 <= steps <= 32:
+        raise ValueError(f"steps: 1 to 32 is wanted, not {steps}")
+    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
+        raise ValueError(f"coefficients: three finite numbers are wanted, not {coefficients}")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps: {eps}")
+    if _lib.lib().lrb_muon_bound(int(steps), *coefficients) > _DIVERGED:
+        raise ValueError(f"coefficients {tuple(coefficients)}: a singular value may grow beyond {_DIVERGED:g} in {steps} steps")
+
+
+def _muon_call(device, items, momentum, nesterov, steps, coefficients, eps):
+    lib = _lib.lib()
+    raw = C.create_string_buffer(b"".join(items), _ITEM.size * len(items))
+    ws_bytes = lib.lrb_muon_ws_bytes(raw, len(items))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    a, b, c = coefficients
+    check("lrb_muon_dev", lib.lrb_muon_dev(device.index, _stream(device), raw, len(items), momentum, 1 if nesterov else 0, int(steps),
+                                           a, b, c, eps, ws.data_ptr() if ws_bytes else None, ws_bytes))
+
+
+def _orthogonal_plain(u, steps, coefficients, eps):
+    """In float32, whatever u's type; u: [..., rows, columns]."""
+    a, b, c = coefficients
+    x = u.float()
+    turned = x.shape[-2] > x.shape[-1]
+    x = x.transpose(-1, -2) if turned else x
+    x = x / torch.linalg.vector_norm(x, dim=(-2, -1), keepdim=True, dtype=torch.float64).clamp_min(eps).float()
+    for _ in range(int(steps)):
+        gram = x @ x.transpose(-1, -2)
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.transpose(-1, -2) if turned else x
+
+
+@torch.no_grad()
+def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
+    """g / max(|g|_F, eps), then ``steps`` times X <- a X + (b A + c A^2) X with A = X X^T (of a tall matrix X^T X): the singular
+    vectors stay, the singular values go towards 1 (with the default coefficients into about 0.7 to 1.2).  Coefficients under which a singular
+    value from [0, 1] may grow beyond 64 on the way are refused.
+
+    g: [..., rows, columns], any strides; each matrix by itself; one that holds an infinity or a NaN becomes NaN.
+    ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are as exact as
+    float32 ones for every type of g.  No gradient: an update is not differentiated."""
+    _known_type(g, "g")
+    if g.dim() < 2:
+        raise ValueError(f"g: a matrix is wanted, not shape {tuple(g.shape)}")
+    _check_iteration(steps, coefficients, eps)
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    else:
+        _known_type(out, "out")
+        if out.shape != g.shape or out.device != g.device:
+            raise ValueError(f"out: shape {tuple(g.shape)} on {g.device} is wanted, not {tuple(out.shape)} on {out.device}")
+        _written(out, "out")
+        if g.dim() > 3:
+            _stack(out, "out")
+    if g.numel() == 0:
+        return out
+    if not g.is_cuda:
+        return out.copy_(_orthogonal_plain(g, steps, coefficients, eps))
+    g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "g")
+    o3 = _stack(out, "out")
+    item = _ITEM.pack(o3.data_ptr(), g3.data_ptr(), 0, *o3.stride(), *g3.stride(), 0, 0, 0, *g3.shape,
+                      _TYPES[out.dtype], _TYPES[g.dtype], 0, 1.0, 0.0, 0)
+    _muon_call(g.device, [item], 0.0, False, steps, coefficients, eps)
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
+@torch.no_grad()
+def muon_step(params, grads, momenta=None, *, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+              coefficients=COEFFICIENTS, eps=1e-7, scale=None):
+    """One step of the orthogonalised momentum update on a list of weights, in place:
+
+        m <- momentum m + (1 - momentum) g;  u = (1 - momentum) g + momentum m  (nesterov; else m; g without ``momenta``)
+        p <- (1 - lr weight_decay) p - lr scale orthogonalize(u)
+
+    params, grads, momenta: lists of [..., rows, columns] of one device, each of its own type and strides (momenta best in
+    float32); leading axes are a stack of weights.  ``scale``: None for sqrt(max(1, rows / columns)), or a number.  The
+    weights of a list share their launches, so one call for all of a network's is best.  No two written tensors may overlap."""
+    params, grads = list(params), list(grads)
+    momenta = [None] * len(params) if momenta is None else list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(momenta)} momenta")
+    _check_iteration(steps, coefficients, eps)
+    for v, name in ((lr, "lr"), (momentum, "momentum"), (weight_decay, "weight_decay"), (0.0 if scale is None else scale, "scale")):
+        if not math.isfinite(v):
+            raise ValueError(f"{name}: {v}")
+    if not params:
+        return
+    device, seen = params[0].device, set()
+    for p, g, m in zip(params, grads, momenta):
+        for t, name in ((p, "params"), (g, "grads"), (m, "momenta")):
+            if t is None and name == "momenta":
+                continue
+            _known_type(t, name)
+            if t.dim() < 2 or t.shape != p.shape:
+                raise ValueError(f"{name}: a matrix, and the shape of its weight {tuple(p.shape)} is wanted, not {tuple(t.shape)}")
+            if t.device != device:
+                raise ValueError(f"{name}: one device is wanted, not {t.device} and {device}")
+            if name != "grads" and t.numel():
+                _written(t, name)
+                if t.data_ptr() in seen:
+                    raise ValueError(f"{name}: a tensor is listed twice")
+                seen.add(t.data_ptr())
+    if any(g.numel() and g.data_ptr() in seen for g in grads):
+        raise ValueError("grads: a tensor is among the written ones too")
+    decay = 1.0 - lr * weight_decay
+    if device.type != "cuda":
+        for p, g, m in zip(params, grads, momenta):
+            if not p.numel():
+                continue
+            u = g.float()
+            if m is not None:
+                m.copy_(momentum * m.float() + (1.0 - momentum) * u)
+                u = (1.0 - momentum) * u + momentum * m.float() if nesterov else m.float()
+            by = math.sqrt(max(1.0, p.shape[-2] / p.shape[-1])) if scale is None else scale
+            p.copy_(decay * p.float() - lr * by * _orthogonal_plain(u, steps, coefficients, eps))
+        return
+    items = []
+    for p, g, m in zip(params, grads, momenta):
+        if not p.numel():
+            continue
+        p3, m3 = _stack(p, "params"), None if m is None else _stack(m, "momenta")
+        g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "grads")
+        count, rows, cols = p3.shape
+        by = math.sqrt(max(1.0, rows / cols)) if scale is None else scale
+        items.append(_ITEM.pack(p3.data_ptr(), g3.data_ptr(), 0 if m is None else m3.data_ptr(), *p3.stride(), *g3.stride(),
+                                *((0, 0, 0) if m is None else m3.stride()), count, rows, cols, _TYPES[p.dtype], _TYPES[g.dtype],
+                                0 if m is None else _TYPES[m.dtype], -lr * by, decay, 0))
+    if items:
+        _muon_call(device, items, momentum, nesterov, steps, coefficients, eps)
+    torch.autograd.graph.increment_version([t for t in params + momenta if t is not None])
+
+
+class Muon(torch.optim.Optimizer):
+    """``muon_step`` over the parameters that have a gradient; matrices only (what has one axis wants another optimiser).
+
+    The momentum is held in float32.  A step may be captured in a HIP graph once one step has been taken: the buffers have
+    to be there before, and the learning rate of the capture stays."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+        _check_iteration(steps, coefficients, eps)
+        if not lr >= 0.0 or not 0.0 <= momentum < 1.0 or not weight_decay >= 0.0:
+            raise ValueError(f"lr {lr}, momentum {momentum}, weight_decay {weight_decay}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=tuple(coefficients), eps=eps))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                raise ValueError(f"Muon takes matrices, not a parameter of shape {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)  # casts the state to the parameters' type: the momentum stays float32
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+            if i in state_dict["state"]:
+                self.state[p]["momentum"] = state_dict["state"][i]["momentum"].to(device=p.device, dtype=torch.float32, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_device = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: take one step before the capture, or each replay clears the momentum")
+                    state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                by_device.setdefault(p.device, []).append((p, p.grad, state["momentum"]))
+            for of in by_device.values():
+                muon_step(*zip(*of), lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
+                          weight_decay=group["weight_decay"], steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
+        return loss

@@ -1,0 +1,226 @@
+"""lrbinner_amd.train_ops on the CPU: the definitions against 64 bits and against differences, the refusals, and what the
+C entry points refuse without a GPU."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from lrbinner_amd import _lib, train_ops
+from train_ops_ref import gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
+
+
+def make(rows, cols, seed=0, dtype=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, cols, generator=gen) * 2 + 0.5).to(dtype)
+    w, b = 1 + 0.3 * torch.randn(cols, generator=gen), torch.randn(cols, generator=gen)
+    return x, w, b, torch.randn(rows, cols, generator=gen).to(dtype), torch.rand(rows, cols, generator=gen) >= 0.3
+
+
+@pytest.mark.parametrize("block", [False, True])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (17, 128), (5, 1001)])
+def test_layer_norm_and_gradients(rows, cols, block):
+    x, w, b, dy, keep = make(rows, cols)
+    more = dict(slope=0.01, keep=keep, keep_scale=1 / 0.7) if block else {}
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = train_ops.layer_norm(*leaves, 1e-5, **more)
+    got = (y, *torch.autograd.grad(y, leaves, dy))
+    want, tol = norm_ref(x, w, b, 1e-5, dy, **more)
+    for name, g, e, t in zip(("y", "dx", "dw", "db"), got, want, tol):
+        # torch's own backward is made of other float32 operations than the formula's: four times as many
+        within(g.detach(), e, 4 * t + 1e-6 * float(e.abs().max()), name)
+
+
+def test_layer_norm_formula_against_differences():
+    x, w, b, dy, keep = make(4, 33)
+    more = dict(slope=0.2, keep=keep, keep_scale=1.5)
+    (_, dx, dw, db), _ = norm_ref(x, w, b, 1e-5, dy, **more)
+    gen = torch.Generator().manual_seed(9)
+    for k, (t, grad) in enumerate(((x, dx), (w, dw), (b, db))):
+        v, h = torch.randn(t.shape, generator=gen, dtype=torch.float64), 1e-6
+        v = v * (t.abs() > 1e-3)  # not across the activation's kink
+        at = [t.double() for t in (x, w, b)]
+
+        def loss(s):
+            moved = [a + s * v if i == k else a for i, a in enumerate(at)]
+            u = torch.where(keep, torch.where(moved[0] > 0, moved[0], 0.2 * moved[0]) * 1.5, torch.zeros_like(moved[0]))
+            c = u - u.mean(1, keepdim=True)
+            return ((c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-5) * moved[1] + moved[2]) * dy.double()).sum()
+
+        diff = (loss(h) - loss(-h)) / (2 * h)
+        assert abs(float(diff - (grad * v).sum())) < 1e-6 * (1 + abs(float(diff)))
+
+
+def test_what_is_dropped_does_not_count():
+    x, w, b, _, keep = make(6, 40)
+    keep[2] = False  # nothing is left of a row
+    clean = train_ops.layer_norm(x, w, b, slope=0.01, keep=keep, keep_scale=2.0)
+    x[~keep] = float("nan")
+    assert torch.equal(train_ops.layer_norm(x, w, b, slope=0.01, keep=keep, keep_scale=2.0), clean)
+    assert torch.equal(clean[2], b)
+
+
+def test_layer_norm_module():
+    m = train_ops.LayerNorm(8, slope=0.1)
+    assert sorted(m.state_dict()) == ["bias", "weight"]
+    x = torch.randn(3, 8)
+    assert torch.equal(m(x), train_ops.layer_norm(x, m.weight, m.bias, slope=0.1))
+
+
+@pytest.mark.parametrize("bad,error", [
+    (dict(x=torch.zeros(2, 4, dtype=torch.float64)), TypeError),
+    (dict(x=torch.zeros(2, 4, dtype=torch.long)), TypeError),
+    (dict(x=torch.zeros(2, 0)), ValueError),
+    (dict(x=torch.zeros(())), ValueError),
+    (dict(weight=torch.ones(3)), ValueError),
+    (dict(weight=torch.ones(1, 4)), ValueError),
+    (dict(weight=torch.ones(4, dtype=torch.bfloat16)), TypeError),
+    (dict(x=torch.zeros(2, 4, dtype=torch.bfloat16), weight=torch.ones(4, dtype=torch.bfloat16), bias=torch.ones(4)), TypeError),
+    (dict(x=torch.zeros(2, 4, dtype=torch.bfloat16), weight=torch.ones(4, dtype=torch.float16)), TypeError),
+    (dict(bias=torch.ones(5)), ValueError),
+    (dict(keep=torch.ones(2, 3, dtype=torch.bool)), ValueError),
+    (dict(keep=torch.ones(2, 4)), TypeError),
+    (dict(eps=-1.0), ValueError),
+    (dict(eps=float("nan")), ValueError),
+    (dict(slope=float("inf")), ValueError),
+    (dict(keep=torch.ones(2, 4, dtype=torch.bool), keep_scale=float("nan")), ValueError),
+    (dict(weight=torch.ones(4, device="meta")), ValueError),
+])
+def test_layer_norm_refuses(bad, error):
+    args = dict(x=torch.zeros(2, 4)) | bad
+    with pytest.raises(error):
+        train_ops.layer_norm(args.pop("x"), **args)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 9), (7, 1), (12, 31), (40, 25), (3, 20, 33)])
+def test_orthogonalize(shape):
+    g = gradient_like(*shape[-2:], torch.Generator().manual_seed(1), count=shape[:-2])
+    want = orthogonal_ref(g, 5, train_ops.COEFFICIENTS, 1e-7)
+    matrices_within(train_ops.orthogonalize(g), want, orthogonal_tolerance(want, g, 5, train_ops.COEFFICIENTS, 1e-7))
+    if min(shape[-2:]) > 1:
+        # the singular vectors stay: the polynomial acts on the singular values
+        u, s, vt = torch.linalg.svd((g.double() / torch.linalg.vector_norm(g.double(), dim=(-2, -1), keepdim=True)), full_matrices=False)
+        a, b, c = train_ops.COEFFICIENTS
+        for _ in range(5):
+            s = a * s + b * s ** 3 + c * s ** 5
+        assert float((u * s.unsqueeze(-2) @ vt - want).abs().max()) < 1e-9
+
+
+def test_orthogonalize_edges():
+    assert torch.equal(train_ops.orthogonalize(torch.zeros(4, 6)), torch.zeros(4, 6))
+    assert train_ops.orthogonalize(torch.zeros(0, 6)).shape == (0, 6)
+    g = torch.randn(4, 6)
+    assert train_ops.orthogonalize(g, out=g) is g
+
+
+@pytest.mark.parametrize("call,error", [
+    (lambda: train_ops.orthogonalize(torch.zeros(4)), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4, dtype=torch.float64)), TypeError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), steps=0), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), steps=33), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), steps=2.5), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), coefficients=(1.0, 2.0)), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), coefficients=(1.0, float("nan"), 0.0)), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), eps=-1.0), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), steps=2, coefficients=(6.0, -9.0, 4.0)), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), out=torch.zeros(4, 5)), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), out=torch.zeros(4, 4, dtype=torch.int32)), TypeError),
+    (lambda: train_ops.orthogonalize(torch.zeros(4, 4), out=torch.zeros(4, 1).expand(4, 4)), ValueError),
+    (lambda: train_ops.orthogonalize(torch.zeros(2, 3, 4, 4), out=torch.zeros(3, 2, 4, 4).transpose(0, 1)), ValueError),
+])
+def test_orthogonalize_refuses(call, error):
+    with pytest.raises(error):
+        call()
+
+
+@pytest.mark.parametrize("nesterov", [False, True])
+def test_muon_step(nesterov):
+    gen = torch.Generator().manual_seed(3)
+    shapes = [(6, 9), (9, 6), (2, 4, 5)]
+    p, g, m = ([torch.randn(s, generator=gen) for s in shapes] for _ in range(3))
+    want = []
+    for a, b, c in zip(p, g, m):
+        c = 0.9 * c.double() + 0.1 * b.double()
+        u = 0.1 * b.double() + 0.9 * c if nesterov else c
+        o = orthogonal_ref(u, 5, train_ops.COEFFICIENTS, 1e-7)
+        want.append((a.double() * (1 - 0.1 * 0.5) - 0.1 * math.sqrt(max(1, a.shape[-2] / a.shape[-1])) * o, c))
+    versions = [t._version for t in p + m]
+    train_ops.muon_step(p, g, m, lr=0.1, momentum=0.9, nesterov=nesterov, weight_decay=0.5)
+    for a, c, (wa, wc) in zip(p, m, want):
+        assert float((a - wa).abs().max()) < 1e-5 and float((c - wc).abs().max()) < 1e-6
+    assert all(t._version > v for t, v in zip(p + m, versions))
+
+
+def test_muon_step_refuses():
+    p, q = torch.zeros(4, 4), torch.zeros(4, 4)
+    for args, error in [(([p], [], None), ValueError), (([p], [torch.zeros(4, 3)], None), ValueError),
+                        (([p, p], [q, q], None), ValueError), (([p], [q], [p]), ValueError), (([p], [p], None), ValueError),
+                        (([p], [q], [q]), ValueError), (([torch.zeros(4)], [torch.zeros(4)], None), ValueError),
+                        (([p], [q.double()], None), TypeError), (([torch.zeros(1, 4).expand(4, 4)], [q], None), ValueError),
+                        (([p], [torch.zeros(4, 4, device="meta")], None), ValueError)]:
+        with pytest.raises(error):
+            train_ops.muon_step(*args, lr=0.1)
+    with pytest.raises(ValueError):
+        train_ops.muon_step([p], [q], lr=float("nan"))
+    with pytest.raises(ValueError):
+        train_ops.muon_step([p], [q], lr=0.1, momentum=float("inf"))
+    train_ops.muon_step([], [], lr=0.1)
+
+
+def test_muon_optimizer(tmp_path):
+    torch.manual_seed(0)
+    w = torch.nn.Parameter(torch.randn(6, 4, dtype=torch.bfloat16))
+    opt = train_ops.Muon([w], lr=0.1, weight_decay=0.1)
+    w.grad = torch.randn(6, 4, dtype=torch.bfloat16)
+    opt.step()
+    kept = opt.state[w]["momentum"].clone()
+    assert kept.dtype == torch.float32
+    again = train_ops.Muon([w], lr=0.5)
+    again.load_state_dict(opt.state_dict())
+    assert torch.equal(again.state[w]["momentum"], kept) and again.state[w]["momentum"].dtype == torch.float32
+    assert again.param_groups[0]["lr"] == 0.1
+    with pytest.raises(ValueError):
+        train_ops.Muon([torch.nn.Parameter(torch.zeros(4))])
+    with pytest.raises(ValueError):
+        train_ops.Muon([w], momentum=1.0)
+
+
+def test_c_entry_points_refuse_before_they_touch_a_device():
+    L = _lib.lib()
+    buf = C.create_string_buffer(64)
+    p = C.addressof(buf)
+    fwd = lambda x_type=0, w_type=0, rows=1, cols=4, x=p, y=p, mean=None, rstd=None: L.lrb_layer_norm_fwd_dev(
+        0, None, x_type, w_type, rows, cols, x, cols, None, None, 1e-5, 1.0, None, 1.0, y, mean, rstd)
+    assert fwd(rows=0) == 0
+    for bad in (dict(x_type=3), dict(x_type=-1), dict(w_type=1), dict(x_type=1, w_type=2), dict(cols=0), dict(cols=1 << 40),
+                dict(rows=1 << 50), dict(x=None), dict(y=None), dict(mean=p)):
+        assert fwd(**bad) == 1, bad
+    assert L.lrb_layer_norm_bwd_ws_bytes(7, 4, 4) == 0
+    assert L.lrb_layer_norm_bwd_dev(0, None, 0, 0, 1, 4, p, 4, p, 4, None, p, p, 1.0, None, 1.0, p, p, None, p, 0) == 1  # no room
+    assert L.lrb_layer_norm_bwd_dev(0, None, 0, 0, 1, 4, None, 4, p, 4, None, p, p, 1.0, None, 1.0, p, None, None, None, 0) == 1
+
+    def item(rows=4, cols=4, count=1, p_ptr=p, p_type=0, g_type=0, m=0, m_type=0):
+        return C.create_string_buffer(train_ops._ITEM.pack(p_ptr, p, m, 16, 4, 1, 16, 4, 1, 0, 0, 0, count, rows, cols, p_type, g_type, m_type, 1.0, 0.0, 0))
+
+    step = lambda it, n=1, steps=5, eps=0.0, ws=p, ws_bytes=64: L.lrb_muon_dev(0, None, it, n, 0.9, 1, steps, 1.5, -0.5, 0.0, eps, ws, ws_bytes)
+    assert step(None, 0) == 0 and step(item(rows=0)) == 0 and step(item(count=0)) == 0
+    for it, more in ((item(rows=-1), {}), (item(cols=1 << 25), {}), (item(rows=1 << 20, cols=1 << 20), {}), (item(p_ptr=0), {}),
+                     (item(p_type=3), {}), (item(g_type=-1), {}), (item(m=p, m_type=9), {}), (item(), dict(steps=0)),
+                     (item(), dict(steps=33)), (item(), dict(eps=-1.0)), (item(), dict(n=-1)), (None, {}), (item(), dict(ws=None)),
+                     (item(), dict(ws_bytes=64))):
+        assert step(it, **more) == 1, more
+    assert L.lrb_muon_ws_bytes(item(), 1) >= 16 * 64 * 64
+    assert L.lrb_muon_dev(0, None, item(), 1, 0.9, 1, 2, 6.0, -9.0, 4.0, 0.0, p, 1 << 30) == 1       # diverges
+    assert L.lrb_muon_dev(0, None, item(), 1, 0.9, 1, 2, float("nan"), 1.0, 1.0, 0.0, p, 1 << 30) == 1
+
+
+def test_muon_bound():
+    bound = lambda steps, c: _lib.lib().lrb_muon_bound(steps, *c)
+    for c in (train_ops.COEFFICIENTS, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (0.0, 0.0, 0.0), (-1.2, 0.3, 0.1), (1.0, 1.0, 0.0)):
+        s = torch.linspace(0, 1, 100001, dtype=torch.float64)
+        most = 1.0
+        for _ in range(4):
+            # of the interval up to the largest value so far, as the bound is made
+            s = torch.linspace(0, float((c[0] * s + c[1] * s ** 3 + c[2] * s ** 5).abs().max()), 100001, dtype=torch.float64)
+            most = max(most, float(s[-1]))
+        assert abs(bound(4, c) - most) < 1e-6 * most, c
