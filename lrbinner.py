@@ -25,6 +25,8 @@ ENVIRONMENT = """environment (this build; the full list is in INTEGRATION.md):
                                very large inputs on slow file systems)
   LRB_DEVICE=I                 GPU of a single-GPU run (default 0)
   LRB_SEED=S                   seed random / numpy / torch (the reference never seeds)
+  LRB_VAE_NORM=layer           the VAE's blocks normalise each read by itself instead of over the batch
+  LRB_VAE_OPTIMIZER=muon       orthogonalised updates for the VAE's hidden weights, Adam for the rest
   LRB_VAE_DETERMINISTIC=1      with LRB_SEED: the VAE's sums in a fixed order -- the same latents run after run
 """
 

@@ -18,7 +18,7 @@ import os
 
 import numpy as np
 
-from . import _npcache
+from . import _npcache, train_ops
 import torch
 from torch import nn, optim
 
@@ -73,10 +73,32 @@ def make_data(covs, profs, device):
     return torch.from_numpy(x).to(device)
 
 
+class _Both:
+    """Two optimisers as one."""
+
+    def __init__(self, *optimizers):
+        self.optimizers = optimizers
+
+    def zero_grad(self, set_to_none=True):
+        for o in self.optimizers:
+            o.zero_grad(set_to_none=set_to_none)
+
+    def step(self):
+        for o in self.optimizers:
+            o.step()
+
+
 class VAE(nn.Module):
+    """``norm``: "batch" (the reference's BatchNorm) or "layer": layer normalisation, which treats every row by itself -- no
+    running statistics, and a row's latent does not depend on what else was in its batches.  Its blocks run LeakyReLU,
+    dropout and norm as one operator (train_ops.layer_norm)."""
+
     def __init__(self, cov_size, prof_size, *, latent_dims=8, hidden_layers=[128, 128],
-                 constraints=None, device='cpu'):
+                 constraints=None, device='cpu', norm='batch'):
         super().__init__()
+        if norm not in ('batch', 'layer'):
+            raise ValueError(f"norm: 'batch' or 'layer' is wanted, not {norm!r}")
+        self.norm = norm
         self.cov_size = cov_size
         self.prof_size = prof_size
         self.hidden_layers = list(hidden_layers)
@@ -91,13 +113,13 @@ class VAE(nn.Module):
         widths = [cov_size + prof_size] + self.hidden_layers
         for nin, nout in zip(widths[:-1], widths[1:]):
             self.encoderlayers.append(nn.Linear(nin, nout))
-            self.encodernorms.append(nn.BatchNorm1d(nout))
+            self.encodernorms.append(self._norm_of(nout))
         self.mu = nn.Linear(self.hidden_layers[-1], latent_dims)
         self.logsigma = nn.Linear(self.hidden_layers[-1], latent_dims)
         widths = [latent_dims] + self.hidden_layers[::-1]
         for nin, nout in zip(widths[:-1], widths[1:]):
             self.decoderlayers.append(nn.Linear(nin, nout))
-            self.decodernorms.append(nn.BatchNorm1d(nout))
+            self.decodernorms.append(self._norm_of(nout))
         self.outputlayer = nn.Linear(self.hidden_layers[0], cov_size + prof_size)
 
         self.relu = nn.LeakyReLU()
@@ -119,15 +141,29 @@ class VAE(nn.Module):
         s = {(min(int(a), int(b)), max(int(a), int(b))) for a, b in lst if int(a) != int(b)}
         return np.array(sorted(s), dtype=np.int64).reshape(-1, 2)
 
+    def _norm_of(self, width):
+        if self.norm == 'layer':
+            return train_ops.LayerNorm(width, slope=0.01)  # nn.LeakyReLU's default, which the operator applies
+        return nn.BatchNorm1d(width)
+
     # block = BatchNorm(Dropout(LeakyReLU(Linear(x))))  -- ae_utils.py:130-133,173-176
+    def _block(self, layer, norm, x):
+        if self.norm == 'batch':
+            return norm(self.dropoutlayer(self.relu(layer(x))))
+        x = layer(x)
+        if not self.training:
+            return norm(x)
+        keep = torch.empty(x.shape, dtype=torch.bool, device=x.device).bernoulli_(1 - self.dropout)
+        return norm(x, keep, 1 / (1 - self.dropout))
+
     def _encode(self, x):
         for layer, norm in zip(self.encoderlayers, self.encodernorms):
-            x = norm(self.dropoutlayer(self.relu(layer(x))))
+            x = self._block(layer, norm, x)
         return self.mu(x), self.softplus(self.logsigma(x))
 
     def _decode(self, z):
         for layer, norm in zip(self.decoderlayers, self.decodernorms):
-            z = norm(self.dropoutlayer(self.relu(layer(z))))
+            z = self._block(layer, norm, z)
         return self.outputlayer(z)
 
     def forward(self, x):
@@ -182,25 +218,40 @@ class VAE(nn.Module):
         optimizer.step()
         sums += torch.stack([loss.detach(), e_cov.detach(), e_comp.detach(), kld.detach()])
 
+    def _optimizer(self, name, lrate, muon_lrate, capturable):
+        if name == 'adam':
+            return optim.Adam(self.parameters(), lr=lrate, capturable=capturable)
+        hidden = [l.weight for l in (*self.encoderlayers, *self.decoderlayers)]
+        ids = {id(p) for p in hidden}
+        rest = [p for p in self.parameters() if id(p) not in ids]
+        return _Both(train_ops.Muon(hidden, lr=muon_lrate), optim.Adam(rest, lr=lrate, capturable=capturable))
+
     def trainmodel(self, data, *, nepochs=500, lrate=1e-3, batchsteps=(25, 75, 150, 300),
-                   batch_size=1024, save_path=None, use_graph=None):
+                   batch_size=1024, save_path=None, use_graph=None, optimizer='adam', muon_lrate=0.02):
         """Adam over all parameters; the batch doubles at every epoch in ``batchsteps``;
         the ragged tail of each epoch is dropped (ae_utils.py:199-281).
+
+        ``optimizer`` = "muon": the hidden layers' weights take orthogonalised updates (train_ops.Muon, with
+        ``muon_lrate``), heads, output layer, biases and norms stay with Adam.  The fused step below is BatchNorm with
+        Adam; other choices run as torch modules, in a graph as well.
 
         The step is ~45 k MACs per sample: on a GPU it is launch-bound (about thirty tiny
         kernels).  On CUDA/HIP devices the whole step -- gather, forward, loss, backward,
         Adam -- is therefore captured once per batch size in a HIP graph and replayed;
         only the 8 KB index vector changes between replays."""
+        if optimizer not in ('adam', 'muon'):
+            raise ValueError(f"optimizer: 'adam' or 'muon' is wanted, not {optimizer!r}")
         steps = set(batchsteps)
         self._n_rows = data.shape[0]
         on_gpu = data.is_cuda
-        if on_gpu and use_graph is None and self.constraints is None \
+        if on_gpu and use_graph is None and self.constraints is None and self.norm == 'batch' and optimizer == 'adam' \
                 and os.environ.get("LRB_VAE_NATIVE", "1") != "0":
             return self._trainmodel_native(data, nepochs, lrate, steps, batch_size, save_path)
         if use_graph is None:
             use_graph = on_gpu and os.environ.get("LRB_VAE_GRAPH", "1") != "0" \
                 and self.constraints is None
-        optimizer = optim.Adam(self.parameters(), lr=lrate, capturable=bool(use_graph))
+        self.release_native()  # what an earlier run left for encode() would be out of date
+        optimizer = self._optimizer(optimizer, lrate, muon_lrate, bool(use_graph))
         n = data.shape[0]
         graphs = {}  # batch size -> (graph, static index buffer)
         for epoch in range(nepochs):
@@ -327,30 +378,37 @@ class VAE(nn.Module):
         return out
 
     def save(self, save_path):
-        torch.save({'cov_size': self.cov_size, 'prof_size': self.prof_size,
-                    'dropout': self.dropout, 'hidden_layers': self.hidden_layers,
-                    'latent_dims': self.latent_dims, 'state': self.state_dict()}, save_path)
+        saved = {'cov_size': self.cov_size, 'prof_size': self.prof_size,
+                 'dropout': self.dropout, 'hidden_layers': self.hidden_layers,
+                 'latent_dims': self.latent_dims, 'state': self.state_dict()}
+        if self.norm != 'batch':  # the reference's layout has no such key
+            saved['norm'] = self.norm
+        torch.save(saved, save_path)
 
 
 def count_parameters(model):
     return sum(p.numel() for p in model.parameters() if p.requires_grad)
 
 
-def vae_encode(output, latent_dims, hidden_layers, epochs, constraints, cuda):
+def vae_encode(output, latent_dims, hidden_layers, epochs, constraints, cuda, norm=None, optimizer=None):
+    """``norm`` and ``optimizer`` as in VAE and VAE.trainmodel; None: LRB_VAE_NORM and LRB_VAE_OPTIMIZER, or the reference's."""
     import time
+    norm = norm or os.environ.get("LRB_VAE_NORM", "batch")
+    optimizer = optimizer or os.environ.get("LRB_VAE_OPTIMIZER", "adam")
     t0 = time.time()
     comp_profiles = _npcache.load(f"{output}/profiles/com_profs.npy")
     cov_profiles = _npcache.load(f"{output}/profiles/cov_profs.npy")
     device = "cuda" if cuda else "cpu"
 
     vae = VAE(cov_profiles.shape[1], comp_profiles.shape[1], latent_dims=latent_dims,
-              hidden_layers=hidden_layers, constraints=constraints, device=device)
+              hidden_layers=hidden_layers, constraints=constraints, device=device, norm=norm)
     logger.debug(f"Model param count = {count_parameters(vae)}")
     logger.debug(vae)
 
     data = make_data(cov_profiles, comp_profiles, device)
     t1 = time.time()
-    vae.trainmodel(data, save_path=f"{output}/model.pt", nepochs=epochs, batchsteps=[50, 100, 150])
+    vae.trainmodel(data, save_path=f"{output}/model.pt", nepochs=epochs, batchsteps=[50, 100, 150],
+                   optimizer=optimizer)
     t2 = time.time()
     latent = vae.encode(data)
     vae.release_native()

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from lrbinner_amd import train_ops
+from lrbinner_amd import ae_utils, train_ops
 from train_ops_ref import HALF_STEP, gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
 
 pytestmark = pytest.mark.gpu
@@ -484,3 +484,72 @@ def test_versions_are_counted():
     train_ops.muon_step(p, g, m, lr=0.1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+# ---- the network that uses them -------------------------------------------------------------------
+
+def test_vae_with_layer_norm_runs_as_its_formula():
+    torch.manual_seed(0)
+    vae = ae_utils.VAE(32, 136, norm="layer", device="cuda")
+    twin = ae_utils.VAE(32, 136, norm="layer").double()
+    twin.load_state_dict({k: v.cpu() for k, v in vae.state_dict().items()})
+    x = torch.rand(300, 168, device="cuda")
+    mu = vae.encode(x)
+    z = x.cpu().double()
+    for lin, norm in zip(twin.encoderlayers, twin.encodernorms):
+        z = torch.nn.functional.leaky_relu(lin(z), 0.01)
+        z = (z - z.mean(1, keepdim=True)) / torch.sqrt(z.var(1, unbiased=False, keepdim=True) + 1e-5) * norm.weight + norm.bias
+    assert float((twin.mu(z).detach() - torch.from_numpy(mu)).abs().max()) < 1e-4
+    # a training step's gradients, dropout included: the draws of the same seed, once by the operator, once by formulas
+    vae.train()
+
+    def loss_and_grads(model, block):
+        torch.manual_seed(5)
+        model._block = block
+        recon, m, s = model(x)
+        loss = model.calc_loss(x, recon, m, s)[0]
+        grads = torch.autograd.grad(loss, list(model.parameters()))
+        del model._block
+        return float(loss.detach()), grads
+
+    def by_formulas(layer, norm, v):
+        v = layer(v)
+        keep = torch.empty(v.shape, dtype=torch.bool, device=v.device).bernoulli_(1 - vae.dropout)
+        v = torch.nn.functional.leaky_relu(v, 0.01) * keep / (1 - vae.dropout)
+        c = v - v.mean(1, keepdim=True)
+        return c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-5) * norm.weight + norm.bias
+
+    own, own_grads = loss_and_grads(vae, vae._block)
+    ref, ref_grads = loss_and_grads(vae, by_formulas)
+    assert abs(own - ref) < 1e-5 * abs(ref)
+    for a, b in zip(own_grads, ref_grads):
+        assert float((a - b).norm()) < 1e-4 * float(b.norm()) + 1e-7
+
+
+@pytest.mark.parametrize("norm,optimizer", [("layer", "muon"), ("layer", "adam"), ("batch", "muon")])
+@pytest.mark.parametrize("use_graph", [None, False])
+def test_vae_trains(norm, optimizer, use_graph):
+    torch.manual_seed(0)
+    data = torch.rand(3000, 168, device="cuda")
+    vae = ae_utils.VAE(32, 136, norm=norm, device="cuda")
+    before = {k: v.clone() for k, v in vae.state_dict().items()}
+    vae.trainmodel(data, nepochs=4, batchsteps=[2], batch_size=256, optimizer=optimizer, use_graph=use_graph)
+    for k, v in vae.state_dict().items():
+        assert bool(torch.isfinite(v).all()) and not torch.equal(v, before[k]), k
+    assert getattr(vae, "_native", None) is None
+    mu = vae.encode(data, chunk=1000)
+    assert mu.shape == (3000, 8) and bool(torch.isfinite(torch.from_numpy(mu)).all())
+    vae.trainmodel(data, nepochs=1, batchsteps=[], batch_size=256, optimizer=optimizer, use_graph=use_graph)
+
+
+def test_a_run_after_a_fused_one_encodes_with_its_own_weights():
+    torch.manual_seed(0)
+    data = torch.rand(600, 168, device="cuda")
+    vae = ae_utils.VAE(32, 136, device="cuda")
+    vae.trainmodel(data, nepochs=1, batchsteps=[], batch_size=256)
+    assert vae._native is not None
+    vae.trainmodel(data, nepochs=2, batchsteps=[], batch_size=256, optimizer="muon")
+    mu = vae.encode(data)
+    vae.eval()
+    with torch.no_grad():
+        assert float((vae._encode(data)[0].cpu() - torch.from_numpy(mu)).abs().max()) < 1e-5

@@ -3,10 +3,11 @@ C entry points refuse without a GPU."""
 import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from lrbinner_amd import _lib, train_ops
+from lrbinner_amd import _lib, ae_utils, train_ops
 from train_ops_ref import gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
 
 
@@ -224,3 +225,50 @@ def test_muon_bound():
             s = torch.linspace(0, float((c[0] * s + c[1] * s ** 3 + c[2] * s ** 5).abs().max()), 100001, dtype=torch.float64)
             most = max(most, float(s[-1]))
         assert abs(bound(4, c) - most) < 1e-6 * most, c
+
+
+# ---- the network that uses them -------------------------------------------------------------------
+
+def test_vae_with_layer_norm_and_muon(tmp_path):
+    torch.manual_seed(0)
+    data = torch.rand(600, 42)
+    vae = ae_utils.VAE(10, 32, latent_dims=4, hidden_layers=[24, 16], norm="layer")
+    assert [k for k in vae.state_dict() if "norms.0" in k] == ["encodernorms.0.weight", "encodernorms.0.bias",
+                                                                "decodernorms.0.weight", "decodernorms.0.bias"]
+    before = {k: v.clone() for k, v in vae.state_dict().items()}
+    vae.trainmodel(data, nepochs=3, batchsteps=[1], batch_size=64, optimizer="muon", save_path=str(tmp_path / "m.pt"))
+    after = vae.state_dict()
+    assert all(bool(torch.isfinite(v).all()) and not torch.equal(v, before[k]) for k, v in after.items())
+    assert torch.load(str(tmp_path / "m.pt"), weights_only=True)["norm"] == "layer"
+    mu = vae.encode(data, chunk=100)
+    # rows do not depend on each other
+    assert mu.shape == (600, 4) and abs(mu[17:18] - vae.encode(data[17:18])).max() < 1e-5
+    # what the eval pass computes is the module's formula
+    x = data.double()
+    for lin, norm in zip(vae.encoderlayers, vae.encodernorms):
+        x = torch.nn.functional.leaky_relu(x @ lin.weight.double().T + lin.bias.double(), 0.01)
+        x = (x - x.mean(1, keepdim=True)) / torch.sqrt(x.var(1, unbiased=False, keepdim=True) + 1e-5) * norm.weight.double() + norm.bias.double()
+    assert float((x @ vae.mu.weight.double().T + vae.mu.bias.double() - torch.from_numpy(mu)).detach().abs().max()) < 1e-4
+
+
+def test_vae_choices():
+    with pytest.raises(ValueError, match="norm"):
+        ae_utils.VAE(10, 32, norm="group")
+    vae = ae_utils.VAE(10, 32, latent_dims=2, hidden_layers=[8])
+    with pytest.raises(ValueError, match="optimizer"):
+        vae.trainmodel(torch.rand(10, 42), nepochs=1, optimizer="sgd")
+
+
+def test_vae_encode_takes_the_choices_from_the_environment(tmp_path, monkeypatch):
+    (tmp_path / "profiles").mkdir()
+    rng = np.random.default_rng(0)
+    np.save(tmp_path / "profiles" / "com_profs.npy", rng.random((1100, 32)))
+    np.save(tmp_path / "profiles" / "cov_profs.npy", rng.random((1100, 10)))
+    monkeypatch.setenv("LRB_VAE_NORM", "layer")
+    monkeypatch.setenv("LRB_VAE_OPTIMIZER", "muon")
+    ae_utils.vae_encode(str(tmp_path), 3, [8, 8], 2, None, False)
+    assert np.load(tmp_path / "latent.npy").shape == (1100, 3)
+    assert torch.load(str(tmp_path / "model.pt"), weights_only=True)["norm"] == "layer"
+    monkeypatch.setenv("LRB_VAE_OPTIMIZER", "none")
+    with pytest.raises(ValueError, match="optimizer"):
+        ae_utils.vae_encode(str(tmp_path), 3, [8, 8], 2, None, False)
