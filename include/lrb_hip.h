@@ -567,7 +567,7 @@ int lrb_layer_norm_bwd_dev(int device, void *stream, int x_type, int w_type, uin
  *   p <- decay p + alpha X;  with decay = 0 p is not read
  * Strides are in elements, of (matrix, row, column), any values; p and m must not overlap each other, g, or another item's.
  * A matrix that holds an infinity or a NaN gives NaN throughout.  1 <= steps <= 32; a matrix below 2^31 elements with sides
- * below 2^24.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
+ * of at most 2^22.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
 typedef struct {
     void *p;
     const void *g;

@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
 
 enum { MU_GRAM = 0, MU_POLY = 1, MU_APPLY = 2, MU_LAST = 3 };
 
-__device__ __forceinline__ void mu_dma(const mu_h *src, char *dst)
+__device__ __forceinline__ void mu_dma(const char *src, char *dst)
 {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
@@ -277,33 +277,53 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
     const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
-    int i0, j0 = local % per;
+    // Four rows of tiles at a time, column by column: the tiles that an XCD has in flight together are as square a block as
+    // can be, so that its L2 serves most of their loads.
+    int i0 = 0, j0 = local % per;
     if (MODE >= MU_APPLY) {
-        i0 = j0 / tj;
-        j0 -= i0 * tj;
-    } else { // the tiles on and above the diagonal, row by row
-        i0 = 0;
-        while (j0 >= ti - i0) j0 -= ti - i0++;
-        j0 += i0;
+        const int band = j0 / (4 * tj), h = min(4, ti - 4 * band);
+        j0 -= band * 4 * tj;
+        i0 = 4 * band + j0 % h;
+        j0 /= h;
+    } else { // the tiles on and above the diagonal: of each band first the triangle, then what lies right of it
+        int h = min(4, ti);
+        while (j0 >= h * (ti - i0) - h * (h - 1) / 2) {
+            j0 -= h * (ti - i0) - h * (h - 1) / 2;
+            i0 += 4;
+            h = min(4, ti - i0);
+        }
+        const int band = i0, triangle = h * (h + 1) / 2;
+        if (j0 < triangle) {
+            int r = 0;
+            while (j0 >= h - r) j0 -= h - r++;
+            i0 = band + r;
+            j0 += i0;
+        } else {
+            j0 -= triangle;
+            i0 = band + j0 % h;
+            j0 = band + h + j0 / h;
+        }
     }
     i0 *= T, j0 *= T;
     const mu_mat w = mu_planes(a, it, mat);
     const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
     const mu_h *P = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.b, *Q = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.xt;
     const size_t p_plane = (size_t)it.np * K, q_plane = (size_t)jrows * K;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / WN, wj = wave % WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN, wj = wave % WN;
 
-    const mu_h *src[LOADS];
-    int dst[LOADS];
+    // A load of a wave fills 16 rows of a stage.  All addresses are a plane's first row of the tile (uniform) and an offset of
+    // the lane's row in it (32 bits: 256 rows of up to 2^22 entries); rows past the padding (tiles larger than 64) repeat the last
+    // one, and what they give is not stored.
+    constexpr int ROWS = WAVES * 16, HALVES = T / ROWS; // rows that the waves fill together; such fills a part
+    static_assert(HALVES * 4 == LOADS, "");
+    uint32_t off_p[HALVES], off_q[HALVES];
 #pragma unroll
-    for (int q = 0; q < LOADS; ++q) {
-        const int r0 = (q * WAVES + wave) * 16, r = r0 + (lane >> 2); // of the 4 T rows of a stage
-        const int part = r0 / T, row = r % T, chunk = (lane & 3) ^ ((r >> 2) & 3);
-        // rows past the padding (tiles larger than 64) repeat the last one; what they give is not stored
-        const int at = part < 2 ? min(i0 + row, it.np - 1) : min(j0 + row, jrows - 1);
-        src[q] = (part < 2 ? P : Q) + (part & 1 ? (part < 2 ? p_plane : q_plane) : 0) + (size_t)at * K + chunk * 8;
-        dst[q] = r0 * 64;
+    for (int q = 0; q < HALVES; ++q) {
+        const int row = q * ROWS + wave * 16 + (lane >> 2), chunk = (lane & 3) ^ ((row >> 2) & 3);
+        off_p[q] = ((uint32_t)min(row, it.np - 1 - i0) * (uint32_t)K + chunk * 8) * 2;
+        off_q[q] = ((uint32_t)min(row, jrows - 1 - j0) * (uint32_t)K + chunk * 8) * 2;
     }
+    const char *const base_p = (const char *)(P + (size_t)i0 * K), *const base_q = (const char *)(Q + (size_t)j0 * K);
 
     mu_f16 acc[MI][NI];
 #pragma unroll
@@ -315,49 +335,79 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 
     const int frow = lane & 31, fchunk = lane >> 5;
     auto stage = [&](char *buf, int k0) {
+        const char *const p = base_p + 2 * (size_t)k0, *const q = base_q + 2 * (size_t)k0;
+        const int d = wave * 1024;
 #pragma unroll
-        for (int q = 0; q < LOADS; ++q) mu_dma(src[q] + k0, buf + dst[q]);
+        for (int h = 0; h < HALVES; ++h) {
+            mu_dma(p + off_p[h], buf + h * ROWS * 64 + d);
+            mu_dma(p + 2 * p_plane + off_p[h], buf + T * 64 + h * ROWS * 64 + d);
+            mu_dma(q + off_q[h], buf + 2 * T * 64 + h * ROWS * 64 + d);
+            mu_dma(q + 2 * q_plane + off_q[h], buf + 3 * T * 64 + h * ROWS * 64 + d);
+        }
         __builtin_amdgcn_sched_barrier(0); // else the compiler sinks the loads to the wait that ends the stage
     };
-    auto products = [&](const char *buf) {
+    struct frags {
+        mu_h8 ph[MI], pl[MI], qh[NI], ql[NI];
+    };
+    // the chunk of a row does not depend on which 32 rows it is among: (row >> 2) & 3 == (frow >> 2) & 3
+    const int at0 = frow * 64 + ((fchunk ^ ((frow >> 2) & 3)) << 4), at1 = frow * 64 + (((2 + fchunk) ^ ((frow >> 2) & 3)) << 4);
+    auto read = [&](frags &f, const char *buf, int kk) {
+        const char *const p = buf + wi * MI * 2048 + (kk ? at1 : at0), *const q = buf + 2 * T * 64 + wj * NI * 2048 + (kk ? at1 : at0);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            mu_h8 ph[MI], pl[MI], qh[NI], ql[NI];
+        for (int y = 0; y < NI; ++y) {
+            f.qh[y] = *(const mu_h8 *)(q + y * 2048);
+            f.ql[y] = *(const mu_h8 *)(q + T * 64 + y * 2048);
+        }
 #pragma unroll
-            for (int x = 0; x < MI; ++x) {
-                const int row = (wi * MI + x) * 32 + frow, at = row * 64 + (((kk * 2 + fchunk) ^ ((row >> 2) & 3)) << 4);
-                ph[x] = *(const mu_h8 *)(buf + at);
-                pl[x] = *(const mu_h8 *)(buf + T * 64 + at);
-            }
-#pragma unroll
-            for (int y = 0; y < NI; ++y) {
-                const int row = (wj * NI + y) * 32 + frow, at = row * 64 + (((kk * 2 + fchunk) ^ ((row >> 2) & 3)) << 4);
-                qh[y] = *(const mu_h8 *)(buf + 2 * T * 64 + at);
-                ql[y] = *(const mu_h8 *)(buf + 3 * T * 64 + at);
-            }
-#pragma unroll
-            for (int x = 0; x < MI; ++x)
-#pragma unroll
-                for (int y = 0; y < NI; ++y) {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[y], ph[x], acc[x][y], 0, 0, 0);
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[y], pl[x], acc[x][y], 0, 0, 0);
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[y], ph[x], acc[x][y], 0, 0, 0);
-                }
+        for (int x = 0; x < MI; ++x) {
+            f.ph[x] = *(const mu_h8 *)(p + x * 2048);
+            f.pl[x] = *(const mu_h8 *)(p + T * 64 + x * 2048);
         }
     };
-    // K is a multiple of 64: two stages a turn.  A stage is written while the other is read; the barrier says that all waves
-    // have left the one that is written next, the wait before it that the wave's own loads have arrived.
+    auto products = [&](const frags &f) {
+#pragma unroll
+        for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int y = 0; y < NI; ++y) {
+                acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ql[y], f.ph[x], acc[x][y], 0, 0, 0);
+                acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.qh[y], f.pl[x], acc[x][y], 0, 0, 0);
+                acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.qh[y], f.ph[x], acc[x][y], 0, 0, 0);
+            }
+        // the reads of the next fragments, which are independent of these products, go between them
+#pragma unroll
+        for (int r = 0; r < 2 * (MI + NI); ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); // an LDS read
+            __builtin_amdgcn_sched_group_barrier(0x008, 3 * MI * NI / (2 * (MI + NI)), 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 3 * MI * NI, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // K is a multiple of 64: two stages a turn, two times 16 k in each.  While the products of one fragment set run, the next set
+    // is read; in the middle of a stage, when a wave has read all it needs of it, comes the barrier behind which the
+    // stage's buffer is filled again -- by then the other buffer's loads, issued one stage ago, have arrived.  The last turns
+    // load and read the last stage once more than needed: branches would part the reads from the products.
+    frags f0, f1;
+    auto turn = [&](char *buf, char *next, int k0) {
+        read(f1, buf, 1);
+        products(f0);
+        __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0), lgkmcnt(0): the next stage is there, this one is read
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        stage(buf, min(k0 + 2 * MU_BK, K - MU_BK));
+        read(f0, next, 0);
+        products(f1);
+    };
     stage(buf0, 0);
+    stage(buf1, MU_BK);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS); // vmcnt(LOADS): the first stage
+    lrb_barrier();
+    read(f0, buf0, 0);
     for (int k0 = 0; k0 < K; k0 += 2 * MU_BK) {
-        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
-        lrb_barrier();
-        stage(buf1, k0 + MU_BK);
-        products(buf0);
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-        lrb_barrier();
-        if (k0 + 2 * MU_BK < K) stage(buf0, k0 + 2 * MU_BK);
-        products(buf1);
+        turn(buf0, buf1, k0);
+        turn(buf1, buf0, k0 + MU_BK);
     }
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    lrb_barrier();
 
     // lane -> row i of C, four neighbouring columns j in every four registers
     const float *t = a.table + ((size_t)(it.first + mat) * a.steps + a.step) * MU_COEF;
@@ -498,8 +548,8 @@ static bool mu_items_fit(const lrb_muon_item *items, int n)
         const lrb_muon_item &s = items[k];
         if (s.count < 0 || s.rows < 0 || s.cols < 0) return false;
         if (s.count == 0 || s.rows == 0 || s.cols == 0) continue;
-        // a side below 2^24 and planes below 2^31 entries: the kernels' 32-bit indices hold
-        if (s.rows > (1 << 24) || s.cols > (1 << 24) || (s.rows + 63) * (s.cols + 63) > INT_MAX) return false;
+        // a side below 2^22 and planes below 2^31 entries: the kernels' 32-bit indices hold
+        if (s.rows > (1 << 22) || s.cols > (1 << 22) || (s.rows + 63) * (s.cols + 63) > INT_MAX) return false;
         if (!s.p || !s.g || s.p_type < LRB_F32 || s.p_type > LRB_F16 || s.g_type < LRB_F32 || s.g_type > LRB_F16) return false;
         if (s.m && (s.m_type < LRB_F32 || s.m_type > LRB_F16)) return false;
     }
