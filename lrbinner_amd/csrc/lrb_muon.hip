@@ -55,6 +55,9 @@ struct mu_args {
     int nesterov;
     int flip;       // which of the two copies of X is read
     int step;
+    // of a product's launch: the tiles from `direct` on are cut along k, `splits` workgroups each, whose sums go to `parts`
+    int direct, splits;
+    float *parts;
     int start[MU_ITEMS + 1]; // first tile of each item in this launch
     mu_item it[MU_ITEMS];
 };
@@ -260,6 +263,151 @@ __device__ __forceinline__ void mu_dma(const char *src, char *dst)
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
 
+__device__ __forceinline__ void mu_wave_sync() // LDS written by lanes of this wave is read by others of it
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0)
+    __builtin_amdgcn_wave_barrier();
+}
+
+// p <- decay p + alpha v for up to four entries, `stride` apart
+template <typename T> __device__ __forceinline__ void mu_update(const mu_item &it, long long at, long long stride, int count, float4 v)
+{
+    T *p = (T *)it.p + at;
+    if (stride == 1 && count == 4) {
+        T t[4];
+        if (it.decay != 0.0f) {
+            __builtin_memcpy(t, p, sizeof(t));
+            v.x = it.decay * (float)t[0] + it.alpha * v.x, v.y = it.decay * (float)t[1] + it.alpha * v.y;
+            v.z = it.decay * (float)t[2] + it.alpha * v.z, v.w = it.decay * (float)t[3] + it.alpha * v.w;
+        } else {
+            v.x *= it.alpha, v.y *= it.alpha, v.z *= it.alpha, v.w *= it.alpha;
+        }
+        t[0] = (T)v.x, t[1] = (T)v.y, t[2] = (T)v.z, t[3] = (T)v.w;
+        __builtin_memcpy(p, t, sizeof(t));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= count) break;
+        const float x = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+        p[e * stride] = (T)((it.decay != 0.0f ? it.decay * (float)p[e * stride] : 0.0f) + it.alpha * x);
+    }
+}
+__device__ __forceinline__ void mu_update4(const mu_item &it, long long at, long long stride, int count, float4 v)
+{
+    if (it.p_type == LRB_F32) mu_update<float>(it, at, stride, count, v);
+    else if (it.p_type == LRB_BF16) mu_update<__bf16>(it, at, stride, count, v);
+    else mu_update<mu_h>(it, at, stride, count, v);
+}
+
+// What becomes of 32 x 32 NI entries of a product, of which a wave holds the sums: acc[y][4 q + e] of a lane is row (lane & 31),
+// column 32 y + 8 q + 4 (lane >> 5) + e.  They go through `lds` (32 rows of MU_PITCH) to be read, combined and written in
+// whole row segments, and once more by columns for the mirrored or transposed side.
+#define MU_PITCH(NI) (32 * (NI) + 4)
+template <int MODE, int NI>
+__device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, int mat, const mu_mat &w, const mu_f16 (&acc)[NI], int i0, int j0,
+                                         bool mirror, float *lds, int lane)
+{
+    constexpr int PITCH = MU_PITCH(NI), LANES = 8 * NI, ROWS = 64 / LANES; // lanes of a row, rows of a turn
+    const float *t = a.table + ((size_t)(it.first + mat) * a.steps + a.step) * MU_COEF;
+    const float k1 = MODE == MU_GRAM ? 0.0f : MODE == MU_POLY ? t[1] : t[3], k2 = MODE == MU_GRAM ? t[0] : MODE == MU_POLY ? t[2] : t[4];
+    const int ld = MODE >= MU_APPLY ? it.lp : it.np;
+    const size_t plane = (size_t)it.np * ld;
+    float *full = MODE <= MU_POLY ? w.a32 : w.x32;
+    mu_h *out = MODE == MU_GRAM ? w.a : MODE == MU_POLY ? w.b : w.x2, *out_t = MODE == MU_APPLY ? w.xt2 : out;
+    const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1; // which way p is written
+    mu_wave_sync();
+#pragma unroll
+    for (int y = 0; y < NI; ++y)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *(float4 *)(lds + (lane & 31) * PITCH + 32 * y + 8 * q + 4 * (lane >> 5)) =
+                make_float4(acc[y][4 * q], acc[y][4 * q + 1], acc[y][4 * q + 2], acc[y][4 * q + 3]);
+    mu_wave_sync();
+    const bool back = MODE == MU_LAST ? !by_rows : mirror;
+#pragma unroll(MODE == MU_LAST ? 1 : 4)
+    for (int r = lane / LANES; r < 32; r += ROWS) {
+        const int c = (lane % LANES) * 4, i = i0 + r, j = j0 + c;
+        if (i >= it.np || j >= ld) continue;
+        float4 v = *(const float4 *)(lds + r * PITCH + c);
+        float4 *const old = (float4 *)(full + (size_t)i * ld + j);
+        const float4 o = MODE == MU_GRAM ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *old;
+        v = make_float4(k1 * o.x + k2 * v.x, k1 * o.y + k2 * v.y, k1 * o.z + k2 * v.z, k1 * o.w + k2 * v.w);
+        if (back) *(float4 *)(lds + r * PITCH + c) = v;
+        if (MODE == MU_LAST) {
+            if (by_rows && i < it.n && j < it.l) mu_update4(it, mat * it.ps[0] + i * it.ps[1] + j * it.ps[2], it.ps[2], min(4, it.l - j), v);
+        } else {
+            mu_h h0, h1, h2, h3, l0, l1, l2, l3;
+            mu_split(v.x, h0, l0), mu_split(v.y, h1, l1), mu_split(v.z, h2, l2), mu_split(v.w, h3, l3);
+            if (MODE != MU_POLY) *old = v; // B is a factor only
+            *(mu_h4 *)(out + (size_t)i * ld + j) = mu_h4{h0, h1, h2, h3};
+            *(mu_h4 *)(out + plane + (size_t)i * ld + j) = mu_h4{l0, l1, l2, l3};
+        }
+    }
+    if (!back) return;
+    mu_wave_sync();
+#pragma unroll(MODE == MU_LAST ? 1 : 2 * NI)
+    for (int s = 0; s < 2 * NI; ++s) {
+        const int c = s * 16 + lane / 4, r = (lane % 4) * 8, i = i0 + r, j = j0 + c;
+        if (i >= it.np || j >= ld) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = lds[(r + e) * PITCH + c];
+        if (MODE == MU_LAST) {
+            if (j >= it.l) continue;
+            const long long at = mat * it.ps[0] + i * it.ps[1] + j * it.ps[2];
+            if (i < it.n) mu_update4(it, at, it.ps[1], min(4, it.n - i), make_float4(v[0], v[1], v[2], v[3]));
+            if (i + 4 < it.n) mu_update4(it, at + 4 * it.ps[1], it.ps[1], min(4, it.n - i - 4), make_float4(v[4], v[5], v[6], v[7]));
+        } else {
+            mu_h8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                mu_h h, l;
+                mu_split(v[e], h, l);
+                hi[e] = h, lo[e] = l;
+            }
+            *(mu_h8 *)(out_t + (size_t)j * it.np + i) = hi;
+            *(mu_h8 *)(out_t + plane + (size_t)j * it.np + i) = lo;
+        }
+    }
+}
+
+// Where the tile with number `local` of a matrix lies, in tiles.  Four rows of tiles at a time, column by column: the tiles
+// that an XCD has in flight together are as square a block as can be, so that its L2 serves most of their loads.
+template <int MODE> __device__ __forceinline__ void mu_place(int local, int ti, int tj, int &i0, int &j0)
+{
+    i0 = 0, j0 = local;
+    if (MODE >= MU_APPLY) {
+        const int band = j0 / (4 * tj), h = min(4, ti - 4 * band);
+        j0 -= band * 4 * tj;
+        i0 = 4 * band + j0 % h;
+        j0 /= h;
+        return;
+    }
+    // the tiles on and above the diagonal: of each band first the triangle, then what lies right of it
+    int h = min(4, ti);
+    while (j0 >= h * (ti - i0) - h * (h - 1) / 2) {
+        j0 -= h * (ti - i0) - h * (h - 1) / 2;
+        i0 += 4;
+        h = min(4, ti - i0);
+    }
+    const int band = i0, triangle = h * (h + 1) / 2;
+    if (j0 < triangle) {
+        int r = 0;
+        while (j0 >= h - r) j0 -= h - r++;
+        i0 = band + r;
+        j0 += i0;
+    } else {
+        j0 -= triangle;
+        i0 = band + j0 % h;
+        j0 = band + h + j0 / h;
+    }
+}
+
+// neighbouring workgroups go to different XCDs: each of the eight takes a run of neighbouring tiles
+__device__ __forceinline__ int mu_by_xcd(int block, int total) { return (block & 7) * ((total + 7) / 8) + (block >> 3); }
+
 // One tile of a product.  LDS holds two stages of 32 k: rows of 64 bytes, P hi, P lo, Q hi, Q lo; the four 16-byte chunks of
 // a row lie at chunk ^ ((row >> 2) & 3), which spreads the 16 rows that a quarter wave reads over all 64 banks.  The loads go
 // from global memory to LDS directly, one stage ahead of the products.
@@ -269,41 +417,18 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     constexpr int WAVES = WM * WN, MI = T / WM / 32, NI = T / WN / 32, LOADS = 4 * T / 16 / WAVES;
     __shared__ __attribute__((aligned(1024))) char buf0[4 * T * 64];
     __shared__ __attribute__((aligned(1024))) char buf1[4 * T * 64];
-    // neighbouring workgroups go to different XCDs: each of the eight takes a run of neighbouring tiles
-    const int total = a.start[a.n_items], per_xcd = (total + 7) / 8;
-    const int tile = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (tile >= total) return;
+    // first the workgroups of the whole tiles, then those of the tiles that are cut along k
+    const int total = a.start[a.n_items], whole = (a.direct + 7) / 8 * 8, cut = total - a.direct;
+    const int unit = (int)blockIdx.x < whole ? mu_by_xcd(blockIdx.x, a.direct) : mu_by_xcd(blockIdx.x - whole, cut * a.splits);
+    const bool part = (int)blockIdx.x >= whole;
+    if (unit >= (part ? cut * a.splits : a.direct)) return;
+    const int tile = part ? a.direct + unit / a.splits : unit;
     const int k = mu_find(a, tile);
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
     const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
-    // Four rows of tiles at a time, column by column: the tiles that an XCD has in flight together are as square a block as
-    // can be, so that its L2 serves most of their loads.
-    int i0 = 0, j0 = local % per;
-    if (MODE >= MU_APPLY) {
-        const int band = j0 / (4 * tj), h = min(4, ti - 4 * band);
-        j0 -= band * 4 * tj;
-        i0 = 4 * band + j0 % h;
-        j0 /= h;
-    } else { // the tiles on and above the diagonal: of each band first the triangle, then what lies right of it
-        int h = min(4, ti);
-        while (j0 >= h * (ti - i0) - h * (h - 1) / 2) {
-            j0 -= h * (ti - i0) - h * (h - 1) / 2;
-            i0 += 4;
-            h = min(4, ti - i0);
-        }
-        const int band = i0, triangle = h * (h + 1) / 2;
-        if (j0 < triangle) {
-            int r = 0;
-            while (j0 >= h - r) j0 -= h - r++;
-            i0 = band + r;
-            j0 += i0;
-        } else {
-            j0 -= triangle;
-            i0 = band + j0 % h;
-            j0 = band + h + j0 / h;
-        }
-    }
+    int i0, j0;
+    mu_place<MODE>(local % per, ti, tj, i0, j0);
     i0 *= T, j0 *= T;
     const mu_mat w = mu_planes(a, it, mat);
     const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
@@ -323,6 +448,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
         off_p[q] = ((uint32_t)min(row, it.np - 1 - i0) * (uint32_t)K + chunk * 8) * 2;
         off_q[q] = ((uint32_t)min(row, jrows - 1 - j0) * (uint32_t)K + chunk * 8) * 2;
     }
+    // this workgroup's k, in units of 64
+    const int units = K / 64, k_first = part ? (int)((long long)units * (unit % a.splits) / a.splits) * 64 : 0;
+    const int k_end = part ? (int)((long long)units * (unit % a.splits + 1) / a.splits) * 64 : K;
     const char *const base_p = (const char *)(P + (size_t)i0 * K), *const base_q = (const char *)(Q + (size_t)j0 * K);
 
     mu_f16 acc[MI][NI];
@@ -393,93 +521,140 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
         __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0), lgkmcnt(0): the next stage is there, this one is read
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        stage(buf, min(k0 + 2 * MU_BK, K - MU_BK));
+        stage(buf, min(k0 + 2 * MU_BK, k_end - MU_BK));
         read(f0, next, 0);
         products(f1);
     };
-    stage(buf0, 0);
-    stage(buf1, MU_BK);
+    stage(buf0, k_first);
+    stage(buf1, k_first + MU_BK);
     __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS); // vmcnt(LOADS): the first stage
     lrb_barrier();
     read(f0, buf0, 0);
-    for (int k0 = 0; k0 < K; k0 += 2 * MU_BK) {
+    for (int k0 = k_first; k0 < k_end; k0 += 2 * MU_BK) {
         turn(buf0, buf1, k0);
         turn(buf1, buf0, k0 + MU_BK);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);
     lrb_barrier();
 
-    // lane -> row i of C, four neighbouring columns j in every four registers
-    const float *t = a.table + ((size_t)(it.first + mat) * a.steps + a.step) * MU_COEF;
-    const float k1 = MODE == MU_GRAM ? 0.0f : MODE == MU_POLY ? t[1] : t[3], k2 = MODE == MU_GRAM ? t[0] : MODE == MU_POLY ? t[2] : t[4];
-    const int ld = MODE >= MU_APPLY ? it.lp : it.np;
-    const size_t plane = (size_t)it.np * ld;
-    float *full = MODE <= MU_POLY ? w.a32 : w.x32;
-    mu_h *out = MODE == MU_GRAM ? w.a : MODE == MU_POLY ? w.b : w.x2, *out_t = MODE == MU_APPLY ? w.xt2 : out;
+    if (part) { // the sums as they lie in the registers: mu_join_kernel adds them up
+        float4 *const out = (float4 *)(a.parts + (size_t)unit * T * T) + (size_t)wave * MI * NI * 256 + lane;
+#pragma unroll
+        for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int y = 0; y < NI; ++y)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    out[((x * NI + y) * 4 + q) * 64] =
+                        make_float4(acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2], acc[x][y][4 * q + 3]);
+        return;
+    }
+    constexpr int HALF = WAVES / 2, LDS_WAVE = 32 * MU_PITCH(NI) * 4;
+    static_assert(HALF * LDS_WAVE <= 4 * T * 64, "");
+    float *const lds = (float *)((wave < HALF ? buf0 : buf1) + (wave % HALF) * LDS_WAVE);
     const bool mirror = MODE == MU_APPLY || i0 != j0;
 #pragma unroll
     for (int x = 0; x < MI; ++x)
+        mu_strip<MODE, NI>(a, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane);
+}
+
+// The tiles that were cut along k: their parts' sums, added up in order, a wave for each 32 rows of one of the tile's waves.
+template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void mu_join_kernel(mu_args a)
+{
+    constexpr int WAVES = WM * WN, MI = T / WM / 32, NI = T / WN / 32;
+    __shared__ float lds[32 * MU_PITCH(NI)];
+    const int lane = threadIdx.x, r = blockIdx.x / (WAVES * MI), strip = blockIdx.x % (WAVES * MI), wave = strip / MI, x = strip % MI;
+    const int tile = a.direct + r, k = mu_find(a, tile);
+    const mu_item &it = a.it[k];
+    const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
+    const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
+    int i0, j0;
+    mu_place<MODE>(local % per, ti, tj, i0, j0);
+    i0 *= T, j0 *= T;
+    const int wi = wave / WN, wj = wave % WN;
+    mu_f16 acc[NI];
+#pragma unroll
+    for (int y = 0; y < NI; ++y)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[y][v] = 0.0f;
+    const float4 *in = (const float4 *)(a.parts + (size_t)r * a.splits * T * T) + (size_t)strip * NI * 256 + lane;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s, in += T * T / 4)
 #pragma unroll
         for (int y = 0; y < NI; ++y)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int i = i0 + (wi * MI + x) * 32 + frow, j = j0 + (wj * NI + y) * 32 + 8 * q + 4 * fchunk;
-                if (i >= it.np || j >= jrows) continue;
-                float4 v = {};
-                float4 *const old = (float4 *)(full + (size_t)i * ld + j);
-                if (MODE != MU_GRAM) v = *old;
-                v.x = k1 * v.x + k2 * acc[x][y][4 * q], v.y = k1 * v.y + k2 * acc[x][y][4 * q + 1];
-                v.z = k1 * v.z + k2 * acc[x][y][4 * q + 2], v.w = k1 * v.w + k2 * acc[x][y][4 * q + 3];
-                if (MODE == MU_LAST) {
-                    if (i >= it.n) continue;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (j + e >= it.l) continue;
-                        const long long at = mat * it.ps[0] + i * it.ps[1] + (j + e) * it.ps[2];
-                        const float before = it.decay != 0.0f ? it.decay * mu_load(it.p, at, it.p_type) : 0.0f;
-                        mu_store(it.p, at, it.p_type, before + it.alpha * (&v.x)[e]);
-                    }
-                } else {
-                    mu_h4 h4, l4;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        mu_h hi, lo;
-                        mu_split((&v.x)[e], hi, lo);
-                        h4[e] = hi, l4[e] = lo;
-                    }
-                    if (MODE != MU_POLY) *old = v; // B is a factor only
-                    *(mu_h4 *)(out + (size_t)i * ld + j) = h4;
-                    *(mu_h4 *)(out + plane + (size_t)i * ld + j) = l4;
-                    if (mirror) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            out_t[(size_t)(j + e) * it.np + i] = h4[e];
-                            out_t[plane + (size_t)(j + e) * it.np + i] = l4[e];
-                        }
-                    }
-                }
+                const float4 v = in[(y * 4 + q) * 64];
+                acc[y][4 * q] += v.x, acc[y][4 * q + 1] += v.y, acc[y][4 * q + 2] += v.z, acc[y][4 * q + 3] += v.w;
             }
+    const mu_mat w = mu_planes(a, it, mat);
+    mu_strip<MODE, NI>(a, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
+}
+
+// How a product's launch is laid out.
+struct mu_plan {
+    int T;             // side of a tile
+    long long tiles;
+    int direct, splits; // the first `direct` tiles are whole, the others are cut into `splits` along k
+    uint64_t part_bytes() const { return splits > 1 ? (uint64_t)(tiles - direct) * splits * T * T * 4 : 0; }
+};
+
+static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
+{
+    long long sum = 0;
+    for (int k = 0; k < a.n_items; ++k) {
+        if (start) start[k] = (int)sum;
+        const long long ti = (a.it[k].np + T - 1) / T, tj = (a.it[k].lp + T - 1) / T;
+        sum += a.it[k].count * (symmetric ? ti * (ti + 1) / 2 : ti * tj);
+    }
+    if (start) start[a.n_items] = (int)sum;
+    return sum;
+}
+
+// The tile: the largest that still gives most of the 256 CUs one (a larger tile loads less for each product).  Both symmetric
+// products take the same (A in float32 is there on and above the diagonal's tiles only).
+// The cut: a CU holds one, two or four workgroups by their LDS, so 256, 512 or 1024 tiles run side by side and take the same
+// time; the tiles of the last, unfilled round are cut along k so that all CUs share them.
+static mu_plan mu_lay_out(const mu_args &a, int mode)
+{
+    const bool symmetric = mode <= MU_POLY;
+    mu_plan p;
+    p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 200 ? 128 : 64;
+    p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
+    const int slots = p.T == 256 ? 256 : p.T == 128 ? 512 : 1024;
+    const long long rest = p.tiles % slots;
+    p.direct = (int)p.tiles, p.splits = 1;
+    if (rest == 0) return p;
+    long long units = 1ll << 40; // of 64 k, in the shortest of the rest's products
+    long long before = 0;
+    for (int k = 0; k < a.n_items; ++k) {
+        const long long ti = (a.it[k].np + p.T - 1) / p.T, tj = (a.it[k].lp + p.T - 1) / p.T;
+        before += a.it[k].count * (symmetric ? ti * (ti + 1) / 2 : ti * tj);
+        const long long u = (mode == MU_GRAM ? a.it[k].lp : a.it[k].np) / 64;
+        if (before > p.tiles - rest && u < units) units = u;
+    }
+    long long s = slots / rest;
+    if (s > units / 4) s = units / 4; // 256 k a part at least
+    if (s < 2 || units - units / s < 8) return p; // what is saved would not pay for the joining launch
+    p.direct = (int)(p.tiles - rest), p.splits = (int)s;
+    return p;
+}
+
+template <int T, int WM, int WN, int MODE> static void mu_launch_tiles(const mu_args &a, const mu_plan &p, hipStream_t st)
+{
+    const long long cut = p.tiles - p.direct, units = cut * p.splits;
+    hipLaunchKernelGGL((mu_product_kernel<T, WM, WN, MODE>), dim3((unsigned)((p.direct + 7) / 8 * 8 + (units + 7) / 8 * 8)), dim3(64 * WM * WN), 0, st, a);
+    if (cut) hipLaunchKernelGGL((mu_join_kernel<T, WM, WN, MODE>), dim3((unsigned)(cut * (T / 32) * WN)), dim3(64), 0, st, a);
 }
 
 template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
 {
-    auto tiles = [&](int T, bool keep) {
-        long long sum = 0;
-        for (int k = 0; k < a.n_items; ++k) {
-            if (keep) a.start[k] = (int)sum;
-            const long long ti = (a.it[k].np + T - 1) / T, tj = (a.it[k].lp + T - 1) / T;
-            sum += a.it[k].count * (MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2);
-        }
-        if (keep) a.start[a.n_items] = (int)sum;
-        return sum;
-    };
-    // the largest tile that still gives most of the 256 CUs one: a larger tile loads less for each product
-    const int T = MODE != MU_LAST && tiles(256, false) >= 200 ? 256 : tiles(128, false) >= 200 ? 128 : 64;
-    const long long total = tiles(T, true);
-    const dim3 grid((unsigned)((total + 7) / 8 * 8));
-    if (T == 256) hipLaunchKernelGGL((mu_product_kernel<256, 2, 4, MODE == MU_LAST ? MU_APPLY : MODE>), grid, dim3(512), 0, st, a);
-    else if (T == 128) hipLaunchKernelGGL((mu_product_kernel<128, 2, 2, MODE>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((mu_product_kernel<64, 2, 2, MODE>), grid, dim3(256), 0, st, a);
+    const mu_plan p = mu_lay_out(a, MODE);
+    mu_tiles(a, MODE <= MU_POLY, p.T, a.start);
+    a.direct = p.direct, a.splits = p.splits;
+    if (p.T == 256) mu_launch_tiles<256, 2, 4, MODE>(a, p, st);
+    else if (p.T == 128) mu_launch_tiles<128, 2, 2, MODE>(a, p, st);
+    else mu_launch_tiles<64, 2, 2, MODE>(a, p, st);
 }
 
 // A run of items (or of some matrices of one) that fits the descriptors and MU_WS_MOST bytes, and what it takes.
@@ -492,7 +667,12 @@ struct mu_group {
     uint64_t planes;
     uint64_t bytes() const
     {
-        return planes + ((uint64_t)mats * 8 + 255) / 256 * 256 + ((uint64_t)tiles * 8 + 255) / 256 * 256 +
+        uint64_t parts = 0;
+        for (int mode = MU_GRAM; mode <= MU_LAST; ++mode) {
+            const uint64_t b = mu_lay_out(a, mode).part_bytes();
+            parts = b > parts ? b : parts;
+        }
+        return planes + parts + ((uint64_t)mats * 8 + 255) / 256 * 256 + ((uint64_t)tiles * 8 + 255) / 256 * 256 +
                ((uint64_t)mats * MU_STEPS * MU_COEF * 4 + 255) / 256 * 256;
     }
 };
@@ -596,7 +776,8 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
         char *at = g.ws + gr.planes;
         g.x0 = (double *)at, at += ((uint64_t)gr.mats * 8 + 255) / 256 * 256;
         g.part = (double *)at, at += ((uint64_t)gr.tiles * 8 + 255) / 256 * 256;
-        g.table = (float *)at;
+        g.table = (float *)at, at += ((uint64_t)gr.mats * MU_STEPS * MU_COEF * 4 + 255) / 256 * 256;
+        g.parts = (float *)at;
         g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
         hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
         hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
