@@ -62,14 +62,16 @@ struct mu_args {
     mu_item it[MU_ITEMS];
 };
 
-// The planes of a matrix: X and its transpose twice (read and written in turn), A, B, hi then lo in each; and X and A in
+// The factors of a matrix: X and its transpose twice (read and written in turn), A, B, as rows of 32 hi, the 32 lo of the same
+// entries, the next 32 hi ...: 32 k of a row are one whole line of 128 bytes, which halves the requests that the L2 gets for a
+// stage against separate planes (2.1 -> 1.05 requests for 128 bytes).  And X and A in
 // float32, for the terms a X and b A: hi + lo is a rounding more than float32 is, and these terms would pass it on.
 __host__ __device__ inline unsigned long long mu_plane_x(const mu_item &it) { return 2ull * (unsigned long long)it.np * it.lp; }
 __host__ __device__ inline unsigned long long mu_plane_a(const mu_item &it) { return 2ull * (unsigned long long)it.np * it.np; }
 __host__ __device__ inline unsigned long long mu_bytes(const mu_item &it) { return 10 * mu_plane_x(it) + 6 * mu_plane_a(it); }
 
 struct mu_mat {
-    mu_h *x, *xt, *x2, *xt2, *a, *b; // lo planes follow their hi planes
+    mu_h *x, *xt, *x2, *xt2, *a, *b;
     float *x32, *a32;
 };
 __device__ __forceinline__ mu_mat mu_planes(const mu_args &a, const mu_item &it, int mat)
@@ -87,6 +89,9 @@ __device__ __forceinline__ mu_mat mu_planes(const mu_args &a, const mu_item &it,
     r.a32 = (float *)(w + 5 * px + 2 * pa);
     return r;
 }
+
+// hi of entry (row, k) of a factor with rows of `len`; lo lies 32 further
+__device__ __forceinline__ size_t mu_at(int row, int k, int len) { return (size_t)row * 2 * len + (k >> 5) * 64 + (k & 31); }
 
 __device__ __forceinline__ float mu_load(const void *p, long long at, int type)
 {
@@ -228,13 +233,12 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
     }
     lrb_barrier();
     const mu_mat w = mu_planes(a, it, mat);
-    const size_t plane = (size_t)it.np * it.lp;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int q = e * 256 + threadIdx.x, row = q >> 3, c = (q & 7) * 8;
         float v[8];
         mu_h8 hi, lo;
-        const size_t at = (size_t)(i0 + row) * it.lp + j0 + c, at_t = (size_t)(j0 + row) * it.np + i0 + c;
+        const size_t at = mu_at(i0 + row, j0 + c, it.lp), at_t = mu_at(j0 + row, i0 + c, it.np);
 #pragma unroll
         for (int e8 = 0; e8 < 8; ++e8) {
             mu_h h, l;
@@ -242,9 +246,9 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
             mu_split(v[e8], h, l);
             hi[e8] = h, lo[e8] = l;
         }
-        __builtin_memcpy(w.x32 + at, v, 32);
+        __builtin_memcpy(w.x32 + (size_t)(i0 + row) * it.lp + j0 + c, v, 32);
         *(mu_h8 *)(w.x + at) = hi;
-        *(mu_h8 *)(w.x + plane + at) = lo;
+        *(mu_h8 *)(w.x + at + 32) = lo;
 #pragma unroll
         for (int e8 = 0; e8 < 8; ++e8) {
             mu_h h, l;
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
             hi[e8] = h, lo[e8] = l;
         }
         *(mu_h8 *)(w.xt + at_t) = hi;
-        *(mu_h8 *)(w.xt + plane + at_t) = lo;
+        *(mu_h8 *)(w.xt + at_t + 32) = lo;
     }
 }
 
@@ -313,7 +317,6 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, in
     const float *t = a.table + ((size_t)(it.first + mat) * a.steps + a.step) * MU_COEF;
     const float k1 = MODE == MU_GRAM ? 0.0f : MODE == MU_POLY ? t[1] : t[3], k2 = MODE == MU_GRAM ? t[0] : MODE == MU_POLY ? t[2] : t[4];
     const int ld = MODE >= MU_APPLY ? it.lp : it.np;
-    const size_t plane = (size_t)it.np * ld;
     float *full = MODE <= MU_POLY ? w.a32 : w.x32;
     mu_h *out = MODE == MU_GRAM ? w.a : MODE == MU_POLY ? w.b : w.x2, *out_t = MODE == MU_APPLY ? w.xt2 : out;
     const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1; // which way p is written
@@ -341,8 +344,8 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, in
             mu_h h0, h1, h2, h3, l0, l1, l2, l3;
             mu_split(v.x, h0, l0), mu_split(v.y, h1, l1), mu_split(v.z, h2, l2), mu_split(v.w, h3, l3);
             if (MODE != MU_POLY) *old = v; // B is a factor only
-            *(mu_h4 *)(out + (size_t)i * ld + j) = mu_h4{h0, h1, h2, h3};
-            *(mu_h4 *)(out + plane + (size_t)i * ld + j) = mu_h4{l0, l1, l2, l3};
+            *(mu_h4 *)(out + mu_at(i, j, ld)) = mu_h4{h0, h1, h2, h3};
+            *(mu_h4 *)(out + mu_at(i, j, ld) + 32) = mu_h4{l0, l1, l2, l3};
         }
     }
     if (!back) return;
@@ -367,8 +370,8 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, in
                 mu_split(v[e], h, l);
                 hi[e] = h, lo[e] = l;
             }
-            *(mu_h8 *)(out_t + (size_t)j * it.np + i) = hi;
-            *(mu_h8 *)(out_t + plane + (size_t)j * it.np + i) = lo;
+            *(mu_h8 *)(out_t + mu_at(j, i, it.np)) = hi;
+            *(mu_h8 *)(out_t + mu_at(j, i, it.np) + 32) = lo;
         }
     }
 }
@@ -408,13 +411,13 @@ template <int MODE> __device__ __forceinline__ void mu_place(int local, int ti, 
 // neighbouring workgroups go to different XCDs: each of the eight takes a run of neighbouring tiles
 __device__ __forceinline__ int mu_by_xcd(int block, int total) { return (block & 7) * ((total + 7) / 8) + (block >> 3); }
 
-// One tile of a product.  LDS holds two stages of 32 k: rows of 64 bytes, P hi, P lo, Q hi, Q lo; the four 16-byte chunks of
-// a row lie at chunk ^ ((row >> 2) & 3), which spreads the 16 rows that a quarter wave reads over all 64 banks.  The loads go
-// from global memory to LDS directly, one stage ahead of the products.
+// One tile of a product.  LDS holds two stages of 32 k: T rows of P and T of Q, 128 bytes each; the eight 16-byte chunks of a
+// row (four of hi, four of lo) lie at chunk ^ ((row >> 1) & 7), which spreads the 16 rows that a quarter wave reads over all
+// 64 banks.  The loads go from global memory to LDS directly, one stage ahead of the products.
 template <int T, int WM, int WN, int MODE>
 __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 {
-    constexpr int WAVES = WM * WN, MI = T / WM / 32, NI = T / WN / 32, LOADS = 4 * T / 16 / WAVES;
+    constexpr int WAVES = WM * WN, MI = T / WM / 32, NI = T / WN / 32;
     __shared__ __attribute__((aligned(1024))) char buf0[4 * T * 64];
     __shared__ __attribute__((aligned(1024))) char buf1[4 * T * 64];
     // first the workgroups of the whole tiles, then those of the tiles that are cut along k
@@ -433,25 +436,23 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const mu_mat w = mu_planes(a, it, mat);
     const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
     const mu_h *P = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.b, *Q = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.xt;
-    const size_t p_plane = (size_t)it.np * K, q_plane = (size_t)jrows * K;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN, wj = wave % WN;
 
-    // A load of a wave fills 16 rows of a stage.  All addresses are a plane's first row of the tile (uniform) and an offset of
+    // A load of a wave fills eight rows of a stage.  All addresses are a factor's first row of the tile (uniform) and an offset of
     // the lane's row in it (32 bits: 256 rows of up to 2^22 entries); rows past the padding (tiles larger than 64) repeat the last
     // one, and what they give is not stored.
-    constexpr int ROWS = WAVES * 16, HALVES = T / ROWS; // rows that the waves fill together; such fills a part
-    static_assert(HALVES * 4 == LOADS, "");
-    uint32_t off_p[HALVES], off_q[HALVES];
+    constexpr int ROWS = WAVES * 8, FILLS = T / ROWS; // rows that the waves fill together; such fills of P, and of Q
+    uint32_t off_p[FILLS], off_q[FILLS];
 #pragma unroll
-    for (int q = 0; q < HALVES; ++q) {
-        const int row = q * ROWS + wave * 16 + (lane >> 2), chunk = (lane & 3) ^ ((row >> 2) & 3);
-        off_p[q] = ((uint32_t)min(row, it.np - 1 - i0) * (uint32_t)K + chunk * 8) * 2;
-        off_q[q] = ((uint32_t)min(row, jrows - 1 - j0) * (uint32_t)K + chunk * 8) * 2;
+    for (int q = 0; q < FILLS; ++q) {
+        const int row = q * ROWS + wave * 8 + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
+        off_p[q] = (uint32_t)min(row, it.np - 1 - i0) * (uint32_t)K * 4 + chunk * 16;
+        off_q[q] = (uint32_t)min(row, jrows - 1 - j0) * (uint32_t)K * 4 + chunk * 16;
     }
     // this workgroup's k, in units of 64
     const int units = K / 64, k_first = part ? (int)((long long)units * (unit % a.splits) / a.splits) * 64 : 0;
     const int k_end = part ? (int)((long long)units * (unit % a.splits + 1) / a.splits) * 64 : K;
-    const char *const base_p = (const char *)(P + (size_t)i0 * K), *const base_q = (const char *)(Q + (size_t)j0 * K);
+    const char *const base_p = (const char *)(P + (size_t)i0 * 2 * K), *const base_q = (const char *)(Q + (size_t)j0 * 2 * K);
 
     mu_f16 acc[MI][NI];
 #pragma unroll
@@ -463,33 +464,31 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 
     const int frow = lane & 31, fchunk = lane >> 5;
     auto stage = [&](char *buf, int k0) {
-        const char *const p = base_p + 2 * (size_t)k0, *const q = base_q + 2 * (size_t)k0;
-        const int d = wave * 1024;
+        const char *const p = base_p + 4 * (size_t)k0, *const q = base_q + 4 * (size_t)k0;
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-            mu_dma(p + off_p[h], buf + h * ROWS * 64 + d);
-            mu_dma(p + 2 * p_plane + off_p[h], buf + T * 64 + h * ROWS * 64 + d);
-            mu_dma(q + off_q[h], buf + 2 * T * 64 + h * ROWS * 64 + d);
-            mu_dma(q + 2 * q_plane + off_q[h], buf + 3 * T * 64 + h * ROWS * 64 + d);
+        for (int h = 0; h < FILLS; ++h) {
+            mu_dma(p + off_p[h], buf + (h * ROWS + wave * 8) * 128);
+            mu_dma(q + off_q[h], buf + (T + h * ROWS + wave * 8) * 128);
         }
         __builtin_amdgcn_sched_barrier(0); // else the compiler sinks the loads to the wait that ends the stage
     };
     struct frags {
         mu_h8 ph[MI], pl[MI], qh[NI], ql[NI];
     };
-    // the chunk of a row does not depend on which 32 rows it is among: (row >> 2) & 3 == (frow >> 2) & 3
-    const int at0 = frow * 64 + ((fchunk ^ ((frow >> 2) & 3)) << 4), at1 = frow * 64 + (((2 + fchunk) ^ ((frow >> 2) & 3)) << 4);
+    // the chunk of a row does not depend on which 32 rows it is among: (row >> 1) & 7 == (frow >> 1) & 7
+    const int at = frow * 128 + ((fchunk ^ ((frow >> 1) & 7)) << 4);
     auto read = [&](frags &f, const char *buf, int kk) {
-        const char *const p = buf + wi * MI * 2048 + (kk ? at1 : at0), *const q = buf + 2 * T * 64 + wj * NI * 2048 + (kk ? at1 : at0);
+        const char *const p = buf + wi * MI * 4096, *const q = buf + T * 128 + wj * NI * 4096;
+        const int hi = at ^ (kk * 32), lo = hi ^ 64;
 #pragma unroll
         for (int y = 0; y < NI; ++y) {
-            f.qh[y] = *(const mu_h8 *)(q + y * 2048);
-            f.ql[y] = *(const mu_h8 *)(q + T * 64 + y * 2048);
+            f.qh[y] = *(const mu_h8 *)(q + y * 4096 + hi);
+            f.ql[y] = *(const mu_h8 *)(q + y * 4096 + lo);
         }
 #pragma unroll
         for (int x = 0; x < MI; ++x) {
-            f.ph[x] = *(const mu_h8 *)(p + x * 2048);
-            f.pl[x] = *(const mu_h8 *)(p + T * 64 + x * 2048);
+            f.ph[x] = *(const mu_h8 *)(p + x * 4096 + hi);
+            f.pl[x] = *(const mu_h8 *)(p + x * 4096 + lo);
         }
     };
     auto products = [&](const frags &f) {
@@ -527,7 +526,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     };
     stage(buf0, k_first);
     stage(buf1, k_first + MU_BK);
-    __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS); // vmcnt(LOADS): the first stage
+    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
     lrb_barrier();
     read(f0, buf0, 0);
     for (int k0 = k_first; k0 < k_end; k0 += 2 * MU_BK) {
