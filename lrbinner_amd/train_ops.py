@@ -26,8 +26,9 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # LRB_F32, LRB
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# hipStream_t of torch's current stream on a device, by its index (a call of torch.cuda.current_stream costs a small
+# operator as much as its launch)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _known_type(t, name):
@@ -43,63 +44,78 @@ def _rows(t, cols):
     return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _packed(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, stats):
+    """y, and with `stats` the float32 [2, rows] of means and 1 / deviations that the backward pass takes."""
     cols = x.shape[-1]
     rows = x.numel() // cols
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        both = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        mean, rstd = both[0], both[1]
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
     if rows:
-        x2 = _rows(x, cols)
+        stride = cols
+        if not x.is_contiguous():
+            x = _rows(x, cols)
+            stride = x.stride(0)
+        weight, bias, keep = _packed(weight), _packed(bias), _packed(keep)
         ref = weight if weight is not None else bias
-        weight = weight if weight is None else weight.contiguous()
-        bias = bias if bias is None else bias.contiguous()
-        keep = keep if keep is None else keep.contiguous()
-        check("lrb_layer_norm_fwd_dev", _lib.lib().lrb_layer_norm_fwd_dev(
-            x.device.index, _stream(x.device), _TYPES[x.dtype], 0 if ref is None else _TYPES[ref.dtype], rows, cols,
-            x2.data_ptr(), x2.stride(0), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
-            eps, slope, None if keep is None else keep.data_ptr(), keep_scale, y.data_ptr(),
-            mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None))
-    return y, mean, rstd
+        at = _address(stats)
+        index = x.device.index
+        rc = _lib.lib().lrb_layer_norm_fwd_dev(
+            index, _stream(index), _TYPES[x.dtype], 0 if ref is None else _TYPES[ref.dtype], rows, cols, x.data_ptr(), stride,
+            _address(weight), _address(bias), eps, slope, _address(keep), keep_scale, y.data_ptr(), at, at and at + 4 * rows)
+        if rc:
+            check("lrb_layer_norm_fwd_dev", rc)
+    return y, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, keep, eps, slope, keep_scale):
-        y, mean, rstd = _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, True)
-        ctx.save_for_backward(x, weight, keep, mean, rstd)
-        ctx.bias_type = None if bias is None else bias.dtype
-        ctx.slope, ctx.keep_scale = slope, keep_scale
+        y, stats = _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, True)
+        ctx.save_for_backward(x, weight, keep, stats)
+        ctx.more = None if bias is None else bias.dtype, slope, keep_scale
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, keep, mean, rstd = ctx.saved_tensors
+        x, weight, keep, stats = ctx.saved_tensors
+        bias_type, slope, keep_scale = ctx.more
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         cols = x.shape[-1]
         rows = x.numel() // cols
-        w_type = weight.dtype if weight is not None else ctx.bias_type
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        w_type = weight.dtype if weight is not None else bias_type
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
         dw = torch.empty(cols, dtype=w_type, device=x.device) if need_w else None
         db = torch.empty(cols, dtype=w_type, device=x.device) if need_b else None
         lib = _lib.lib()
+        x_type = _TYPES[x.dtype]
         ws, ws_bytes = None, 0
         if need_w or need_b:
-            ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(_TYPES[x.dtype], rows, cols)
+            ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(x_type, rows, cols)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-        x2, dy2 = _rows(x, cols), _rows(dy, cols)
-        weight = weight if weight is None else weight.contiguous()
-        keep = keep if keep is None else keep.contiguous()
-        check("lrb_layer_norm_bwd_dev", lib.lrb_layer_norm_bwd_dev(
-            x.device.index, _stream(x.device), _TYPES[x.dtype], 0 if w_type is None else _TYPES[w_type], rows, cols,
-            x2.data_ptr() if rows else None, x2.stride(0), dy2.data_ptr() if rows else None, dy2.stride(0),
-            None if weight is None else weight.data_ptr(), mean.data_ptr() if rows else None, rstd.data_ptr() if rows else None,
-            ctx.slope, None if keep is None or not rows else keep.data_ptr(), ctx.keep_scale,
-            dx.data_ptr() if need_x and rows else None, dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None,
-            None if ws is None else ws.data_ptr(), ws_bytes))
+        x_stride = dy_stride = cols
+        if not x.is_contiguous():
+            x = _rows(x, cols)
+            x_stride = x.stride(0)
+        if not dy.is_contiguous():
+            dy = _rows(dy, cols)
+            dy_stride = dy.stride(0)
+        weight, keep = _packed(weight), _packed(keep)
+        index, at = x.device.index, stats.data_ptr() or None
+        rc = lib.lrb_layer_norm_bwd_dev(
+            index, _stream(index), x_type, 0 if w_type is None else _TYPES[w_type], rows, cols, x.data_ptr() or None, x_stride,
+            dy.data_ptr() or None, dy_stride, _address(weight), at, at and at + 4 * rows, slope, _address(keep) or None, keep_scale,
+            _address(dx) or None, _address(dw), _address(db), _address(ws), ws_bytes)
+        if rc:
+            check("lrb_layer_norm_bwd_dev", rc)
         return dx, dw, db, None, None, None, None
 
 
@@ -125,34 +141,36 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, slope=1.0, keep=None, kee
     keep * keep_scale * leaky_relu(x); what is dropped counts as 0 whatever it holds.  ``weight`` and ``bias``: one element a
     column, float32 or of x's type (both alike), or None.  x may have any leading axes and strides; a copy is made only
     where the elements of a row are not side by side, or the rows not evenly spaced.  The statistics are float32."""
-    _known_type(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x: at least one column is wanted, not shape {tuple(x.shape)}")
-    if not (eps >= 0.0 and math.isfinite(eps)):
+    dtype, shape, device = x.dtype, x.shape, x.device
+    if dtype not in _TYPES:
+        _known_type(x, "x")
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"x: at least one column is wanted, not shape {tuple(shape)}")
+    if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps: {eps}")
     if not (math.isfinite(slope) and math.isfinite(keep_scale)):
         raise ValueError(f"slope {slope}, keep_scale {keep_scale}: finite numbers are wanted")
-    cols = x.shape[-1]
+    cols = shape[-1]
     grad = x.requires_grad
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if t.dim() != 1 or t.shape[0] != cols:
+        if t.shape != (cols,):
             raise ValueError(f"{name}: shape ({cols},) is wanted, not {tuple(t.shape)}")
-        if t.dtype != torch.float32 and t.dtype != x.dtype:
-            raise TypeError(f"{name}: float32 or {x.dtype} is wanted, not {t.dtype}")
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        if t.dtype is not torch.float32 and t.dtype is not dtype:
+            raise TypeError(f"{name}: float32 or {dtype} is wanted, not {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, x on {device}")
         grad = grad or t.requires_grad
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise TypeError(f"weight and bias: one type is wanted, not {weight.dtype} and {bias.dtype}")
     if keep is not None:
-        if keep.shape != x.shape:
-            raise ValueError(f"keep: shape {tuple(x.shape)} is wanted, not {tuple(keep.shape)}")
-        if keep.dtype not in (torch.bool, torch.uint8):
+        if keep.shape != shape:
+            raise ValueError(f"keep: shape {tuple(shape)} is wanted, not {tuple(keep.shape)}")
+        if keep.dtype is not torch.bool and keep.dtype is not torch.uint8:
             raise TypeError(f"keep: bool or uint8 is wanted, not {keep.dtype}")
-        if keep.device != x.device:
-            raise ValueError(f"keep is on {keep.device}, x on {x.device}")
+        if keep.device != device:
+            raise ValueError(f"keep is on {keep.device}, x on {device}")
     else:
         keep_scale = 1.0
     if not x.is_cuda:
@@ -218,7 +236,7 @@ def _muon_call(device, items, momentum, nesterov, steps, coefficients, eps):
     ws_bytes = lib.lrb_muon_ws_bytes(raw, len(items))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     a, b, c = coefficients
-    check("lrb_muon_dev", lib.lrb_muon_dev(device.index, _stream(device), raw, len(items), momentum, 1 if nesterov else 0, int(steps),
+    check("lrb_muon_dev", lib.lrb_muon_dev(device.index, _stream(device.index), raw, len(items), momentum, 1 if nesterov else 0, int(steps),
                                            a, b, c, eps, ws.data_ptr() if ws_bytes else None, ws_bytes))
 
 
