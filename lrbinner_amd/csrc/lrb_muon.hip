@@ -19,6 +19,7 @@
 // products the tiles on and above the diagonal are computed and mirrored.  Tiles of all weights of a call share a launch.
 #include <limits.h>
 #include <math.h>
+#include <string.h>
 
 #include "lrb_device.h"
 
@@ -58,9 +59,12 @@ struct mu_args {
     // of a product's launch: the tiles from `direct` on are cut along k, `splits` workgroups each, whose sums go to `parts`
     int direct, splits;
     float *parts;
+    double sx;                      // the scale of X at the start, and the table, for a norm of at least eps
+    float std[MU_STEPS * MU_COEF];
     int start[MU_ITEMS + 1]; // first tile of each item in this launch
     mu_item it[MU_ITEMS];
 };
+static_assert(sizeof(mu_args) <= 4096, "kernel arguments");
 
 // The factors of a matrix: X and its transpose twice (read and written in turn), A, B, as rows of 32 hi, the 32 lo of the same
 // entries, the next 32 hi ...: 32 k of a row are one whole line of 128 bytes, which halves the requests that the L2 gets for a
@@ -112,19 +116,29 @@ __device__ __forceinline__ int mu_find(const mu_args &a, int tile)
     return k;
 }
 
-// u at (i, j); UPDATE also writes the momentum back (each entry by one thread)
-template <bool UPDATE> __device__ __forceinline__ float mu_u(const mu_args &a, const mu_item &it, int mat, int i, int j)
+// u at N places (row i(e), column j(e), where they lie inside), 0 elsewhere.  All loads are issued before the first result is
+// used.  UPDATE also writes the momentum back (each entry by one thread).
+template <bool UPDATE, int N, typename I, typename J>
+__device__ __forceinline__ void mu_u(float beta, int nesterov, const mu_item &it, int mat, I i, J j, float (&u)[N])
 {
-    const float g = mu_load(it.g, mat * it.gs[0] + i * it.gs[1] + j * it.gs[2], it.g_type);
-    if (!it.m) return g;
-    const long long at = mat * it.ms[0] + i * it.ms[1] + j * it.ms[2];
-    float m = mu_load(it.m, at, it.m_type);
-    if (UPDATE) {
-        m = a.beta * m + (1.0f - a.beta) * g;
-        mu_store(it.m, at, it.m_type, m);
-        m = it.m_type == LRB_F32 ? m : it.m_type == LRB_BF16 ? (float)(__bf16)m : (float)(mu_h)m; // u is made of what is kept
+    float m[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const bool in = i(e) < it.n && j(e) < it.l;
+        u[e] = in ? mu_load(it.g, mat * it.gs[0] + i(e) * it.gs[1] + j(e) * it.gs[2], it.g_type) : 0.0f;
+        m[e] = in && it.m ? mu_load(it.m, mat * it.ms[0] + i(e) * it.ms[1] + j(e) * it.ms[2], it.m_type) : 0.0f;
     }
-    return a.nesterov ? (1.0f - a.beta) * g + a.beta * m : m;
+    if (!it.m) return;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (UPDATE) {
+            m[e] = beta * m[e] + (1.0f - beta) * u[e];
+            if (i(e) < it.n && j(e) < it.l) mu_store(it.m, mat * it.ms[0] + i(e) * it.ms[1] + j(e) * it.ms[2], it.m_type, m[e]);
+            // u is made of what is kept
+            m[e] = it.m_type == LRB_F32 ? m[e] : it.m_type == LRB_BF16 ? (float)(__bf16)m[e] : (float)(mu_h)m[e];
+        }
+        u[e] = nesterov ? (1.0f - beta) * u[e] + beta * m[e] : m[e];
+    }
 }
 
 // Momentum, and the sum of the squares of u over a 64 x 64 tile, in double (the squares of large float32 leave its range).
@@ -137,15 +151,14 @@ __global__ __launch_bounds__(256) void mu_momentum_kernel(mu_args a)
     const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
     const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
     double s = 0.0;
-#pragma unroll 4
-    for (int e = 0; e < 16; ++e) {
-        const int q = e * 256 + threadIdx.x, fast = q & 63, slow = q >> 6;
-        const int i = i0 + (along_j ? slow : fast), j = j0 + (along_j ? fast : slow);
-        if (i < it.n && j < it.l) {
-            const double u = mu_u<true>(a, it, mat, i, j);
-            s += u * u;
-        }
-    }
+    // entry e of a thread: 64 of a line by the lanes of a wave, four lines further for each e
+    auto fast = [&](int) { return (int)(threadIdx.x & 63); };
+    auto slow = [&](int e) { return e * 4 + (int)(threadIdx.x >> 6); };
+    float u[16];
+    if (along_j) mu_u<true>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + slow(e); }, [&](int e) { return j0 + fast(e); }, u);
+    else mu_u<true>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + fast(e); }, [&](int e) { return j0 + slow(e); }, u);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s += (double)u[e] * u[e];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -164,9 +177,51 @@ __host__ __device__ double mu_largest_odd(double a, double b, double c, double r
     return best;
 }
 
-__device__ double mu_scale(double r) // the power of two that takes entries up to r to at most MU_TOP
+__host__ __device__ double mu_scale(double r) // the power of two that takes entries up to r to at most MU_TOP
 {
-    return r > 0.0 && r < 1e300 ? exp2(floor(log2(MU_TOP / r))) : 1.0;
+    if (!(r > 0.0 && r < 1e300)) return 1.0;
+    int e;
+    frexp(MU_TOP / r, &e); // MU_TOP / r = f 2^e, 1/2 <= f < 1
+    return ldexp(1.0, e - 1);
+}
+
+// The scale of X at the start, for singular values up to r, and the five factors of every step.
+__host__ __device__ inline double mu_chain(double a, double b, double c, int steps, double r, float *t)
+{
+    const double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
+    r *= slack;
+    const double s0 = mu_scale(r);
+    double sx = s0;
+    for (int q = 0; q < steps; ++q, t += MU_COEF) {
+        const double ra = r * r * slack, sa = mu_scale(ra);
+        double rb = fabs(b * ra + c * ra * ra);
+        if (c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < ra) rb = fmax(rb, b * b / fabs(4.0 * c));
+        rb *= slack;
+        const double sb = mu_scale(rb);
+        r = mu_largest_odd(a, b, c, r) * slack;
+        const double sn = q + 1 < steps ? mu_scale(r) : 1.0;
+        t[0] = (float)(sa / (sx * sx));
+        t[1] = (float)(b * (sb / sa));
+        t[2] = (float)(c * (sb / sa) / sa);
+        t[3] = (float)(a * (sn / sx));
+        t[4] = (float)(sn / sb / sx);
+        sx = sn;
+    }
+    return s0;
+}
+
+// From the sum of the squares of u: what u is multiplied by to become X, and the bound r on X's singular values.  At r = 1 the
+// ready table holds.  An infinity or a NaN anywhere makes the whole matrix NaN.
+struct mu_norm {
+    double x0, r;
+};
+__device__ __forceinline__ mu_norm mu_start(double squares, double eps)
+{
+    const double norm = sqrt(squares), over = fmax(norm, eps);
+    mu_norm n;
+    n.r = !(norm < over) && norm > 0.0 ? 1.0 : fmax(norm / over, 1e-60);
+    n.x0 = !(norm < 1e300) ? (double)NAN : over > 0.0 ? 1.0 / over : 0.0;
+    return n;
 }
 
 // The norm of every matrix, and with it the scales of its factors in every step.
@@ -184,29 +239,10 @@ __global__ __launch_bounds__(256) void mu_table_kernel(mu_args a)
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     lrb_barrier();
-    if (threadIdx.x) return;
-    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
-    const double over = fmax(norm, (double)a.eps);
-    const double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
-    double r = fmax(norm / over, 1e-60) * slack, sx = mu_scale(r);
-    // an infinity or a NaN anywhere makes the whole matrix NaN
-    a.x0[blockIdx.x] = norm < 1e300 ? (over > 0.0 ? sx / over : 0.0) : (double)NAN;
+    const mu_norm n = mu_start(red[0] + red[1] + red[2] + red[3], a.eps);
     float *t = a.table + (size_t)blockIdx.x * a.steps * MU_COEF;
-    for (int q = 0; q < a.steps; ++q, t += MU_COEF) {
-        const double ra = r * r * slack, sa = mu_scale(ra);
-        double rb = fabs(a.b * ra + (double)a.c * ra * ra);
-        if (a.c != 0.0f && -a.b / (2.0 * a.c) > 0.0 && -a.b / (2.0 * a.c) < ra) rb = fmax(rb, (double)a.b * a.b / fabs(4.0 * a.c));
-        rb *= slack;
-        const double sb = mu_scale(rb);
-        r = mu_largest_odd(a.a, a.b, a.c, r) * slack;
-        const double sn = q + 1 < a.steps ? mu_scale(r) : 1.0;
-        t[0] = (float)(sa / (sx * sx));
-        t[1] = (float)(a.b * (sb / sa));
-        t[2] = (float)(a.c * (sb / sa) / sa);
-        t[3] = (float)(a.a * (sn / sx));
-        t[4] = (float)(sn / sb / sx);
-        sx = sn;
-    }
+    if (n.r == 1.0 && (int)threadIdx.x < a.steps * MU_COEF) t[threadIdx.x] = a.std[threadIdx.x];
+    if (threadIdx.x == 0) a.x0[blockIdx.x] = n.x0 * (n.r == 1.0 ? a.sx : mu_chain(a.a, a.b, a.c, a.steps, n.r, t));
 }
 
 __device__ __forceinline__ void mu_split(float v, mu_h &hi, mu_h &lo)
@@ -225,11 +261,15 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
     const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
     const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
     const double scale = a.x0[it.first + mat];
-#pragma unroll 4
+    auto fast = [&](int) { return (int)(threadIdx.x & 63); };
+    auto slow = [&](int e) { return e * 4 + (int)(threadIdx.x >> 6); };
+    float u[16];
+    if (along_j) mu_u<false>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + slow(e); }, [&](int e) { return j0 + fast(e); }, u);
+    else mu_u<false>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + fast(e); }, [&](int e) { return j0 + slow(e); }, u);
+#pragma unroll
     for (int e = 0; e < 16; ++e) {
-        const int q = e * 256 + threadIdx.x, fast = q & 63, slow = q >> 6;
-        const int i = along_j ? slow : fast, j = along_j ? fast : slow;
-        tile[i][j] = i0 + i < it.n && j0 + j < it.l ? (float)(scale * mu_u<false>(a, it, mat, i0 + i, j0 + j)) : 0.0f;
+        const bool in = along_j ? i0 + slow(e) < it.n && j0 + fast(e) < it.l : i0 + fast(e) < it.n && j0 + slow(e) < it.l;
+        tile[along_j ? slow(e) : fast(e)][along_j ? fast(e) : slow(e)] = in ? (float)(scale * u[e]) : 0.0f; // (the scale may be NaN)
     }
     lrb_barrier();
     const mu_mat w = mu_planes(a, it, mat);
@@ -590,6 +630,237 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
     mu_strip<MODE, NI>(a, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
 }
 
+// A matrix that fits one workgroup's LDS (128 x 176, 64 x 448, 32 x 1,136 and less) goes through all its steps there, in one
+// launch: X as rows of hi then lo, and A, then B, as rows of hi then lo; rows are 16 bytes longer than their entries, so that
+// 16 of them start in different banks.  Each wave keeps its 32 x 32 tiles of X, and of A on and above the diagonal, in float32
+// in registers from step to step.  X^T for B X is read from X by the transposing LDS read: of 16 lanes that address four
+// rows of 16 entries it gives each lane a column's four.
+// Bound: the matrix cores of one CU and the barriers (five a step).
+#define MU_SMALL_WAVES 16
+#define MU_SMALL_LDS (158 * 1024) // of 160 KB; the static arrays take the rest
+#define MU_SMALL_TILES 3          // of X for a wave at most
+
+__host__ __device__ inline int mu_small_n(int n) { return (n + 31) / 32 * 32; }
+__host__ __device__ inline int mu_small_l(int l) { return (l + 15) / 16 * 16; }
+static inline int mu_small_bytes(int n, int l) // 0: too large
+{
+    const long long np = mu_small_n(n), lp = mu_small_l(l), bytes = np * (4 * lp + 16) + np * (4 * np + 16);
+    const long long tiles = np / 32 * ((lp + 31) / 32);
+    return np <= 128 && bytes <= MU_SMALL_LDS && tiles <= MU_SMALL_TILES * MU_SMALL_WAVES ? (int)bytes : 0;
+}
+
+__device__ __forceinline__ mu_h4 mu_read_column(const char *p)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(mu_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p));
+}
+
+// hi and lo of four neighbouring entries
+__device__ __forceinline__ void mu_put4(char *hi_at, char *lo_at, float v0, float v1, float v2, float v3, mu_h4 &hi, mu_h4 &lo)
+{
+    mu_h h0, h1, h2, h3, l0, l1, l2, l3;
+    mu_split(v0, h0, l0), mu_split(v1, h1, l1), mu_split(v2, h2, l2), mu_split(v3, h3, l3);
+    hi = mu_h4{h0, h1, h2, h3}, lo = mu_h4{l0, l1, l2, l3};
+    *(mu_h4 *)hi_at = hi;
+    *(mu_h4 *)lo_at = lo;
+}
+
+// tile (ti, tj) of a symmetric matrix of np rows, and its mirror image
+__device__ __forceinline__ void mu_put_symmetric(char *A, int np, int ti, int tj, int lane, const mu_f16 &v)
+{
+    const int pa = 4 * np + 16, i = ti * 32 + (lane & 31), j = tj * 32 + 4 * (lane >> 5);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        mu_h4 hi, lo;
+        char *const at = A + i * pa + 2 * (j + 8 * q);
+        mu_put4(at, at + 2 * np, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], hi, lo);
+        if (ti == tj) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            char *const to = A + (j + 8 * q + e) * pa + 2 * i;
+            *(mu_h *)to = hi[e];
+            *(mu_h *)(to + 2 * np) = lo[e];
+        }
+    }
+}
+
+// the product of 32 rows at p and 32 rows at q, of len entries each (lo behind hi)
+__device__ __forceinline__ void mu_small_rows(const char *p, const char *q, int len, mu_f16 &acc)
+{
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll 2
+    for (int k0 = 0; k0 < len; k0 += 16, p += 32, q += 32) {
+        const mu_h8 ph = *(const mu_h8 *)p, pl = *(const mu_h8 *)(p + 2 * len), qh = *(const mu_h8 *)q, ql = *(const mu_h8 *)(q + 2 * len);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
+    }
+}
+
+__global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args by_value)
+{
+    // The arguments where they lie (the first one starts the kernel's argument segment): with this many uses of `by_value` the
+    // compiler copies all 3.5 KB of it to every thread's scratch.
+    const mu_args &a = *(const mu_args *)__builtin_amdgcn_kernarg_segment_ptr();
+    extern __shared__ __attribute__((aligned(16))) char mu_lds[];
+    __shared__ double red[MU_SMALL_WAVES];
+    __shared__ float own[MU_STEPS * MU_COEF];
+    int k = 0;
+    while (k + 1 < a.n_items && (int)blockIdx.x >= a.it[k + 1].first) ++k;
+    const mu_item &it = a.it[k];
+    const int mat = blockIdx.x - it.first, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = lane & 31, half = lane >> 5; // of a fragment: its row, and which 8 of 16 k
+    const int np = mu_small_n(it.n), lp = mu_small_l(it.l), nt = np / 32, tiles = nt * ((lp + 31) / 32);
+    const int px = 4 * lp + 16, pa = 4 * np + 16;
+    char *const X = mu_lds, *const A = mu_lds + np * px;
+
+    // A wave's tiles of X, four neighbouring columns in every four registers.  They are read (and at the end written) in pieces of
+    // four along the side on which g (p) is contiguous, and change hands through LDS, where X will be.
+    double s = 0.0;
+    const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
+#pragma unroll 1
+    for (int tile = wave; tile < tiles; tile += MU_SMALL_WAVES) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int line = 8 * q + lane / 8, at = lane % 8 * 4;
+            const int i = tile % nt * 32 + (along_j ? line : at), j = tile / nt * 32 + (along_j ? at : line);
+            float u[4];
+            if (along_j) mu_u<true>(a.beta, a.nesterov, it, mat, [&](int) { return i; }, [&](int e) { return j + e; }, u);
+            else mu_u<true>(a.beta, a.nesterov, it, mat, [&](int e) { return i + e; }, [&](int) { return j; }, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += (double)u[e] * u[e];
+            if (j >= lp) continue; // (a piece lies within lp or outside)
+            if (along_j) {
+                *(float4 *)(X + i * px + 4 * j) = make_float4(u[0], u[1], u[2], u[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) *(float *)(X + (i + e) * px + 4 * j) = u[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) red[wave] = s;
+    lrb_barrier();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < MU_SMALL_WAVES; ++w) s += red[w];
+    const mu_norm n = mu_start(s, a.eps);
+    double x0 = n.x0;
+    if (n.r == 1.0) { // (all threads have the same s)
+        if ((int)threadIdx.x < a.steps * MU_COEF) own[threadIdx.x] = a.std[threadIdx.x];
+        x0 *= a.sx;
+    } else { // a norm below eps
+        lrb_barrier(); // red has been read
+        if (threadIdx.x == 0) red[0] = mu_chain(a.a, a.b, a.c, a.steps, n.r, own);
+        lrb_barrier();
+        x0 *= red[0];
+    }
+    const float *coef = own;
+    float x[MU_SMALL_TILES][16];
+#pragma unroll
+    for (int t = 0; t < MU_SMALL_TILES; ++t) {
+        const int tile = wave + t * MU_SMALL_WAVES;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = tile % nt * 32 + row, j = tile / nt * 32 + 4 * half + 8 * q;
+            const float4 v = tile < tiles && j < lp ? *(const float4 *)(X + i * px + 4 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x[t][4 * q] = (float)(x0 * v.x), x[t][4 * q + 1] = (float)(x0 * v.y);
+            x[t][4 * q + 2] = (float)(x0 * v.z), x[t][4 * q + 3] = (float)(x0 * v.w);
+        }
+    }
+
+    lrb_barrier(); // all have read: what follows writes hi and lo there
+    // the wave's tile of the symmetric products, on or above the diagonal
+    int ti = 0, tj = wave;
+    while (ti < nt && tj >= nt - ti) tj -= nt - ti++;
+    tj += ti;
+    const bool sym = ti < nt;
+    for (int step = 0; step < a.steps; ++step, coef += MU_COEF) {
+        // the addresses below are made anew in every step: kept over the steps, all of them together spill
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int row = lane & 31, half = lane >> 5;
+#pragma unroll
+        for (int t = 0; t < MU_SMALL_TILES; ++t) {
+            const int tile = wave + t * MU_SMALL_WAVES, i = tile % nt * 32 + row, j = tile / nt * 32 + 4 * half;
+            if (tile >= tiles) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (j + 8 * q >= lp) continue;
+                mu_h4 hi, lo;
+                char *const at = X + i * px + 2 * (j + 8 * q);
+                mu_put4(at, at + 2 * lp, x[t][4 * q], x[t][4 * q + 1], x[t][4 * q + 2], x[t][4 * q + 3], hi, lo);
+            }
+        }
+        lrb_barrier();
+        mu_f16 full, acc;
+        if (sym) {
+            mu_small_rows(X + (ti * 32 + row) * px + 16 * half, X + (tj * 32 + row) * px + 16 * half, lp, full);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) full[e] *= coef[0];
+            mu_put_symmetric(A, np, ti, tj, lane, full);
+        }
+        lrb_barrier();
+        if (sym) {
+            mu_small_rows(A + (ti * 32 + row) * pa + 16 * half, A + (tj * 32 + row) * pa + 16 * half, np, acc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = coef[1] * full[e] + coef[2] * acc[e];
+        }
+        lrb_barrier();
+        if (sym) mu_put_symmetric(A, np, ti, tj, lane, acc);
+        lrb_barrier();
+#pragma unroll
+        for (int t = 0; t < MU_SMALL_TILES; ++t) {
+            const int tile = wave + t * MU_SMALL_WAVES;
+            if (tile >= tiles) continue;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+            const char *p = A + (tile % nt * 32 + row) * pa + 16 * half;
+            // rows k of X, 16 columns of the tile for each 16 lanes; columns past the end give what is not kept
+            const char *q = X + (8 * half + (lane & 15) / 4) * px + 2 * (tile / nt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+#pragma unroll 2
+            for (int k0 = 0; k0 < np; k0 += 16, p += 32, q += 16 * px) {
+                const mu_h8 ph = *(const mu_h8 *)p, pl = *(const mu_h8 *)(p + 2 * np);
+                const mu_h4 h0 = mu_read_column(q), h1 = mu_read_column(q + 4 * px), l0 = mu_read_column(q + 2 * lp),
+                            l1 = mu_read_column(q + 4 * px + 2 * lp);
+                const mu_h8 qh = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7), ql = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[t][e] = coef[3] * x[t][e] + coef[4] * acc[e];
+        }
+        lrb_barrier();
+    }
+#pragma unroll
+    for (int t = 0; t < MU_SMALL_TILES; ++t) {
+        const int tile = wave + t * MU_SMALL_WAVES;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = tile % nt * 32 + row, j = tile / nt * 32 + 4 * half + 8 * q;
+            if (tile < tiles && j < lp) *(float4 *)(X + i * px + 4 * j) = make_float4(x[t][4 * q], x[t][4 * q + 1], x[t][4 * q + 2], x[t][4 * q + 3]);
+        }
+    }
+    mu_wave_sync();
+    const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1;
+#pragma unroll 1
+    for (int tile = wave; tile < tiles; tile += MU_SMALL_WAVES) {
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+            const int line = 8 * q + lane / 8, at = lane % 8 * 4;
+            const int i = tile % nt * 32 + (by_rows ? line : at), j = tile / nt * 32 + (by_rows ? at : line);
+            if (i >= it.n || j >= it.l) continue;
+            const char *v = X + i * px + 4 * j;
+            const int step = by_rows ? 4 : px;
+            const float4 f = make_float4(*(const float *)v, *(const float *)(v + step), *(const float *)(v + 2 * step), *(const float *)(v + 3 * step));
+            mu_update4(it, mat * it.ps[0] + i * it.ps[1] + j * it.ps[2], by_rows ? it.ps[2] : it.ps[1], min(4, by_rows ? it.l - j : it.n - i), f);
+        }
+    }
+}
+
 // How a product's launch is laid out.
 struct mu_plan {
     int T;             // side of a tile
@@ -661,11 +932,13 @@ template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
 #define MU_MATS_MOST 4096
 struct mu_group {
     mu_args a;
+    int lds; // of a group whose matrices fit a workgroup's LDS: the most that one takes; else 0
     int mats;
     long long tiles;
     uint64_t planes;
     uint64_t bytes() const
     {
+        if (lds) return 0;
         uint64_t parts = 0;
         for (int mode = MU_GRAM; mode <= MU_LAST; ++mode) {
             const uint64_t b = mu_lay_out(a, mode).part_bytes();
@@ -676,49 +949,63 @@ struct mu_group {
     }
 };
 
-// Calls `go(group)` for each group of the list in turn; stops at its first non-zero answer.
+// Calls `go(group)` for each group of the list in turn, those of small matrices first; stops at its first non-zero answer.
 template <typename F> static int mu_each_group(const lrb_muon_item *items, int n_items, F go)
 {
-    mu_group gr = {};
-    for (int k = 0; k < n_items; ++k) {
-        const lrb_muon_item &s = items[k];
-        if (s.count <= 0 || s.rows <= 0 || s.cols <= 0) continue;
-        for (int64_t done = 0; done < s.count;) {
-            mu_item it = {};
+    for (int small = 1; small >= 0; --small) {
+        mu_group gr = {};
+        for (int k = 0; k < n_items; ++k) {
+            const lrb_muon_item &s = items[k];
+            if (s.count <= 0 || s.rows <= 0 || s.cols <= 0) continue;
             const bool turned = s.rows > s.cols;
+            mu_item it = {};
             it.n = (int)(turned ? s.cols : s.rows), it.l = (int)(turned ? s.rows : s.cols);
+            const int lds = mu_small_bytes(it.n, it.l);
+            if ((lds != 0) != (small != 0)) continue;
             it.np = (it.n + 63) / 64 * 64, it.lp = (it.l + 63) / 64 * 64;
             it.step = mu_bytes(it);
-            const long long per = (long long)(it.np / 64) * (it.lp / 64);
-            uint64_t room = gr.planes < MU_WS_MOST ? (MU_WS_MOST - gr.planes) / it.step : 0;
-            if (room == 0 && gr.a.n_items == 0) room = 1;
-            if (room > (uint64_t)(MU_MATS_MOST - gr.mats)) room = MU_MATS_MOST - gr.mats;
-            if (per * (long long)room > (1 << 28) - gr.tiles && room > 1) room = ((1 << 28) - gr.tiles) / per;
-            if (room == 0 || gr.a.n_items == MU_ITEMS) {
-                if (int rc = go(gr)) return rc;
-                gr = {};
-                continue;
-            }
-            it.count = (int)(s.count - done < (int64_t)room ? s.count - done : (int64_t)room);
-            const int size_p = s.p_type == LRB_F32 ? 4 : 2, size_g = s.g_type == LRB_F32 ? 4 : 2, size_m = s.m_type == LRB_F32 ? 4 : 2;
-            it.p = (char *)s.p + done * s.p_stride[0] * size_p;
-            it.g = (const char *)s.g + done * s.g_stride[0] * size_g;
-            it.m = s.m ? (char *)s.m + done * s.m_stride[0] * size_m : nullptr;
             for (int d = 0; d < 3; ++d) {
                 const int from = d && turned ? 3 - d : d;
                 it.ps[d] = s.p_stride[from], it.gs[d] = s.g_stride[from], it.ms[d] = s.m_stride[from];
             }
             it.p_type = s.p_type, it.g_type = s.g_type, it.m_type = s.m_type;
             it.alpha = s.alpha, it.decay = s.decay;
-            it.off = gr.planes, it.first = gr.mats;
-            gr.a.start[gr.a.n_items] = (int)gr.tiles;
-            gr.a.it[gr.a.n_items++] = it;
-            gr.planes += it.step * it.count, gr.mats += it.count, gr.tiles += per * it.count;
-            gr.a.start[gr.a.n_items] = (int)gr.tiles;
-            done += it.count;
+            const long long per = (long long)(it.np / 64) * (it.lp / 64);
+            const int size_p = s.p_type == LRB_F32 ? 4 : 2, size_g = s.g_type == LRB_F32 ? 4 : 2, size_m = s.m_type == LRB_F32 ? 4 : 2;
+            for (int64_t done = 0; done < s.count;) {
+                int64_t room = (1 << 20) - gr.mats;
+                if (!small) {
+                    room = gr.planes < MU_WS_MOST ? (int64_t)((MU_WS_MOST - gr.planes) / it.step) : 0;
+                    if (room == 0 && gr.a.n_items == 0) room = 1;
+                    if (room > MU_MATS_MOST - gr.mats) room = MU_MATS_MOST - gr.mats;
+                    if (per * room > (1 << 28) - gr.tiles && room > 1) room = ((1 << 28) - gr.tiles) / per;
+                }
+                if (room == 0 || gr.a.n_items == MU_ITEMS) {
+                    if (int rc = go(gr)) return rc;
+                    gr = {};
+                    continue;
+                }
+                it.count = (int)(s.count - done < room ? s.count - done : room);
+                it.p = (char *)s.p + done * s.p_stride[0] * size_p;
+                it.g = (const char *)s.g + done * s.g_stride[0] * size_g;
+                it.m = s.m ? (char *)s.m + done * s.m_stride[0] * size_m : nullptr;
+                it.off = gr.planes, it.first = gr.mats;
+                gr.a.start[gr.a.n_items] = (int)gr.tiles;
+                gr.a.it[gr.a.n_items++] = it;
+                gr.mats += it.count;
+                if (small) {
+                    gr.lds = gr.lds > lds ? gr.lds : lds;
+                } else {
+                    gr.planes += it.step * it.count, gr.tiles += per * it.count;
+                }
+                gr.a.start[gr.a.n_items] = (int)gr.tiles;
+                done += it.count;
+            }
         }
+        if (gr.a.n_items)
+            if (int rc = go(gr)) return rc;
     }
-    return gr.a.n_items ? go(gr) : LRB_OK;
+    return LRB_OK;
 }
 
 static bool mu_items_fit(const lrb_muon_item *items, int n)
@@ -764,20 +1051,35 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
     ARG_TRY(lrb_muon_bound(steps, a, b, c) <= LRB_MUON_DIVERGED);
     ARG_TRY(mu_items_fit(items, n_items));
     const uint64_t need = lrb_muon_ws_bytes(items, n_items);
-    if (need == 0) return LRB_OK;
-    ARG_TRY(d_ws != nullptr && ws_bytes >= need && ((uintptr_t)d_ws & 255) == 0);
+    ARG_TRY(need == 0 || (d_ws != nullptr && ws_bytes >= need && ((uintptr_t)d_ws & 255) == 0));
+    bool any = false;
+    for (int k = 0; k < n_items; ++k) any |= items[k].count > 0 && items[k].rows > 0 && items[k].cols > 0;
+    if (!any) return LRB_OK;
     lrb_on_device on(device);
     HIP_TRY(on.err);
     hipStream_t st = (hipStream_t)stream;
+    float std[MU_STEPS * MU_COEF] = {};
+    const double sx = mu_chain(a, b, c, steps, 1.0, std);
     return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
         mu_args &g = gr.a;
+        g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
+        g.sx = sx;
+        memcpy(g.std, std, sizeof(std));
+        if (gr.lds) {
+            static lrb_per_device_once raised;
+            if (raised.need(device)) {
+                HIP_TRY(hipFuncSetAttribute((const void *)mu_small_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MU_SMALL_LDS));
+            }
+            hipLaunchKernelGGL(mu_small_kernel, dim3(gr.mats), dim3(64 * MU_SMALL_WAVES), gr.lds, st, g);
+            HIP_TRY(hipGetLastError());
+            return LRB_OK;
+        }
         g.ws = (char *)d_ws;
         char *at = g.ws + gr.planes;
         g.x0 = (double *)at, at += ((uint64_t)gr.mats * 8 + 255) / 256 * 256;
         g.part = (double *)at, at += ((uint64_t)gr.tiles * 8 + 255) / 256 * 256;
         g.table = (float *)at, at += ((uint64_t)gr.mats * MU_STEPS * MU_COEF * 4 + 255) / 256 * 256;
         g.parts = (float *)at;
-        g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
         hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
         hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
         hipLaunchKernelGGL(mu_split_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);

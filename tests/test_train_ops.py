@@ -200,8 +200,8 @@ def test_c_entry_points_refuse_before_they_touch_a_device():
     assert L.lrb_layer_norm_bwd_dev(0, None, 0, 0, 1, 4, p, 4, p, 4, None, p, p, 1.0, None, 1.0, p, p, None, p, 0) == 1  # no room
     assert L.lrb_layer_norm_bwd_dev(0, None, 0, 0, 1, 4, None, 4, p, 4, None, p, p, 1.0, None, 1.0, p, None, None, None, 0) == 1
 
-    def item(rows=4, cols=4, count=1, p_ptr=p, p_type=0, g_type=0, m=0, m_type=0):
-        return C.create_string_buffer(train_ops._ITEM.pack(p_ptr, p, m, 16, 4, 1, 16, 4, 1, 0, 0, 0, count, rows, cols, p_type, g_type, m_type, 1.0, 0.0, 0))
+    def item(rows=300, cols=300, count=1, p_ptr=p, p_type=0, g_type=0, m=0, m_type=0):
+        return C.create_string_buffer(train_ops._ITEM.pack(p_ptr, p, m, 90000, 300, 1, 90000, 300, 1, 0, 0, 0, count, rows, cols, p_type, g_type, m_type, 1.0, 0.0, 0))
 
     step = lambda it, n=1, steps=5, eps=0.0, ws=p, ws_bytes=64: L.lrb_muon_dev(0, None, it, n, 0.9, 1, steps, 1.5, -0.5, 0.0, eps, ws, ws_bytes)
     assert step(None, 0) == 0 and step(item(rows=0)) == 0 and step(item(count=0)) == 0
@@ -210,7 +210,7 @@ def test_c_entry_points_refuse_before_they_touch_a_device():
                      (item(), dict(steps=33)), (item(), dict(eps=-1.0)), (item(), dict(n=-1)), (None, {}), (item(), dict(ws=None)),
                      (item(), dict(ws_bytes=64))):
         assert step(it, **more) == 1, more
-    assert L.lrb_muon_ws_bytes(item(), 1) >= 16 * 64 * 64
+    assert L.lrb_muon_ws_bytes(item(), 1) >= 16 * 300 * 300 and L.lrb_muon_ws_bytes(item(rows=4, cols=4), 1) == 0  # (in LDS)
     assert L.lrb_muon_dev(0, None, item(), 1, 0.9, 1, 2, 6.0, -9.0, 4.0, 0.0, p, 1 << 30) == 1       # diverges
     assert L.lrb_muon_dev(0, None, item(), 1, 0.9, 1, 2, float("nan"), 1.0, 1.0, 0.0, p, 1 << 30) == 1
 
