@@ -97,17 +97,6 @@ __device__ __forceinline__ mu_mat mu_planes(const mu_args &a, const mu_item &it,
 // hi of entry (row, k) of a factor with rows of `len`; lo lies 32 further
 __device__ __forceinline__ size_t mu_at(int row, int k, int len) { return (size_t)row * 2 * len + (k >> 5) * 64 + (k & 31); }
 
-__device__ __forceinline__ float mu_load(const void *p, long long at, int type)
-{
-    return type == LRB_F32 ? ((const float *)p)[at] : type == LRB_BF16 ? (float)((const __bf16 *)p)[at] : (float)((const mu_h *)p)[at];
-}
-__device__ __forceinline__ void mu_store(void *p, long long at, int type, float v)
-{
-    if (type == LRB_F32) ((float *)p)[at] = v;
-    else if (type == LRB_BF16) ((__bf16 *)p)[at] = (__bf16)v;
-    else ((mu_h *)p)[at] = (mu_h)v;
-}
-
 // Which item a tile of the launch belongs to.
 __device__ __forceinline__ int mu_find(const mu_args &a, int tile)
 {
@@ -116,30 +105,98 @@ __device__ __forceinline__ int mu_find(const mu_args &a, int tile)
     return k;
 }
 
-// u at N places (row i(e), column j(e), where they lie inside), 0 elsewhere.  All loads are issued before the first result is
-// used.  UPDATE also writes the momentum back (each entry by one thread).
-template <bool UPDATE, int N, typename I, typename J>
-__device__ __forceinline__ void mu_u(float beta, int nesterov, const mu_item &it, int mat, I i, J j, float (&u)[N])
+// R pieces of four entries, `step` apart, of which `count(r)` lie inside (the others are 0): entry e of piece r is at
+// at + r * piece + e * step.  The type is asked for once, so all pieces are on their way together.
+template <typename T, int R, typename C>
+__device__ __forceinline__ void mu_read(const T *p, long long at, long long piece, long long step, C count, float (&v)[4 * R])
 {
-    float m[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const bool in = i(e) < it.n && j(e) < it.l;
-        u[e] = in ? mu_load(it.g, mat * it.gs[0] + i(e) * it.gs[1] + j(e) * it.gs[2], it.g_type) : 0.0f;
-        m[e] = in && it.m ? mu_load(it.m, mat * it.ms[0] + i(e) * it.ms[1] + j(e) * it.ms[2], it.m_type) : 0.0f;
-    }
-    if (!it.m) return;
+    for (int r = 0; r < R; ++r) {
+        const T *const q = p + at + r * piece;
+        const int n = count(r);
+        if (step == 1 && n == 4) {
+            T t[4];
+            __builtin_memcpy(t, q, sizeof(t));
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        if (UPDATE) {
-            m[e] = beta * m[e] + (1.0f - beta) * u[e];
-            if (i(e) < it.n && j(e) < it.l) mu_store(it.m, mat * it.ms[0] + i(e) * it.ms[1] + j(e) * it.ms[2], it.m_type, m[e]);
-            // u is made of what is kept
-            m[e] = it.m_type == LRB_F32 ? m[e] : it.m_type == LRB_BF16 ? (float)(__bf16)m[e] : (float)(mu_h)m[e];
+            for (int e = 0; e < 4; ++e) v[4 * r + e] = (float)t[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * r + e] = e < n ? (float)q[e * step] : 0.0f;
         }
-        u[e] = nesterov ? (1.0f - beta) * u[e] + beta * m[e] : m[e];
     }
 }
+template <int R, typename C>
+__device__ __forceinline__ void mu_read(const void *p, int type, long long at, long long piece, long long step, C count, float (&v)[4 * R])
+{
+    if (type == LRB_F32) mu_read<float, R>((const float *)p, at, piece, step, count, v);
+    else if (type == LRB_BF16) mu_read<__bf16, R>((const __bf16 *)p, at, piece, step, count, v);
+    else mu_read<mu_h, R>((const mu_h *)p, at, piece, step, count, v);
+}
+template <typename T, int R, typename C>
+__device__ __forceinline__ void mu_write(T *p, long long at, long long piece, long long step, C count, float (&v)[4 * R])
+{
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        T *const q = p + at + r * piece;
+        const int n = count(r);
+        T t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            t[e] = (T)v[4 * r + e];
+            v[4 * r + e] = (float)t[e]; // what is kept
+        }
+        if (step == 1 && n == 4) {
+            __builtin_memcpy(q, t, sizeof(t));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < n) q[e * step] = t[e];
+        }
+    }
+}
+
+// u in R pieces of four along the side on which g is contiguous: piece r lies in line `line(r)` of the other side, from `at` on.
+// UPDATE also writes the momentum back (each entry by one thread); u is made of what is kept.
+template <bool UPDATE, int R, typename L>
+__device__ __forceinline__ void mu_u(float beta, int nesterov, const mu_item &it, int mat, bool along_j, L line, int at, float (&u)[4 * R])
+{
+    const int lines = along_j ? it.n : it.l, len = along_j ? it.l : it.n;
+    const long long g_fast = along_j ? it.gs[2] : it.gs[1], g_slow = along_j ? it.gs[1] : it.gs[2];
+    const long long m_fast = along_j ? it.ms[2] : it.ms[1], m_slow = along_j ? it.ms[1] : it.ms[2];
+    auto count = [=](int r) { return line(r) < lines ? max(0, min(4, len - at)) : 0; };
+    const long long gap = R > 1 ? line(1) - line(0) : 0; // lines are evenly spaced
+    mu_read<R>(it.g, it.g_type, mat * it.gs[0] + line(0) * g_slow + at * g_fast, gap * g_slow, g_fast, count, u);
+    if (!it.m) return;
+    float m[4 * R];
+    const long long m_at = mat * it.ms[0] + line(0) * m_slow + at * m_fast;
+    mu_read<R>(it.m, it.m_type, m_at, gap * m_slow, m_fast, count, m);
+    if (UPDATE) {
+#pragma unroll
+        for (int e = 0; e < 4 * R; ++e) m[e] = beta * m[e] + (1.0f - beta) * u[e];
+        if (it.m_type == LRB_F32) mu_write<float, R>((float *)it.m, m_at, gap * m_slow, m_fast, count, m);
+        else if (it.m_type == LRB_BF16) mu_write<__bf16, R>((__bf16 *)it.m, m_at, gap * m_slow, m_fast, count, m);
+        else mu_write<mu_h, R>((mu_h *)it.m, m_at, gap * m_slow, m_fast, count, m);
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * R; ++e) u[e] = nesterov ? (1.0f - beta) * u[e] + beta * m[e] : m[e];
+}
+
+// v times a double, rounded once or nearly so (to 2^-24 (1 + 2^-23)) without double arithmetic for each entry: the factor is
+// (hi + lo) 2^e with 1/2 <= hi < 1.
+struct mu_factor {
+    float hi, lo;
+    int e;
+    __device__ __forceinline__ explicit mu_factor(double f)
+    {
+        const double m = frexp(f, &e); // a NaN or a zero stays
+        hi = (float)m, lo = (float)(m - hi);
+    }
+    __device__ __forceinline__ float operator*(float v) const
+    {
+        const float w = ldexpf(v, e);
+        return fmaf(w, hi, w * lo);
+    }
+};
 
 // Momentum, and the sum of the squares of u over a 64 x 64 tile, in double (the squares of large float32 leave its range).
 __global__ __launch_bounds__(256) void mu_momentum_kernel(mu_args a)
@@ -151,12 +208,10 @@ __global__ __launch_bounds__(256) void mu_momentum_kernel(mu_args a)
     const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
     const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
     double s = 0.0;
-    // entry e of a thread: 64 of a line by the lanes of a wave, four lines further for each e
-    auto fast = [&](int) { return (int)(threadIdx.x & 63); };
-    auto slow = [&](int e) { return e * 4 + (int)(threadIdx.x >> 6); };
+    // sixteen threads a line of 64, four lines of a thread 16 apart
     float u[16];
-    if (along_j) mu_u<true>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + slow(e); }, [&](int e) { return j0 + fast(e); }, u);
-    else mu_u<true>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + fast(e); }, [&](int e) { return j0 + slow(e); }, u);
+    const int line = (along_j ? i0 : j0) + (threadIdx.x >> 4), at = (along_j ? j0 : i0) + (threadIdx.x & 15) * 4;
+    mu_u<true, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, at, u);
 #pragma unroll
     for (int e = 0; e < 16; ++e) s += (double)u[e] * u[e];
 #pragma unroll
@@ -245,10 +300,33 @@ __global__ __launch_bounds__(256) void mu_table_kernel(mu_args a)
     if (threadIdx.x == 0) a.x0[blockIdx.x] = n.x0 * (n.r == 1.0 ? a.sx : mu_chain(a.a, a.b, a.c, a.steps, n.r, t));
 }
 
-__device__ __forceinline__ void mu_split(float v, mu_h &hi, mu_h &lo)
+// hi = fp16(v), lo = fp16(v - hi), in two instructions an entry: pairs are converted together, and the difference takes hi as
+// it is (v_fma_mix_f32; minus_one is hidden from the compiler, which would turn the product into conversions and subtractions).
+template <int N> __device__ __forceinline__ void mu_split(const float (&v)[N], mu_h (&hi)[N], mu_h (&lo)[N])
 {
-    hi = (mu_h)v;
-    lo = (mu_h)(v - (float)hi);
+    typedef mu_h h2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    float minus_one = -1.0f;
+    asm("" : "+s"(minus_one));
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+        const h2 h = __builtin_convertvector((f2){v[e], v[e + 1]}, h2);
+        const h2 l = __builtin_convertvector((f2){__builtin_fmaf((float)h[0], minus_one, v[e]), __builtin_fmaf((float)h[1], minus_one, v[e + 1])}, h2);
+        hi[e] = h[0], hi[e + 1] = h[1], lo[e] = l[0], lo[e + 1] = l[1];
+    }
+}
+__device__ __forceinline__ void mu_split4(float v0, float v1, float v2, float v3, mu_h4 &hi, mu_h4 &lo)
+{
+    const float v[4] = {v0, v1, v2, v3};
+    mu_h h[4], l[4];
+    mu_split<4>(v, h, l);
+    hi = mu_h4{h[0], h[1], h[2], h[3]}, lo = mu_h4{l[0], l[1], l[2], l[3]};
+}
+__device__ __forceinline__ void mu_split8(const float (&v)[8], mu_h8 &hi, mu_h8 &lo)
+{
+    mu_h h[8], l[8];
+    mu_split<8>(v, h, l);
+    hi = mu_h8{h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]}, lo = mu_h8{l[0], l[1], l[2], l[3], l[4], l[5], l[6], l[7]};
 }
 
 // u, scaled and split, as X and as its transpose: a 64 x 64 tile through LDS, so that all sides are read and written in rows.
@@ -260,17 +338,17 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
     const int tj = it.lp / 64, per = (it.np / 64) * tj, local = blockIdx.x - a.start[k], mat = local / per, r = local % per;
     const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
     const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
-    const double scale = a.x0[it.first + mat];
-    auto fast = [&](int) { return (int)(threadIdx.x & 63); };
-    auto slow = [&](int e) { return e * 4 + (int)(threadIdx.x >> 6); };
+    const mu_factor scale(a.x0[it.first + mat]);
     float u[16];
-    if (along_j) mu_u<false>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + slow(e); }, [&](int e) { return j0 + fast(e); }, u);
-    else mu_u<false>(a.beta, a.nesterov, it, mat, [&](int e) { return i0 + fast(e); }, [&](int e) { return j0 + slow(e); }, u);
+    const int first = threadIdx.x >> 4, x = (threadIdx.x & 15) * 4, line = (along_j ? i0 : j0) + first;
+    mu_u<false, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, (along_j ? j0 : i0) + x, u);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const bool in = along_j ? i0 + slow(e) < it.n && j0 + fast(e) < it.l : i0 + fast(e) < it.n && j0 + slow(e) < it.l;
-        tile[along_j ? slow(e) : fast(e)][along_j ? fast(e) : slow(e)] = in ? (float)(scale * u[e]) : 0.0f; // (the scale may be NaN)
-    }
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = along_j ? first + 16 * r : x + e, j = along_j ? x + e : first + 16 * r;
+            tile[i][j] = i0 + i < it.n && j0 + j < it.l ? scale * u[4 * r + e] : 0.0f; // (the scale may be NaN)
+        }
     lrb_barrier();
     const mu_mat w = mu_planes(a, it, mat);
 #pragma unroll
@@ -280,21 +358,14 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
         mu_h8 hi, lo;
         const size_t at = mu_at(i0 + row, j0 + c, it.lp), at_t = mu_at(j0 + row, i0 + c, it.np);
 #pragma unroll
-        for (int e8 = 0; e8 < 8; ++e8) {
-            mu_h h, l;
-            v[e8] = tile[row][c + e8];
-            mu_split(v[e8], h, l);
-            hi[e8] = h, lo[e8] = l;
-        }
+        for (int q = 0; q < 8; ++q) v[q] = tile[row][c + q];
+        mu_split8(v, hi, lo);
         __builtin_memcpy(w.x32 + (size_t)(i0 + row) * it.lp + j0 + c, v, 32);
         *(mu_h8 *)(w.x + at) = hi;
         *(mu_h8 *)(w.x + at + 32) = lo;
 #pragma unroll
-        for (int e8 = 0; e8 < 8; ++e8) {
-            mu_h h, l;
-            mu_split(tile[c + e8][row], h, l);
-            hi[e8] = h, lo[e8] = l;
-        }
+        for (int q = 0; q < 8; ++q) v[q] = tile[c + q][row];
+        mu_split8(v, hi, lo);
         *(mu_h8 *)(w.xt + at_t) = hi;
         *(mu_h8 *)(w.xt + at_t + 32) = lo;
     }
@@ -381,11 +452,11 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, in
         if (MODE == MU_LAST) {
             if (by_rows && i < it.n && j < it.l) mu_update4(it, mat * it.ps[0] + i * it.ps[1] + j * it.ps[2], it.ps[2], min(4, it.l - j), v);
         } else {
-            mu_h h0, h1, h2, h3, l0, l1, l2, l3;
-            mu_split(v.x, h0, l0), mu_split(v.y, h1, l1), mu_split(v.z, h2, l2), mu_split(v.w, h3, l3);
+            mu_h4 hi, lo;
+            mu_split4(v.x, v.y, v.z, v.w, hi, lo);
             if (MODE != MU_POLY) *old = v; // B is a factor only
-            *(mu_h4 *)(out + mu_at(i, j, ld)) = mu_h4{h0, h1, h2, h3};
-            *(mu_h4 *)(out + mu_at(i, j, ld) + 32) = mu_h4{l0, l1, l2, l3};
+            *(mu_h4 *)(out + mu_at(i, j, ld)) = hi;
+            *(mu_h4 *)(out + mu_at(i, j, ld) + 32) = lo;
         }
     }
     if (!back) return;
@@ -404,12 +475,7 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, in
             if (i + 4 < it.n) mu_update4(it, at + 4 * it.ps[1], it.ps[1], min(4, it.n - i - 4), make_float4(v[4], v[5], v[6], v[7]));
         } else {
             mu_h8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                mu_h h, l;
-                mu_split(v[e], h, l);
-                hi[e] = h, lo[e] = l;
-            }
+            mu_split8(v, hi, lo);
             *(mu_h8 *)(out_t + mu_at(j, i, it.np)) = hi;
             *(mu_h8 *)(out_t + mu_at(j, i, it.np) + 32) = lo;
         }
@@ -630,7 +696,7 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
     mu_strip<MODE, NI>(a, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
 }
 
-// A matrix that fits one workgroup's LDS (128 x 176, 64 x 448, 32 x 1,136 and less) goes through all its steps there, in one
+// A matrix that fits one workgroup's LDS (128 x 208, 96 x 320, 64 x 512, 32 x 1,024 and less) goes through all its steps there, in one
 // launch: X as rows of hi then lo, and A, then B, as rows of hi then lo; rows are 16 bytes longer than their entries, so that
 // 16 of them start in different banks.  Each wave keeps its 32 x 32 tiles of X, and of A on and above the diagonal, in float32
 // in registers from step to step.  X^T for B X is read from X by the transposing LDS read: of 16 lanes that address four
@@ -638,15 +704,22 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
 // Bound: the matrix cores of one CU and the barriers (five a step).
 #define MU_SMALL_WAVES 16
 #define MU_SMALL_LDS (158 * 1024) // of 160 KB; the static arrays take the rest
-#define MU_SMALL_TILES 3          // of X for a wave at most
+#define MU_SMALL_TILES 2          // of X for a wave at most
 
 __host__ __device__ inline int mu_small_n(int n) { return (n + 31) / 32 * 32; }
 __host__ __device__ inline int mu_small_l(int l) { return (l + 15) / 16 * 16; }
+// A symmetric matrix of nt x nt blocks of 32 x 32 is kept as its blocks on and above the diagonal, row by row; what lies below is
+// read from above it, by columns.  A block: rows of 32 hi, 32 lo and 16 bytes.
+#define MU_BLOCK_ROW 144
+#define MU_BLOCK (32 * MU_BLOCK_ROW)
+__host__ __device__ inline int mu_block(int ti, int tj, int nt) { return (ti * nt - ti * (ti - 1) / 2 + tj - ti) * MU_BLOCK; }
+// Bytes of a row of X.  A direct read takes 16 bytes each from 16 rows: of all 64 banks once if the pitch is an odd number of 16
+// bytes; a read by columns 64 each from four rows: twice, if that number is not 1 from a multiple of 16 (else four times).
+__host__ __device__ inline int mu_small_pitch(int lp) { return 4 * lp + (lp % 64 ? 16 : 48); }
 static inline int mu_small_bytes(int n, int l) // 0: too large
 {
-    const long long np = mu_small_n(n), lp = mu_small_l(l), bytes = np * (4 * lp + 16) + np * (4 * np + 16);
-    const long long tiles = np / 32 * ((lp + 31) / 32);
-    return np <= 128 && bytes <= MU_SMALL_LDS && tiles <= MU_SMALL_TILES * MU_SMALL_WAVES ? (int)bytes : 0;
+    const long long np = mu_small_n(n), lp = mu_small_l(l), bytes = np * mu_small_pitch((int)lp) + mu_block((int)np / 32, (int)np / 32, (int)np / 32);
+    return np <= 128 && bytes <= MU_SMALL_LDS && (lp + 31) / 32 <= MU_SMALL_TILES * (MU_SMALL_WAVES / (np / 32)) ? (int)bytes : 0;
 }
 
 __device__ __forceinline__ mu_h4 mu_read_column(const char *p)
@@ -656,46 +729,52 @@ __device__ __forceinline__ mu_h4 mu_read_column(const char *p)
 }
 
 // hi and lo of four neighbouring entries
-__device__ __forceinline__ void mu_put4(char *hi_at, char *lo_at, float v0, float v1, float v2, float v3, mu_h4 &hi, mu_h4 &lo)
+__device__ __forceinline__ void mu_put4(char *hi_at, char *lo_at, float v0, float v1, float v2, float v3)
 {
-    mu_h h0, h1, h2, h3, l0, l1, l2, l3;
-    mu_split(v0, h0, l0), mu_split(v1, h1, l1), mu_split(v2, h2, l2), mu_split(v3, h3, l3);
-    hi = mu_h4{h0, h1, h2, h3}, lo = mu_h4{l0, l1, l2, l3};
+    mu_h4 hi, lo;
+    mu_split4(v0, v1, v2, v3, hi, lo);
     *(mu_h4 *)hi_at = hi;
     *(mu_h4 *)lo_at = lo;
 }
 
-// tile (ti, tj) of a symmetric matrix of np rows, and its mirror image
-__device__ __forceinline__ void mu_put_symmetric(char *A, int np, int ti, int tj, int lane, const mu_f16 &v)
+__device__ __forceinline__ void mu_put_block(char *block, int lane, const mu_f16 &v)
 {
-    const int pa = 4 * np + 16, i = ti * 32 + (lane & 31), j = tj * 32 + 4 * (lane >> 5);
+    char *const at = block + (lane & 31) * MU_BLOCK_ROW + 8 * (lane >> 5);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        mu_h4 hi, lo;
-        char *const at = A + i * pa + 2 * (j + 8 * q);
-        mu_put4(at, at + 2 * np, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], hi, lo);
-        if (ti == tj) continue;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            char *const to = A + (j + 8 * q + e) * pa + 2 * i;
-            *(mu_h *)to = hi[e];
-            *(mu_h *)(to + 2 * np) = lo[e];
-        }
-    }
+    for (int q = 0; q < 4; ++q) mu_put4(at + 16 * q, at + 16 * q + 64, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
 
-// the product of 32 rows at p and 32 rows at q, of len entries each (lo behind hi)
-__device__ __forceinline__ void mu_small_rows(const char *p, const char *q, int len, mu_f16 &acc)
+struct mu_pair {
+    mu_h8 hi, lo;
+};
+// A lane's eight k of a row that lies in LDS as it is.  p: the row at its first k.
+__device__ __forceinline__ mu_pair mu_by_row(const char *p, int lo) { return {*(const mu_h8 *)p, *(const mu_h8 *)(p + lo)}; }
+// ... of a column of what lies there.  p: where mu_column_at says, in the row of the first k.
+__device__ __forceinline__ mu_pair mu_by_column(const char *p, int pitch, int lo)
+{
+    const mu_h4 h0 = mu_read_column(p), h1 = mu_read_column(p + 4 * pitch), l0 = mu_read_column(p + lo), l1 = mu_read_column(p + 4 * pitch + lo);
+    return {__builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7), __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7)};
+}
+// of 16 lanes four address the same row k, 16 columns; the upper half of a wave takes k from 8 on
+__device__ __forceinline__ int mu_column_at(int lane, int pitch) { return (8 * (lane >> 5) + (lane & 15) / 4) * pitch + 32 * (lane >> 4 & 1) + 8 * (lane & 3); }
+
+__device__ __forceinline__ void mu_three(const mu_pair &p, const mu_pair &q, mu_f16 &acc)
+{
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.lo, p.hi, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.hi, p.lo, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.hi, p.hi, acc, 0, 0, 0);
+}
+// the first of a sum: 0 as an operand of the instruction instead of 16 registers that are cleared
+__device__ __forceinline__ mu_f16 mu_three(const mu_pair &p, const mu_pair &q)
+{
+    mu_f16 acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.lo, p.hi, (mu_f16)(0.0f), 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.hi, p.lo, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(q.hi, p.hi, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mu_zero(mu_f16 &acc)
 {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-#pragma unroll 2
-    for (int k0 = 0; k0 < len; k0 += 16, p += 32, q += 32) {
-        const mu_h8 ph = *(const mu_h8 *)p, pl = *(const mu_h8 *)(p + 2 * len), qh = *(const mu_h8 *)q, ql = *(const mu_h8 *)(q + 2 * len);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
-    }
 }
 
 __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args by_value)
@@ -711,31 +790,32 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     const mu_item &it = a.it[k];
     const int mat = blockIdx.x - it.first, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = lane & 31, half = lane >> 5; // of a fragment: its row, and which 8 of 16 k
-    const int np = mu_small_n(it.n), lp = mu_small_l(it.l), nt = np / 32, tiles = nt * ((lp + 31) / 32);
-    const int px = 4 * lp + 16, pa = 4 * np + 16;
+    const int np = mu_small_n(it.n), lp = mu_small_l(it.l), nt = np / 32;
+    const int px = mu_small_pitch(lp);
     char *const X = mu_lds, *const A = mu_lds + np * px;
 
-    // A wave's tiles of X, four neighbouring columns in every four registers.  They are read (and at the end written) in pieces of
+    // A wave's tiles of X all lie in the same 32 rows (they share what they read of B): tiles (xi, xj + t groups).
+    const int groups = MU_SMALL_WAVES / nt, xi = wave % nt, xj = wave / nt, last = wave < groups * nt ? (lp + 31) / 32 : 0;
+    // A tile is held as four neighbouring columns in every four registers.  They are read (and at the end written) in pieces of
     // four along the side on which g (p) is contiguous, and change hands through LDS, where X will be.
     double s = 0.0;
     const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
 #pragma unroll 1
-    for (int tile = wave; tile < tiles; tile += MU_SMALL_WAVES) {
+    for (int tile = xj; tile < last; tile += groups) {
+        const int i0 = xi * 32, j0 = tile * 32, x = lane % 8 * 4, line = (along_j ? i0 : j0) + lane / 8;
+        float u[16];
+        mu_u<true, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 8 * r; }, (along_j ? j0 : i0) + x, u);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int line = 8 * q + lane / 8, at = lane % 8 * 4;
-            const int i = tile % nt * 32 + (along_j ? line : at), j = tile / nt * 32 + (along_j ? at : line);
-            float u[4];
-            if (along_j) mu_u<true>(a.beta, a.nesterov, it, mat, [&](int) { return i; }, [&](int e) { return j + e; }, u);
-            else mu_u<true>(a.beta, a.nesterov, it, mat, [&](int e) { return i + e; }, [&](int) { return j; }, u);
+        for (int r = 0; r < 4; ++r) {
+            const int i = i0 + (along_j ? 8 * r + lane / 8 : x), j = j0 + (along_j ? x : 8 * r + lane / 8);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += (double)u[e] * u[e];
+            for (int e = 0; e < 4; ++e) s += (double)u[4 * r + e] * u[4 * r + e];
             if (j >= lp) continue; // (a piece lies within lp or outside)
             if (along_j) {
-                *(float4 *)(X + i * px + 4 * j) = make_float4(u[0], u[1], u[2], u[3]);
+                *(float4 *)(X + i * px + 4 * j) = make_float4(u[4 * r], u[4 * r + 1], u[4 * r + 2], u[4 * r + 3]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) *(float *)(X + (i + e) * px + 4 * j) = u[e];
+                for (int e = 0; e < 4; ++e) *(float *)(X + (i + e) * px + 4 * j) = u[4 * r + e];
             }
         }
     }
@@ -757,17 +837,17 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
         lrb_barrier();
         x0 *= red[0];
     }
+    const mu_factor scale(x0);
     const float *coef = own;
     float x[MU_SMALL_TILES][16];
 #pragma unroll
     for (int t = 0; t < MU_SMALL_TILES; ++t) {
-        const int tile = wave + t * MU_SMALL_WAVES;
+        const int tile = xj + t * groups;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int i = tile % nt * 32 + row, j = tile / nt * 32 + 4 * half + 8 * q;
-            const float4 v = tile < tiles && j < lp ? *(const float4 *)(X + i * px + 4 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            x[t][4 * q] = (float)(x0 * v.x), x[t][4 * q + 1] = (float)(x0 * v.y);
-            x[t][4 * q + 2] = (float)(x0 * v.z), x[t][4 * q + 3] = (float)(x0 * v.w);
+            const int i = xi * 32 + row, j = tile * 32 + 4 * half + 8 * q;
+            const float4 v = tile < last && j < lp ? *(const float4 *)(X + i * px + 4 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x[t][4 * q] = scale * v.x, x[t][4 * q + 1] = scale * v.y, x[t][4 * q + 2] = scale * v.z, x[t][4 * q + 3] = scale * v.w;
         }
     }
 
@@ -784,74 +864,104 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
         const int row = lane & 31, half = lane >> 5;
 #pragma unroll
         for (int t = 0; t < MU_SMALL_TILES; ++t) {
-            const int tile = wave + t * MU_SMALL_WAVES, i = tile % nt * 32 + row, j = tile / nt * 32 + 4 * half;
-            if (tile >= tiles) continue;
+            const int tile = xj + t * groups, i = xi * 32 + row, j = tile * 32 + 4 * half;
+            if (tile >= last) continue;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (j + 8 * q >= lp) continue;
-                mu_h4 hi, lo;
                 char *const at = X + i * px + 2 * (j + 8 * q);
-                mu_put4(at, at + 2 * lp, x[t][4 * q], x[t][4 * q + 1], x[t][4 * q + 2], x[t][4 * q + 3], hi, lo);
+                mu_put4(at, at + 2 * lp, x[t][4 * q], x[t][4 * q + 1], x[t][4 * q + 2], x[t][4 * q + 3]);
             }
         }
         lrb_barrier();
         mu_f16 full, acc;
+        mu_zero(full);
         if (sym) {
-            mu_small_rows(X + (ti * 32 + row) * px + 16 * half, X + (tj * 32 + row) * px + 16 * half, lp, full);
+            const char *p = X + (ti * 32 + row) * px + 16 * half, *q = X + (tj * 32 + row) * px + 16 * half;
+            if (ti == tj) {
+                const mu_pair f = mu_by_row(p, 2 * lp);
+                full = mu_three(f, f);
+#pragma unroll 2
+                for (int k0 = 16; k0 < lp; k0 += 16) {
+                    const mu_pair v = mu_by_row(p += 32, 2 * lp);
+                    mu_three(v, v, full);
+                }
+            } else {
+                full = mu_three(mu_by_row(p, 2 * lp), mu_by_row(q, 2 * lp));
+#pragma unroll 2
+                for (int k0 = 16; k0 < lp; k0 += 16) mu_three(mu_by_row(p += 32, 2 * lp), mu_by_row(q += 32, 2 * lp), full);
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) full[e] *= coef[0];
-            mu_put_symmetric(A, np, ti, tj, lane, full);
+            mu_put_block(A + mu_block(ti, tj, nt), lane, full);
         }
         lrb_barrier();
+        const int by_row = row * MU_BLOCK_ROW + 16 * half, by_column = mu_column_at(lane, MU_BLOCK_ROW);
+        mu_zero(acc);
         if (sym) {
-            mu_small_rows(A + (ti * 32 + row) * pa + 16 * half, A + (tj * 32 + row) * pa + 16 * half, np, acc);
+            for (int kb = 0; kb < ti; ++kb) {
+                const char *p = A + mu_block(kb, ti, nt) + by_column, *q = A + mu_block(kb, tj, nt) + by_column;
+#pragma unroll
+                for (int h = 0; h < 2; ++h, p += 16 * MU_BLOCK_ROW, q += 16 * MU_BLOCK_ROW)
+                    mu_three(mu_by_column(p, MU_BLOCK_ROW, 64), mu_by_column(q, MU_BLOCK_ROW, 64), acc);
+            }
+            for (int kb = ti; kb < tj; ++kb) {
+                const char *p = A + mu_block(ti, kb, nt) + by_row, *q = A + mu_block(kb, tj, nt) + by_column;
+#pragma unroll
+                for (int h = 0; h < 2; ++h, p += 32, q += 16 * MU_BLOCK_ROW) mu_three(mu_by_row(p, 64), mu_by_column(q, MU_BLOCK_ROW, 64), acc);
+            }
+            for (int kb = tj; kb < nt; ++kb) {
+                const char *p = A + mu_block(ti, kb, nt) + by_row, *q = A + mu_block(tj, kb, nt) + by_row;
+#pragma unroll
+                for (int h = 0; h < 2; ++h, p += 32, q += 32) mu_three(mu_by_row(p, 64), mu_by_row(q, 64), acc);
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[e] = coef[1] * full[e] + coef[2] * acc[e];
         }
         lrb_barrier();
-        if (sym) mu_put_symmetric(A, np, ti, tj, lane, acc);
+        if (sym) mu_put_block(A + mu_block(ti, tj, nt), lane, acc);
         lrb_barrier();
+        if (xj < last) { // both tiles at once
+            static_assert(MU_SMALL_TILES == 2, "");
+            const bool two = xj + groups < last;
+            mu_f16 other;
+            mu_zero(acc), mu_zero(other);
+            // rows k of X, read by columns; columns past the end give what is not kept
+            const char *q = X + mu_column_at(lane, px) + 64 * xj;
+            for (int kb = 0; kb < nt; ++kb) {
+                const char *p = A + (kb < xi ? mu_block(kb, xi, nt) + by_column : mu_block(xi, kb, nt) + by_row);
 #pragma unroll
-        for (int t = 0; t < MU_SMALL_TILES; ++t) {
-            const int tile = wave + t * MU_SMALL_WAVES;
-            if (tile >= tiles) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-            const char *p = A + (tile % nt * 32 + row) * pa + 16 * half;
-            // rows k of X, 16 columns of the tile for each 16 lanes; columns past the end give what is not kept
-            const char *q = X + (8 * half + (lane & 15) / 4) * px + 2 * (tile / nt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
-#pragma unroll 2
-            for (int k0 = 0; k0 < np; k0 += 16, p += 32, q += 16 * px) {
-                const mu_h8 ph = *(const mu_h8 *)p, pl = *(const mu_h8 *)(p + 2 * np);
-                const mu_h4 h0 = mu_read_column(q), h1 = mu_read_column(q + 4 * px), l0 = mu_read_column(q + 2 * lp),
-                            l1 = mu_read_column(q + 4 * px + 2 * lp);
-                const mu_h8 qh = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7), ql = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
+                for (int h = 0; h < 2; ++h, q += 16 * px) {
+                    const mu_pair v = kb < xi ? mu_by_column(p + h * 16 * MU_BLOCK_ROW, MU_BLOCK_ROW, 64) : mu_by_row(p + h * 32, 64);
+                    mu_three(v, mu_by_column(q, px, 2 * lp), acc);
+                    if (two) mu_three(v, mu_by_column(q + 64 * groups, px, 2 * lp), other);
+                }
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[t][e] = coef[3] * x[t][e] + coef[4] * acc[e];
+            for (int e = 0; e < 16; ++e) {
+                x[0][e] = coef[3] * x[0][e] + coef[4] * acc[e];
+                x[1][e] = coef[3] * x[1][e] + coef[4] * other[e];
+            }
         }
         lrb_barrier();
     }
 #pragma unroll
     for (int t = 0; t < MU_SMALL_TILES; ++t) {
-        const int tile = wave + t * MU_SMALL_WAVES;
+        const int tile = xj + t * groups;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int i = tile % nt * 32 + row, j = tile / nt * 32 + 4 * half + 8 * q;
-            if (tile < tiles && j < lp) *(float4 *)(X + i * px + 4 * j) = make_float4(x[t][4 * q], x[t][4 * q + 1], x[t][4 * q + 2], x[t][4 * q + 3]);
+            const int i = xi * 32 + row, j = tile * 32 + 4 * half + 8 * q;
+            if (tile < last && j < lp) *(float4 *)(X + i * px + 4 * j) = make_float4(x[t][4 * q], x[t][4 * q + 1], x[t][4 * q + 2], x[t][4 * q + 3]);
         }
     }
     mu_wave_sync();
     const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1;
 #pragma unroll 1
-    for (int tile = wave; tile < tiles; tile += MU_SMALL_WAVES) {
+    for (int tile = xj; tile < last; tile += groups) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
             const int line = 8 * q + lane / 8, at = lane % 8 * 4;
-            const int i = tile % nt * 32 + (by_rows ? line : at), j = tile / nt * 32 + (by_rows ? at : line);
+            const int i = xi * 32 + (by_rows ? line : at), j = tile * 32 + (by_rows ? at : line);
             if (i >= it.n || j >= it.l) continue;
             const char *v = X + i * px + 4 * j;
             const int step = by_rows ? 4 : px;
