@@ -524,8 +524,12 @@ template <int T, int WM, int WN, int MODE>
 __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 {
     constexpr int WAVES = WM * WN, MI = T / WM / 32, NI = T / WN / 32;
+    // the smallest tile's products of a stage take less time than its loads: its loads run three stages ahead
+    constexpr int STAGES = T == 64 ? 4 : 2;
     __shared__ __attribute__((aligned(1024))) char buf0[4 * T * 64];
     __shared__ __attribute__((aligned(1024))) char buf1[4 * T * 64];
+    __shared__ __attribute__((aligned(1024))) char buf2[STAGES > 2 ? 4 * T * 64 : 1024];
+    __shared__ __attribute__((aligned(1024))) char buf3[STAGES > 2 ? 4 * T * 64 : 1024];
     // first the workgroups of the whole tiles, then those of the tiles that are cut along k
     const int total = a.start[a.n_items], whole = (a.direct + 7) / 8 * 8, cut = total - a.direct;
     const int unit = (int)blockIdx.x < whole ? mu_by_xcd(blockIdx.x, a.direct) : mu_by_xcd(blockIdx.x - whole, cut * a.splits);
@@ -623,21 +627,49 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     auto turn = [&](char *buf, char *next, int k0) {
         read(f1, buf, 1);
         products(f0);
-        __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0), lgkmcnt(0): the next stage is there, this one is read
+        // lgkmcnt(0): this stage is read; vmcnt: of the loads those of the next stage have arrived
+        __builtin_amdgcn_s_waitcnt(0x0070 | (STAGES - 2) * 2 * FILLS);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        stage(buf, min(k0 + 2 * MU_BK, k_end - MU_BK));
+        stage(buf, min(k0 + STAGES * MU_BK, k_end - MU_BK));
         read(f0, next, 0);
         products(f1);
     };
-    stage(buf0, k_first);
-    stage(buf1, k_first + MU_BK);
-    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
-    lrb_barrier();
-    read(f0, buf0, 0);
-    for (int k0 = k_first; k0 < k_end; k0 += 2 * MU_BK) {
-        turn(buf0, buf1, k0);
-        turn(buf1, buf0, k0 + MU_BK);
+    static_assert((STAGES - 1) * 2 * FILLS < 16 || STAGES == 2, "");
+    int k0 = k_first;
+    auto begin = [&](char *first, char *second, char *third, char *fourth) {
+        stage(first, k0);
+        stage(second, k0 + MU_BK);
+        if (STAGES > 2) {
+            stage(third, min(k0 + 2 * MU_BK, k_end - MU_BK));
+            stage(fourth, min(k0 + 3 * MU_BK, k_end - MU_BK));
+        }
+        __builtin_amdgcn_s_waitcnt(STAGES > 2 ? 0x0F70 | (STAGES - 1) * 2 * FILLS : 0x0F70); // the first stage is there
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        read(f0, first, 0);
+    };
+    if (STAGES == 2) {
+        begin(buf0, buf1, buf2, buf3);
+        for (; k0 < k_end; k0 += 2 * MU_BK) {
+            turn(buf0, buf1, k0);
+            turn(buf1, buf0, k0 + MU_BK);
+        }
+    } else {
+        if ((k_end - k0) & (2 * MU_BK)) { // two stages first, so that four remain a turn
+            begin(buf2, buf3, buf0, buf1);
+            turn(buf2, buf3, k0);
+            turn(buf3, buf0, k0 + MU_BK);
+            k0 += 2 * MU_BK;
+        } else {
+            begin(buf0, buf1, buf2, buf3);
+        }
+        for (; k0 < k_end; k0 += 4 * MU_BK) {
+            turn(buf0, buf1, k0);
+            turn(buf1, buf2, k0 + MU_BK);
+            turn(buf2, buf3, k0 + 2 * MU_BK);
+            turn(buf3, buf0, k0 + 3 * MU_BK);
+        }
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);
     lrb_barrier();
@@ -993,7 +1025,7 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
 
 // The tile: the largest that still gives most of the 256 CUs one (a larger tile loads less for each product).  Both symmetric
 // products take the same (A in float32 is there on and above the diagonal's tiles only).
-// The cut: a CU holds one, two or four workgroups by their LDS, so 256, 512 or 1024 tiles run side by side and take the same
+// The cut: a CU holds one or two workgroups by their LDS, so 256 or 512 tiles run side by side and take the same
 // time; the tiles of the last, unfilled round are cut along k so that all CUs share them.
 static mu_plan mu_lay_out(const mu_args &a, int mode)
 {
@@ -1001,7 +1033,7 @@ static mu_plan mu_lay_out(const mu_args &a, int mode)
     mu_plan p;
     p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 200 ? 128 : 64;
     p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
-    const int slots = p.T == 256 ? 256 : p.T == 128 ? 512 : 1024;
+    const int slots = p.T == 256 ? 256 : 512;
     const long long rest = p.tiles % slots;
     p.direct = (int)p.tiles, p.splits = 1;
     if (rest == 0) return p;
