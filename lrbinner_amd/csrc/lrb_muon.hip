@@ -21,6 +21,10 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "lrb_device.h"
 
 typedef _Float16 mu_h;
@@ -514,8 +518,12 @@ template <int MODE> __device__ __forceinline__ void mu_place(int local, int ti, 
     }
 }
 
-// neighbouring workgroups go to different XCDs: each of the eight takes a run of neighbouring tiles
-__device__ __forceinline__ int mu_by_xcd(int block, int total) { return (block & 7) * ((total + 7) / 8) + (block >> 3); }
+// Neighbouring workgroups go to different XCDs: each of the eight takes a run of neighbouring ones of the n (-1: none is left).
+__host__ __device__ inline int mu_by_xcd(int xcd, int rank, int n)
+{
+    const int first = (int)((long long)n * xcd / 8), end = (int)((long long)n * (xcd + 1) / 8);
+    return first + rank < end ? first + rank : -1;
+}
 
 // One tile of a product.  LDS holds two stages of 32 k: T rows of P and T of Q, 128 bytes each; the eight 16-byte chunks of a
 // row (four of hi, four of lo) lie at chunk ^ ((row >> 1) & 7), which spreads the 16 rows that a quarter wave reads over all
@@ -530,13 +538,28 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     __shared__ __attribute__((aligned(1024))) char buf1[4 * T * 64];
     __shared__ __attribute__((aligned(1024))) char buf2[STAGES > 2 ? 4 * T * 64 : 1024];
     __shared__ __attribute__((aligned(1024))) char buf3[STAGES > 2 ? 4 * T * 64 : 1024];
-    // first the workgroups of the whole tiles, then those of the tiles that are cut along k
-    const int total = a.start[a.n_items], whole = (a.direct + 7) / 8 * 8, cut = total - a.direct;
-    const int unit = (int)blockIdx.x < whole ? mu_by_xcd(blockIdx.x, a.direct) : mu_by_xcd(blockIdx.x - whole, cut * a.splits);
-    const bool part = (int)blockIdx.x >= whole;
-    if (unit >= (part ? cut * a.splits : a.direct)) return;
-    const int tile = part ? a.direct + unit / a.splits : unit;
-    const int k = mu_find(a, tile);
+    // First the workgroups of the whole tiles, item by item, an eighth of each item on every XCD (the items' k differ); then
+    // those of the tiles that are cut along k.
+    int rank = blockIdx.x >> 3, tile = -1, k = 0;
+    for (; k < a.n_items && tile < 0; ++k) {
+        const int n = min(a.start[k + 1], a.direct) - a.start[k], each = (n + 7) / 8;
+        if (n <= 0) continue;
+        if (rank < each) {
+            tile = mu_by_xcd((blockIdx.x + a.start[k]) & 7, rank, n); // (so that items of a few tiles do not all take the same XCDs)
+            if (tile < 0) return;
+            tile += a.start[k--];
+        } else {
+            rank -= each;
+        }
+    }
+    const int units_all = (a.start[a.n_items] - a.direct) * a.splits;
+    const bool part = tile < 0;
+    const int unit = part ? mu_by_xcd(blockIdx.x & 7, rank, units_all) : 0;
+    if (unit < 0) return;
+    if (part) {
+        tile = a.direct + unit / a.splits;
+        k = mu_find(a, tile);
+    }
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
     const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
@@ -1025,16 +1048,16 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
 
 // The tile: the largest that still gives most of the 256 CUs one (a larger tile loads less for each product).  Both symmetric
 // products take the same (A in float32 is there on and above the diagonal's tiles only).
-// The cut: a CU holds one or two workgroups by their LDS, so 256 or 512 tiles run side by side and take the same
-// time; the tiles of the last, unfilled round are cut along k so that all CUs share them.
+// The cut: a round of 256 tiles gives every CU one; the tiles that are left over behind the last whole round are cut along k so
+// that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 12 units of 64 k of the
+// smallest tile, one of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
 static mu_plan mu_lay_out(const mu_args &a, int mode)
 {
     const bool symmetric = mode <= MU_POLY;
     mu_plan p;
     p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 200 ? 128 : 64;
     p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
-    const int slots = p.T == 256 ? 256 : 512;
-    const long long rest = p.tiles % slots;
+    const long long rest = p.tiles % 256;
     p.direct = (int)p.tiles, p.splits = 1;
     if (rest == 0) return p;
     long long units = 1ll << 40; // of 64 k, in the shortest of the rest's products
@@ -1045,9 +1068,9 @@ static mu_plan mu_lay_out(const mu_args &a, int mode)
         const long long u = (mode == MU_GRAM ? a.it[k].lp : a.it[k].np) / 64;
         if (before > p.tiles - rest && u < units) units = u;
     }
-    long long s = slots / rest;
-    if (s > units / 4) s = units / 4; // 256 k a part at least
-    if (s < 2 || units - units / s < 8) return p; // what is saved would not pay for the joining launch
+    long long s = 256 / rest;
+    if (s > units / 3) s = units / 3; // at least 192 k a part
+    if (s < 2 || units - units / s < (p.T == 64 ? 14 : p.T == 128 ? 5 : 2)) return p;
     p.direct = (int)(p.tiles - rest), p.splits = (int)s;
     return p;
 }
@@ -1055,7 +1078,12 @@ static mu_plan mu_lay_out(const mu_args &a, int mode)
 template <int T, int WM, int WN, int MODE> static void mu_launch_tiles(const mu_args &a, const mu_plan &p, hipStream_t st)
 {
     const long long cut = p.tiles - p.direct, units = cut * p.splits;
-    hipLaunchKernelGGL((mu_product_kernel<T, WM, WN, MODE>), dim3((unsigned)((p.direct + 7) / 8 * 8 + (units + 7) / 8 * 8)), dim3(64 * WM * WN), 0, st, a);
+    long long grid = (units + 7) / 8;
+    for (int k = 0; k < a.n_items; ++k) {
+        const int n = (a.start[k + 1] < p.direct ? a.start[k + 1] : p.direct) - a.start[k];
+        if (n > 0) grid += (n + 7) / 8;
+    }
+    hipLaunchKernelGGL((mu_product_kernel<T, WM, WN, MODE>), dim3((unsigned)(grid * 8)), dim3(64 * WM * WN), 0, st, a);
     if (cut) hipLaunchKernelGGL((mu_join_kernel<T, WM, WN, MODE>), dim3((unsigned)(cut * (T / 32) * WN)), dim3(64), 0, st, a);
 }
 
@@ -1094,9 +1122,13 @@ struct mu_group {
 // Calls `go(group)` for each group of the list in turn, those of small matrices first; stops at its first non-zero answer.
 template <typename F> static int mu_each_group(const lrb_muon_item *items, int n_items, F go)
 {
+    // the largest first: what is left for the last, unfilled round of a launch are then the least
+    std::vector<int> order(n_items);
+    for (int k = 0; k < n_items; ++k) order[k] = k;
+    std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return items[x].rows * items[x].cols > items[y].rows * items[y].cols; });
     for (int small = 1; small >= 0; --small) {
         mu_group gr = {};
-        for (int k = 0; k < n_items; ++k) {
+        for (int k : order) {
             const lrb_muon_item &s = items[k];
             if (s.count <= 0 || s.rows <= 0 || s.cols <= 0) continue;
             const bool turned = s.rows > s.cols;
@@ -1178,10 +1210,14 @@ extern "C" uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items)
 {
     if (n_items <= 0 || !items || !mu_items_fit(items, n_items)) return 0;
     uint64_t most = 0;
-    mu_each_group(items, n_items, [&](mu_group &gr) {
-        if (gr.bytes() > most) most = gr.bytes();
-        return LRB_OK;
-    });
+    try {
+        mu_each_group(items, n_items, [&](mu_group &gr) {
+            if (gr.bytes() > most) most = gr.bytes();
+            return LRB_OK;
+        });
+    } catch (const std::bad_alloc &) {
+        return UINT64_MAX; // no workspace is as large: the call that follows is refused
+    }
     return most;
 }
 
@@ -1202,7 +1238,8 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
     hipStream_t st = (hipStream_t)stream;
     float std[MU_STEPS * MU_COEF] = {};
     const double sx = mu_chain(a, b, c, steps, 1.0, std);
-    return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
+    try {
+        return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
         mu_args &g = gr.a;
         g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
         g.sx = sx;
@@ -1236,4 +1273,8 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
         HIP_TRY(hipGetLastError());
         return LRB_OK;
     });
+    } catch (const std::bad_alloc &) {
+        lrb_set_error("out of memory%s%s", "", "");
+        return LRB_ERR_NOMEM;
+    }
 }
