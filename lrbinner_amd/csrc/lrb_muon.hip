@@ -32,9 +32,11 @@ typedef mu_h mu_h8 __attribute__((ext_vector_type(8)));
 typedef mu_h mu_h4 __attribute__((ext_vector_type(4)));
 typedef float mu_f16 __attribute__((ext_vector_type(16)));
 
-#define MU_ITEMS 16       // weights of one launch (their descriptors travel as kernel arguments)
+#define MU_ITEMS 14       // weights of one launch (their descriptors travel as kernel arguments)
 #define MU_STEPS 32       // longest iteration
-#define MU_COEF 5         // floats of the table for each matrix and step: kA, kB1, kB2, kX1, kX2
+#define MU_BLOCK_STEPS 5  // most steps between two formations of X
+#define MU_COEF 3         // factors of an operation
+#define MU_OPS 128        // operations of the longest iteration: 3 of a single step, 4 n - 1 of a block of n
 #define MU_TOP 57344.0    // the largest entry that a factor is scaled to: 7/8 of fp16's largest number
 #define MU_BK 32          // k of one stage in LDS
 
@@ -52,49 +54,58 @@ struct mu_item {
 
 struct mu_args {
     char *ws;
-    double *x0;     // [matrices] what u is multiplied by
-    float *table;   // [matrices][steps][MU_COEF]
+    double *x0;     // [matrices][2] what u is multiplied by; 1 if the launch's own factors hold, 0 for those of the table
+    float *table;   // [matrices][MU_OPS][MU_COEF]
     double *part;   // [tiles of 64 x 64 of all matrices] sums of squares
     int n_items, steps;
     float beta, eps, a, b, c;
     int nesterov;
     int flip;       // which of the two copies of X is read
-    int step;
+    // the operation: its number, its factors for a norm of at least eps, and the n x n buffers it reads and writes (see mu_strip)
+    int op;
+    float k[MU_COEF];
+    int u, v, old, old2, out, keep; // keep: the result in float32 too
+    int n_sizes;                     // the iteration's blocks
+    uint8_t sizes[MU_STEPS];
     // of a product's launch: the tiles from `direct` on are cut along k, `splits` workgroups each, whose sums go to `parts`
     int direct, splits;
     float *parts;
-    double sx;                      // the scale of X at the start, and the table, for a norm of at least eps
-    float std[MU_STEPS * MU_COEF];
+    double sx;                       // the scale of X at the start for a norm of at least eps
+    float std[MU_STEPS * 3 * MU_COEF]; // and all factors, of single steps (for the small matrices)
     int start[MU_ITEMS + 1]; // first tile of each item in this launch
     mu_item it[MU_ITEMS];
 };
 static_assert(sizeof(mu_args) <= 4096, "kernel arguments");
 
-// The factors of a matrix: X and its transpose twice (read and written in turn), A, B, as rows of 32 hi, the 32 lo of the same
-// entries, the next 32 hi ...: 32 k of a row are one whole line of 128 bytes, which halves the requests that the L2 gets for a
-// stage against separate planes (2.1 -> 1.05 requests for 128 bytes).  And X and A in
-// float32, for the terms a X and b A: hi + lo is a rounding more than float32 is, and these terms would pass it on.
-__host__ __device__ inline unsigned long long mu_plane_x(const mu_item &it) { return 2ull * (unsigned long long)it.np * it.lp; }
-__host__ __device__ inline unsigned long long mu_plane_a(const mu_item &it) { return 2ull * (unsigned long long)it.np * it.np; }
-__host__ __device__ inline unsigned long long mu_bytes(const mu_item &it) { return 10 * mu_plane_x(it) + 6 * mu_plane_a(it); }
+// A matrix in the workspace: X and its transpose twice (read and written in turn), and four n x n buffers for A, B and what
+// is made of them, as rows of 32 hi, the 32 lo of the same entries, the next 32 hi ...: 32 k of a row are one whole line of 128
+// bytes, which halves the requests that the L2 gets for a stage against separate planes of hi and lo (4096 x 4096, B X: 43 M ->
+// 21 M).  And X and the buffers in float32, for the terms that are not products (a X, b A ...): hi + lo is a rounding more than
+// float32 is, and these terms would pass it on.  Of symmetric matrices the float32 is there on and above the diagonal's tiles.
+__host__ __device__ inline unsigned long long mu_plane_x(const mu_item &it) { return 4ull * (unsigned long long)it.np * it.lp; }
+__host__ __device__ inline unsigned long long mu_plane_a(const mu_item &it) { return 4ull * (unsigned long long)it.np * it.np; }
+__host__ __device__ inline unsigned long long mu_bytes(const mu_item &it, int buffers) { return 5 * mu_plane_x(it) + 2 * buffers * mu_plane_a(it); }
 
 struct mu_mat {
-    mu_h *x, *xt, *x2, *xt2, *a, *b;
-    float *x32, *a32;
+    mu_h *x, *xt, *x2, *xt2;
+    float *x32;
+    char *buffers;
+    unsigned long long pa;
+    __device__ __forceinline__ mu_h *half(int b) const { return (mu_h *)(buffers + 2 * b * pa); }
+    __device__ __forceinline__ float *full(int b) const { return (float *)(buffers + (2 * b + 1) * pa); }
 };
 __device__ __forceinline__ mu_mat mu_planes(const mu_args &a, const mu_item &it, int mat)
 {
     char *w = a.ws + it.off + (unsigned long long)mat * it.step;
-    const unsigned long long px = 2 * mu_plane_x(it), pa = 2 * mu_plane_a(it);
+    const unsigned long long px = mu_plane_x(it);
     mu_mat r;
     r.x = (mu_h *)(w + (a.flip ? 2 * px : 0));
     r.xt = (mu_h *)(w + (a.flip ? 3 * px : px));
     r.x2 = (mu_h *)(w + (a.flip ? 0 : 2 * px));
     r.xt2 = (mu_h *)(w + (a.flip ? px : 3 * px));
-    r.a = (mu_h *)(w + 4 * px);
-    r.b = (mu_h *)(w + 4 * px + pa);
-    r.x32 = (float *)(w + 4 * px + 2 * pa);
-    r.a32 = (float *)(w + 5 * px + 2 * pa);
+    r.x32 = (float *)(w + 4 * px);
+    r.buffers = w + 5 * px;
+    r.pa = mu_plane_a(it);
     return r;
 }
 
@@ -244,30 +255,96 @@ __host__ __device__ double mu_scale(double r) // the power of two that takes ent
     return ldexp(1.0, e - 1);
 }
 
-// The scale of X at the start, for singular values up to r, and the five factors of every step.
-__host__ __device__ inline double mu_chain(double a, double b, double c, int steps, double r, float *t)
+// The operations of an iteration in blocks of sizes[0], sizes[1] ... steps, in their order:
+//   gram()       A = X X^T
+//   then for every step k of a block of n
+//   poly(k)      P = b A + c A^2
+//   sum(k)       k > 0: S <- a S + a^k P + P S        (a^(k+1) I + S is the product of all (a I + P) so far; S = P for k = 0)
+//   turn()       k + 1 < n: C = a A + P A             (all of these are polynomials of the same A: they commute, and the
+//   turn2()                 A <- a C + C P             products are symmetric)
+//   apply(n)     X <- a^n X + S X
+// A block of one step is the iteration as it is written.  A longer one forms X and X X^T once for its n steps, and pays with
+// four symmetric n x n products a step more: for X of n x r n entries 1.5 r + 4.5 units of 2 n^3 for three steps against
+// 4.5 r + 1.5.
+template <typename V> __host__ __device__ inline void mu_walk(const uint8_t *sizes, int n_sizes, V &v)
 {
-    const double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
-    r *= slack;
-    const double s0 = mu_scale(r);
-    double sx = s0;
-    for (int q = 0; q < steps; ++q, t += MU_COEF) {
-        const double ra = r * r * slack, sa = mu_scale(ra);
-        double rb = fabs(b * ra + c * ra * ra);
-        if (c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < ra) rb = fmax(rb, b * b / fabs(4.0 * c));
-        rb *= slack;
-        const double sb = mu_scale(rb);
-        r = mu_largest_odd(a, b, c, r) * slack;
-        const double sn = q + 1 < steps ? mu_scale(r) : 1.0;
-        t[0] = (float)(sa / (sx * sx));
-        t[1] = (float)(b * (sb / sa));
-        t[2] = (float)(c * (sb / sa) / sa);
-        t[3] = (float)(a * (sn / sx));
-        t[4] = (float)(sn / sb / sx);
-        sx = sn;
+    for (int q = 0; q < n_sizes; ++q) {
+        const int n = sizes[q];
+        v.gram();
+        for (int k = 0; k < n; ++k) {
+            v.poly(k, n);
+            if (k > 0) v.sum(k, n);
+            if (k + 1 < n) {
+                v.turn();
+                v.turn2();
+            }
+        }
+        v.apply(n, q + 1 == n_sizes);
     }
-    return s0;
 }
+
+// Writes the factors of every operation: of the old entry, the sum of products, and the second old entry.  Scales are powers
+// of two, from bounds on the largest singular values.
+struct mu_chain {
+    double a, b, c, r, sx, ra = 0.0, sa = 0.0, sp = 0.0, ss = 0.0, sc = 0.0, product = 1.0;
+    float *t;
+    static constexpr double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
+    __host__ __device__ mu_chain(double a_, double b_, double c_, double r_, float *t_) : a(a_), b(b_), c(c_), r(r_ * slack), t(t_) { sx = mu_scale(r); }
+    __host__ __device__ void put(double k0, double k1, double k2)
+    {
+        t[0] = (float)k0, t[1] = (float)k1, t[2] = (float)k2;
+        t += MU_COEF;
+    }
+    __host__ __device__ double largest(double first) const // max |first + b t + c t^2| over [0, ra]
+    {
+        double m = fmax(fabs(first), fabs(first + b * ra + c * ra * ra));
+        if (c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < ra) m = fmax(m, fabs(first - b * b / (4.0 * c)));
+        return m * slack;
+    }
+    __host__ __device__ void gram()
+    {
+        ra = r * r * slack, sa = mu_scale(ra);
+        put(0.0, sa / (sx * sx), 0.0);
+    }
+    __host__ __device__ void poly(int k, int)
+    {
+        sp = mu_scale(largest(0.0));
+        put(b * (sp / sa), c * (sp / sa) / sa, 0.0);
+        product = (k ? product : 1.0) * largest(a);
+        if (k == 0) ss = sp;
+    }
+    __host__ __device__ void sum(int k, int)
+    {
+        double power = 1.0;
+        for (int q = 0; q < k; ++q) power *= a;
+        const double s = mu_scale(fabs(power * a) + product);
+        put(a * (s / ss), s / sp / ss, power * (s / sp));
+        ss = s;
+    }
+    __host__ __device__ void turn()
+    {
+        const double next = mu_largest_odd(a, b, c, r) * slack;
+        sc = mu_scale(r * next * slack);
+        put(a * (sc / sa), sc / sp / sa, 0.0);
+        r = next;
+    }
+    __host__ __device__ void turn2()
+    {
+        ra = r * r * slack;
+        const double s = mu_scale(ra);
+        put(a * (s / sc), s / sc / sp, 0.0);
+        sa = s;
+    }
+    __host__ __device__ void apply(int n, bool last)
+    {
+        double power = 1.0;
+        for (int q = 0; q < n; ++q) power *= a;
+        r = mu_largest_odd(a, b, c, r) * slack;
+        const double s = last ? 1.0 : mu_scale(r);
+        put(power * (s / sx), s / ss / sx, 0.0);
+        sx = s;
+    }
+};
 
 // From the sum of the squares of u: what u is multiplied by to become X, and the bound r on X's singular values.  At r = 1 the
 // ready table holds.  An infinity or a NaN anywhere makes the whole matrix NaN.
@@ -298,10 +375,16 @@ __global__ __launch_bounds__(256) void mu_table_kernel(mu_args a)
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     lrb_barrier();
+    if (threadIdx.x) return;
     const mu_norm n = mu_start(red[0] + red[1] + red[2] + red[3], a.eps);
-    float *t = a.table + (size_t)blockIdx.x * a.steps * MU_COEF;
-    if (n.r == 1.0 && (int)threadIdx.x < a.steps * MU_COEF) t[threadIdx.x] = a.std[threadIdx.x];
-    if (threadIdx.x == 0) a.x0[blockIdx.x] = n.x0 * (n.r == 1.0 ? a.sx : mu_chain(a.a, a.b, a.c, a.steps, n.r, t));
+    double scale = a.sx;
+    if (n.r != 1.0) {
+        mu_chain chain(a.a, a.b, a.c, n.r, a.table + (size_t)blockIdx.x * MU_OPS * MU_COEF);
+        scale = chain.sx;
+        mu_walk(a.sizes, a.n_sizes, chain);
+    }
+    a.x0[2 * blockIdx.x] = n.x0 * scale;
+    a.x0[2 * blockIdx.x + 1] = n.r == 1.0 ? 1.0 : 0.0;
 }
 
 // hi = fp16(v), lo = fp16(v - hi), in two instructions an entry: pairs are converted together, and the difference takes hi as
@@ -342,7 +425,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
     const int tj = it.lp / 64, per = (it.np / 64) * tj, local = blockIdx.x - a.start[k], mat = local / per, r = local % per;
     const int i0 = (r / tj) * 64, j0 = (r % tj) * 64;
     const bool along_j = it.gs[2] == 1 || it.gs[1] != 1;
-    const mu_factor scale(a.x0[it.first + mat]);
+    const mu_factor scale(a.x0[2 * (it.first + mat)]);
     float u[16];
     const int first = threadIdx.x >> 4, x = (threadIdx.x & 15) * 4, line = (along_j ? i0 : j0) + first;
     mu_u<false, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, (along_j ? j0 : i0) + x, u);
@@ -375,7 +458,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
     }
 }
 
-enum { MU_GRAM = 0, MU_POLY = 1, MU_APPLY = 2, MU_LAST = 3 };
+enum { MU_GRAM = 0, MU_SYM = 1, MU_APPLY = 2, MU_LAST = 3 };
 
 __device__ __forceinline__ void mu_dma(const char *src, char *dst)
 {
@@ -423,17 +506,28 @@ __device__ __forceinline__ void mu_update4(const mu_item &it, long long at, long
 // What becomes of 32 x 32 NI entries of a product, of which a wave holds the sums: acc[y][4 q + e] of a lane is row (lane & 31),
 // column 32 y + 8 q + 4 (lane >> 5) + e.  They go through `lds` (32 rows of MU_PITCH) to be read, combined and written in
 // whole row segments, and once more by columns for the mirrored or transposed side.
+//   MU_GRAM, MU_SYM: buffer `out` = k0 old + k1 sum + k2 old2 (buffers; -1: none)      MU_APPLY: X = k0 X + k1 sum; MU_LAST: p
 #define MU_PITCH(NI) (32 * (NI) + 4)
+struct mu_factors {
+    float k0, k1, k2;
+    // (asked for before the products, so that the results do not wait for it)
+    __device__ __forceinline__ mu_factors(const mu_args &a, int matrix) : k0(a.k[0]), k1(a.k[1]), k2(a.k[2])
+    {
+        if (a.x0[2 * matrix + 1] == 0.0) {
+            const float *t = a.table + ((size_t)matrix * MU_OPS + a.op) * MU_COEF;
+            k0 = t[0], k1 = t[1], k2 = t[2];
+        }
+    }
+};
 template <int MODE, int NI>
-__device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, int mat, const mu_mat &w, const mu_f16 (&acc)[NI], int i0, int j0,
+__device__ __forceinline__ void mu_strip(const mu_args &a, const mu_factors &f, const mu_item &it, int mat, const mu_mat &w, const mu_f16 (&acc)[NI], int i0, int j0,
                                          bool mirror, float *lds, int lane)
 {
     constexpr int PITCH = MU_PITCH(NI), LANES = 8 * NI, ROWS = 64 / LANES; // lanes of a row, rows of a turn
-    const float *t = a.table + ((size_t)(it.first + mat) * a.steps + a.step) * MU_COEF;
-    const float k1 = MODE == MU_GRAM ? 0.0f : MODE == MU_POLY ? t[1] : t[3], k2 = MODE == MU_GRAM ? t[0] : MODE == MU_POLY ? t[2] : t[4];
     const int ld = MODE >= MU_APPLY ? it.lp : it.np;
-    float *full = MODE <= MU_POLY ? w.a32 : w.x32;
-    mu_h *out = MODE == MU_GRAM ? w.a : MODE == MU_POLY ? w.b : w.x2, *out_t = MODE == MU_APPLY ? w.xt2 : out;
+    const float *old = MODE >= MU_APPLY ? w.x32 : a.old >= 0 ? w.full(a.old) : nullptr, *old2 = MODE == MU_SYM && a.old2 >= 0 ? w.full(a.old2) : nullptr;
+    float *full = MODE == MU_APPLY ? w.x32 : MODE <= MU_SYM ? w.full(a.out) : nullptr;
+    mu_h *out = MODE == MU_APPLY ? w.x2 : w.half(a.out), *out_t = MODE == MU_APPLY ? w.xt2 : out;
     const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1; // which way p is written
     mu_wave_sync();
 #pragma unroll
@@ -449,16 +543,20 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_item &it, in
         const int c = (lane % LANES) * 4, i = i0 + r, j = j0 + c;
         if (i >= it.np || j >= ld) continue;
         float4 v = *(const float4 *)(lds + r * PITCH + c);
-        float4 *const old = (float4 *)(full + (size_t)i * ld + j);
-        const float4 o = MODE == MU_GRAM ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *old;
-        v = make_float4(k1 * o.x + k2 * v.x, k1 * o.y + k2 * v.y, k1 * o.z + k2 * v.z, k1 * o.w + k2 * v.w);
+        const size_t at = (size_t)i * ld + j;
+        const float4 o = MODE >= MU_APPLY || old ? *(const float4 *)(old + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v = make_float4(f.k0 * o.x + f.k1 * v.x, f.k0 * o.y + f.k1 * v.y, f.k0 * o.z + f.k1 * v.z, f.k0 * o.w + f.k1 * v.w);
+        if (MODE == MU_SYM && old2) {
+            const float4 o2 = *(const float4 *)(old2 + at);
+            v.x += f.k2 * o2.x, v.y += f.k2 * o2.y, v.z += f.k2 * o2.z, v.w += f.k2 * o2.w;
+        }
         if (back) *(float4 *)(lds + r * PITCH + c) = v;
         if (MODE == MU_LAST) {
             if (by_rows && i < it.n && j < it.l) mu_update4(it, mat * it.ps[0] + i * it.ps[1] + j * it.ps[2], it.ps[2], min(4, it.l - j), v);
         } else {
             mu_h4 hi, lo;
             mu_split4(v.x, v.y, v.z, v.w, hi, lo);
-            if (MODE != MU_POLY) *old = v; // B is a factor only
+            if (MODE != MU_SYM || a.keep) *(float4 *)(full + at) = v;
             *(mu_h4 *)(out + mu_at(i, j, ld)) = hi;
             *(mu_h4 *)(out + mu_at(i, j, ld) + 32) = lo;
         }
@@ -567,8 +665,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     mu_place<MODE>(local % per, ti, tj, i0, j0);
     i0 *= T, j0 *= T;
     const mu_mat w = mu_planes(a, it, mat);
+    const mu_factors factors(a, it.first + mat);
     const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
-    const mu_h *P = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.b, *Q = MODE == MU_GRAM ? w.x : MODE == MU_POLY ? w.a : w.xt;
+    const mu_h *P = MODE == MU_GRAM ? w.x : w.half(a.u), *Q = MODE == MU_GRAM ? w.x : MODE == MU_SYM ? w.half(a.v) : w.xt;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN, wj = wave % WN;
 
     // A load of a wave fills eight rows of a stage.  All addresses are a factor's first row of the tile (uniform) and an offset of
@@ -715,7 +814,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const bool mirror = MODE == MU_APPLY || i0 != j0;
 #pragma unroll
     for (int x = 0; x < MI; ++x)
-        mu_strip<MODE, NI>(a, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane);
+        mu_strip<MODE, NI>(a, factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane);
 }
 
 // The tiles that were cut along k: their parts' sums, added up in order, a wave for each 32 rows of one of the tile's waves.
@@ -748,7 +847,8 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
                 acc[y][4 * q] += v.x, acc[y][4 * q + 1] += v.y, acc[y][4 * q + 2] += v.z, acc[y][4 * q + 3] += v.w;
             }
     const mu_mat w = mu_planes(a, it, mat);
-    mu_strip<MODE, NI>(a, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
+    const mu_factors factors(a, it.first + mat);
+    mu_strip<MODE, NI>(a, factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
 }
 
 // A matrix that fits one workgroup's LDS (128 x 208, 96 x 320, 64 x 512, 32 x 1,024 and less) goes through all its steps there, in one
@@ -839,7 +939,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     const mu_args &a = *(const mu_args *)__builtin_amdgcn_kernarg_segment_ptr();
     extern __shared__ __attribute__((aligned(16))) char mu_lds[];
     __shared__ double red[MU_SMALL_WAVES];
-    __shared__ float own[MU_STEPS * MU_COEF];
+    __shared__ float own[MU_STEPS * 3 * MU_COEF];
     int k = 0;
     while (k + 1 < a.n_items && (int)blockIdx.x >= a.it[k + 1].first) ++k;
     const mu_item &it = a.it[k];
@@ -884,11 +984,15 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     const mu_norm n = mu_start(s, a.eps);
     double x0 = n.x0;
     if (n.r == 1.0) { // (all threads have the same s)
-        if ((int)threadIdx.x < a.steps * MU_COEF) own[threadIdx.x] = a.std[threadIdx.x];
+        if ((int)threadIdx.x < a.steps * 3 * MU_COEF) own[threadIdx.x] = a.std[threadIdx.x];
         x0 *= a.sx;
     } else { // a norm below eps
         lrb_barrier(); // red has been read
-        if (threadIdx.x == 0) red[0] = mu_chain(a.a, a.b, a.c, a.steps, n.r, own);
+        if (threadIdx.x == 0) {
+            mu_chain chain(a.a, a.b, a.c, n.r, own);
+            red[0] = chain.sx;
+            mu_walk(a.sizes, a.n_sizes, chain);
+        }
         lrb_barrier();
         x0 *= red[0];
     }
@@ -912,7 +1016,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     while (ti < nt && tj >= nt - ti) tj -= nt - ti++;
     tj += ti;
     const bool sym = ti < nt;
-    for (int step = 0; step < a.steps; ++step, coef += MU_COEF) {
+    for (int step = 0; step < a.steps; ++step, coef += 3 * MU_COEF) {
         // the addresses below are made anew in every step: kept over the steps, all of them together spill
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
@@ -947,7 +1051,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
                 for (int k0 = 16; k0 < lp; k0 += 16) mu_three(mu_by_row(p += 32, 2 * lp), mu_by_row(q += 32, 2 * lp), full);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) full[e] *= coef[0];
+            for (int e = 0; e < 16; ++e) full[e] *= coef[1];
             mu_put_block(A + mu_block(ti, tj, nt), lane, full);
         }
         lrb_barrier();
@@ -971,7 +1075,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
                 for (int h = 0; h < 2; ++h, p += 32, q += 32) mu_three(mu_by_row(p, 64), mu_by_row(q, 64), acc);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = coef[1] * full[e] + coef[2] * acc[e];
+            for (int e = 0; e < 16; ++e) acc[e] = coef[3] * full[e] + coef[4] * acc[e];
         }
         lrb_barrier();
         if (sym) mu_put_block(A + mu_block(ti, tj, nt), lane, acc);
@@ -994,8 +1098,8 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                x[0][e] = coef[3] * x[0][e] + coef[4] * acc[e];
-                x[1][e] = coef[3] * x[1][e] + coef[4] * other[e];
+                x[0][e] = coef[6] * x[0][e] + coef[7] * acc[e];
+                x[1][e] = coef[6] * x[1][e] + coef[7] * other[e];
             }
         }
         lrb_barrier();
@@ -1053,7 +1157,7 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
 // smallest tile, one of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
 static mu_plan mu_lay_out(const mu_args &a, int mode)
 {
-    const bool symmetric = mode <= MU_POLY;
+    const bool symmetric = mode <= MU_SYM;
     mu_plan p;
     p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 200 ? 128 : 64;
     p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
@@ -1090,14 +1194,99 @@ template <int T, int WM, int WN, int MODE> static void mu_launch_tiles(const mu_
 template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
 {
     const mu_plan p = mu_lay_out(a, MODE);
-    mu_tiles(a, MODE <= MU_POLY, p.T, a.start);
+    mu_tiles(a, MODE <= MU_SYM, p.T, a.start);
     a.direct = p.direct, a.splits = p.splits;
     if (p.T == 256) mu_launch_tiles<256, 2, 4, MODE>(a, p, st);
     else if (p.T == 128) mu_launch_tiles<128, 2, 2, MODE>(a, p, st);
     else mu_launch_tiles<64, 2, 2, MODE>(a, p, st);
 }
 
+// How many steps a block takes.  It is longer than one where X is longer than wide (from 1.3 on it saves a tenth and more of the
+// products) and large (below, its launches cost more than that), and as long as the result's type allows.  What a block of n
+// steps loses: A is carried from step to step instead of being formed anew, and its rounding errors in the directions of small
+// singular values, 2^-24 of the largest, grow by a^2 a step; with (3.4445, -4.775, 2.0315) that is at most a^(2 n - 2) 2^-24,
+// which has to stay below half a step of the result (5 steps for bfloat16: measured 2e-4 at the worst, of 1.7e-3 that the rounding
+// of the result makes; 4 for float16).  Float32 takes two steps at the beginning, where that is measured to lose nothing
+// (1.6e-6 against 1.6e-6, 2.1e-6 against 2.1e-6), and single ones from there on (two blocks of two: 1.2 to 2 times the error).
+static void mu_blocks(mu_args &g)
+{
+    double square = 0.0, wide = 0.0;
+    int most = MU_BLOCK_STEPS;
+    bool exact = false;
+    const double a2 = fabs((double)g.a) > 1.0 ? 2.0 * log2(fabs((double)g.a)) : 0.0;
+    for (int k = 0; k < g.n_items; ++k) {
+        const mu_item &it = g.it[k];
+        square += (double)it.count * it.np * it.np * it.np, wide += (double)it.count * it.np * it.np * it.lp;
+        const double spare = it.p_type == LRB_BF16 ? 16.0 : it.p_type == LRB_F16 ? 13.0 : 0.0; // log2 of half a step over 2^-24
+        const int n = a2 > 0.0 ? 1 + (int)fmin(spare / a2, 30.0) : MU_BLOCK_STEPS;
+        exact |= it.p_type == LRB_F32;
+        most = most < n ? most : n;
+    }
+    if (wide < 1.3 * square || wide < 5e8) return;
+    int left = g.steps;
+    g.n_sizes = 0;
+    while (left > 0) {
+        const int n = exact ? (g.n_sizes == 0 ? 2 : 1) : most;
+        g.sizes[g.n_sizes++] = (uint8_t)(n < left ? n : left);
+        left -= n;
+    }
+}
+
+// Launches the operations of an iteration, and says which of the four n x n buffers hold what.
+struct mu_launcher {
+    mu_args &g;
+    hipStream_t st;
+    mu_chain chain;
+    float factors[MU_OPS * MU_COEF];
+    int op = 0, A = 0, P = 1, S = 1, C = 2;
+    mu_launcher(mu_args &args, hipStream_t stream) : g(args), st(stream), chain(g.a, g.b, g.c, 1.0, factors) { mu_walk(g.sizes, g.n_sizes, chain); }
+    mu_launcher(const mu_launcher &) = delete;
+    int unused(int x, int y, int z) const // the least buffer that is none of these
+    {
+        int b = 0;
+        while (b == x || b == y || b == z) ++b;
+        return b;
+    }
+    template <int MODE> void launch(int u, int v, int old, int old2, int out, bool keep = true)
+    {
+        g.op = op;
+        memcpy(g.k, factors + op++ * MU_COEF, sizeof(g.k));
+        g.u = u, g.v = v, g.old = old, g.old2 = old2, g.out = out, g.keep = keep;
+        mu_launch_product<MODE>(g, st);
+    }
+    void gram()
+    {
+        A = 0;
+        launch<MU_GRAM>(0, 0, -1, -1, A);
+    }
+    void poly(int k, int n)
+    {
+        P = k ? unused(A, S, A) : 1;
+        launch<MU_SYM>(A, A, A, -1, P, n > 1); // of a single step's it is a factor only
+        if (k == 0) S = P;
+    }
+    void sum(int k, int n)
+    {
+        const int to = unused(A, P, S);
+        launch<MU_SYM>(P, S, S, P, to, k + 1 < n);
+        S = to;
+    }
+    void turn()
+    {
+        C = unused(A, P, S);
+        launch<MU_SYM>(P, A, A, -1, C);
+    }
+    void turn2() { launch<MU_SYM>(C, P, C, -1, A); }
+    void apply(int, bool last)
+    {
+        if (last) launch<MU_LAST>(S, 0, -1, -1, 0);
+        else launch<MU_APPLY>(S, 0, -1, -1, 0);
+        g.flip ^= 1;
+    }
+};
+
 // A run of items (or of some matrices of one) that fits the descriptors and MU_WS_MOST bytes, and what it takes.
+#define MU_BUFFERS 4 // n x n, of each matrix
 #define MU_WS_MOST (4ull << 30)
 #define MU_MATS_MOST 4096
 struct mu_group {
@@ -1106,6 +1295,10 @@ struct mu_group {
     int mats;
     long long tiles;
     uint64_t planes;
+    // sizes of what lies behind the planes
+    uint64_t x0_bytes() const { return ((uint64_t)mats * 16 + 255) / 256 * 256; }
+    uint64_t sums_bytes() const { return ((uint64_t)tiles * 8 + 255) / 256 * 256; }
+    uint64_t table_bytes() const { return ((uint64_t)mats * MU_OPS * MU_COEF * 4 + 255) / 256 * 256; }
     uint64_t bytes() const
     {
         if (lds) return 0;
@@ -1114,8 +1307,7 @@ struct mu_group {
             const uint64_t b = mu_lay_out(a, mode).part_bytes();
             parts = b > parts ? b : parts;
         }
-        return planes + parts + ((uint64_t)mats * 8 + 255) / 256 * 256 + ((uint64_t)tiles * 8 + 255) / 256 * 256 +
-               ((uint64_t)mats * MU_STEPS * MU_COEF * 4 + 255) / 256 * 256;
+        return planes + parts + x0_bytes() + sums_bytes() + table_bytes();
     }
 };
 
@@ -1137,7 +1329,7 @@ template <typename F> static int mu_each_group(const lrb_muon_item *items, int n
             const int lds = mu_small_bytes(it.n, it.l);
             if ((lds != 0) != (small != 0)) continue;
             it.np = (it.n + 63) / 64 * 64, it.lp = (it.l + 63) / 64 * 64;
-            it.step = mu_bytes(it);
+            it.step = mu_bytes(it, MU_BUFFERS);
             for (int d = 0; d < 3; ++d) {
                 const int from = d && turned ? 3 - d : d;
                 it.ps[d] = s.p_stride[from], it.gs[d] = s.g_stride[from], it.ms[d] = s.m_stride[from];
@@ -1236,14 +1428,20 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
     lrb_on_device on(device);
     HIP_TRY(on.err);
     hipStream_t st = (hipStream_t)stream;
-    float std[MU_STEPS * MU_COEF] = {};
-    const double sx = mu_chain(a, b, c, steps, 1.0, std);
+    float std[MU_STEPS * 3 * MU_COEF] = {};
+    uint8_t ones[MU_STEPS];
+    memset(ones, 1, sizeof(ones));
+    mu_chain chain(a, b, c, 1.0, std);
+    const double sx = chain.sx;
+    mu_walk(ones, steps, chain);
     try {
         return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
         mu_args &g = gr.a;
         g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
         g.sx = sx;
         memcpy(g.std, std, sizeof(std));
+        memcpy(g.sizes, ones, sizeof(ones));
+        g.n_sizes = steps;
         if (gr.lds) {
             static lrb_per_device_once raised;
             if (raised.need(device)) {
@@ -1255,21 +1453,16 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
         }
         g.ws = (char *)d_ws;
         char *at = g.ws + gr.planes;
-        g.x0 = (double *)at, at += ((uint64_t)gr.mats * 8 + 255) / 256 * 256;
-        g.part = (double *)at, at += ((uint64_t)gr.tiles * 8 + 255) / 256 * 256;
-        g.table = (float *)at, at += ((uint64_t)gr.mats * MU_STEPS * MU_COEF * 4 + 255) / 256 * 256;
+        g.x0 = (double *)at, at += gr.x0_bytes();
+        g.part = (double *)at, at += gr.sums_bytes();
+        g.table = (float *)at, at += gr.table_bytes();
         g.parts = (float *)at;
+        mu_blocks(g);
         hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
         hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
         hipLaunchKernelGGL(mu_split_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
-        for (int s = 0; s < steps; ++s) {
-            g.step = s;
-            mu_launch_product<MU_GRAM>(g, st);
-            mu_launch_product<MU_POLY>(g, st);
-            if (s + 1 < steps) mu_launch_product<MU_APPLY>(g, st);
-            else mu_launch_product<MU_LAST>(g, st);
-            g.flip ^= 1;
-        }
+        mu_launcher launcher(g, st);
+        mu_walk(g.sizes, g.n_sizes, launcher);
         HIP_TRY(hipGetLastError());
         return LRB_OK;
     });

@@ -272,6 +272,28 @@ def test_orthogonalize_stacks(count, rows, cols):
     check_orthogonal(g.bfloat16())
 
 
+# long enough that several steps share one formation of X
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(700, 2100), (1500, 600), (513, 4000)])
+def test_orthogonalize_in_blocks_of_steps(rows, cols, kind):
+    gen = torch.Generator().manual_seed(8)
+    g = gradient_like(rows, cols, gen, "cuda").to(TYPES[kind])
+    n = min(rows, cols)
+    for steps in (1, 2, 3, 4, 5, 6, 7, 12):
+        check_orthogonal(g, steps=steps)
+        check_orthogonal(g, steps=steps, coefficients=(15 / 8, -10 / 8, 3 / 8))
+    check_orthogonal(g * 1e-12)
+    check_orthogonal(torch.randn(rows, cols, generator=gen).cuda().to(TYPES[kind]))
+    check_orthogonal((torch.randn(rows, 7, generator=gen) @ torch.randn(7, cols, generator=gen)).cuda().to(TYPES[kind]))
+    u, _, vt = torch.linalg.svd(torch.randn(rows, cols, generator=gen).cuda(), full_matrices=False)
+    check_orthogonal(((u * torch.logspace(0, -5, n, device="cuda")) @ vt).to(TYPES[kind]))
+    three = torch.stack([g, g, g])
+    three[1] = 0
+    got = check_orthogonal(three)
+    # (not the same bits in 0 and 2: which tiles of a launch are cut along k goes by their place in it)
+    assert not bool(got[1].any()) and torch.equal(got, train_ops.orthogonalize(three))
+
+
 @pytest.mark.parametrize("rows,cols", [(37, 90), (90, 37), (128, 168), (300, 200)])
 def test_orthogonalize_strides(rows, cols):
     g = gradient_like(rows, cols, torch.Generator().manual_seed(6), "cuda")
