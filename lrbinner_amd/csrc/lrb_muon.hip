@@ -1150,8 +1150,9 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
     return sum;
 }
 
-// The tile: the largest that still gives most of the 256 CUs one (a larger tile loads less for each product).  Both symmetric
-// products take the same (A in float32 is there on and above the diagonal's tiles only).
+// The tile: the largest that still fills most of the chip (a larger tile loads less for each product): 256 CUs take one each of
+// 256, two each of 128.  (Eight symmetric products of 1024: 288 tiles of 128, 52 us each, 1088 of 64, 47.)  All symmetric
+// products take the same (their float32 is there on and above the diagonal's tiles only).
 // The cut: a round of 256 tiles gives every CU one; the tiles that are left over behind the last whole round are cut along k so
 // that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 12 units of 64 k of the
 // smallest tile, one of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
@@ -1159,7 +1160,7 @@ static mu_plan mu_lay_out(const mu_args &a, int mode)
 {
     const bool symmetric = mode <= MU_SYM;
     mu_plan p;
-    p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 200 ? 128 : 64;
+    p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 400 ? 128 : 64;
     p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
     const long long rest = p.tiles % 256;
     p.direct = (int)p.tiles, p.splits = 1;
