@@ -369,9 +369,14 @@ class Muon(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                raise ValueError(f"Muon takes matrices, not a parameter of shape {tuple(p.shape)}")
+        try:
+            for p in self.param_groups[-1]["params"]:
+                _known_type(p, "params")
+                if p.dim() < 2:
+                    raise ValueError(f"Muon takes matrices, not a parameter of shape {tuple(p.shape)}")
+        except (TypeError, ValueError):
+            self.param_groups.pop()  # a refused group leaves the optimizer as it was
+            raise
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)  # casts the state to the parameters' type: the momentum stays float32

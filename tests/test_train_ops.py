@@ -184,6 +184,12 @@ def test_muon_optimizer(tmp_path):
         train_ops.Muon([torch.nn.Parameter(torch.zeros(4))])
     with pytest.raises(ValueError):
         train_ops.Muon([w], momentum=1.0)
+    with pytest.raises(TypeError):
+        train_ops.Muon([torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float64))])
+    live = train_ops.Muon([w])
+    with pytest.raises(ValueError):
+        live.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))]})
+    assert len(live.param_groups) == 1
 
 
 def test_c_entry_points_refuse_before_they_touch_a_device():
