@@ -22,6 +22,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <new>
 #include <vector>
 
@@ -1154,8 +1155,8 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
 // 256, two each of 128.  (Eight symmetric products of 1024: 288 tiles of 128, 52 us each, 1088 of 64, 47.)  All symmetric
 // products take the same (their float32 is there on and above the diagonal's tiles only).
 // The cut: a round of 256 tiles gives every CU one; the tiles that are left over behind the last whole round are cut along k so
-// that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 12 units of 64 k of the
-// smallest tile, one of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
+// that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 14 units of 64 k of the
+// smallest tile, five of the middle one, two of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
 static mu_plan mu_lay_out(const mu_args &a, int mode)
 {
     const bool symmetric = mode <= MU_SYM;
@@ -1437,36 +1438,39 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
     mu_walk(ones, steps, chain);
     try {
         return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
-        mu_args &g = gr.a;
-        g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
-        g.sx = sx;
-        memcpy(g.std, std, sizeof(std));
-        memcpy(g.sizes, ones, sizeof(ones));
-        g.n_sizes = steps;
-        if (gr.lds) {
-            static lrb_per_device_once raised;
-            if (raised.need(device)) {
-                HIP_TRY(hipFuncSetAttribute((const void *)mu_small_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MU_SMALL_LDS));
+            mu_args &g = gr.a;
+            g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
+            g.sx = sx;
+            memcpy(g.std, std, sizeof(std));
+            memcpy(g.sizes, ones, sizeof(ones));
+            g.n_sizes = steps;
+            if (gr.lds) {
+                // (a bit a device, set behind the call: a thread that finds it may launch)
+                static std::atomic<uint64_t> raised{0};
+                const uint64_t bit = device < 64 ? 1ull << device : 0;
+                if (!(raised.load(std::memory_order_acquire) & bit)) {
+                    HIP_TRY(hipFuncSetAttribute((const void *)mu_small_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MU_SMALL_LDS));
+                    raised.fetch_or(bit, std::memory_order_release);
+                }
+                hipLaunchKernelGGL(mu_small_kernel, dim3(gr.mats), dim3(64 * MU_SMALL_WAVES), gr.lds, st, g);
+                HIP_TRY(hipGetLastError());
+                return LRB_OK;
             }
-            hipLaunchKernelGGL(mu_small_kernel, dim3(gr.mats), dim3(64 * MU_SMALL_WAVES), gr.lds, st, g);
+            g.ws = (char *)d_ws;
+            char *at = g.ws + gr.planes;
+            g.x0 = (double *)at, at += gr.x0_bytes();
+            g.part = (double *)at, at += gr.sums_bytes();
+            g.table = (float *)at, at += gr.table_bytes();
+            g.parts = (float *)at;
+            mu_blocks(g);
+            hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
+            hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
+            hipLaunchKernelGGL(mu_split_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
+            mu_launcher launcher(g, st);
+            mu_walk(g.sizes, g.n_sizes, launcher);
             HIP_TRY(hipGetLastError());
             return LRB_OK;
-        }
-        g.ws = (char *)d_ws;
-        char *at = g.ws + gr.planes;
-        g.x0 = (double *)at, at += gr.x0_bytes();
-        g.part = (double *)at, at += gr.sums_bytes();
-        g.table = (float *)at, at += gr.table_bytes();
-        g.parts = (float *)at;
-        mu_blocks(g);
-        hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
-        hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
-        hipLaunchKernelGGL(mu_split_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
-        mu_launcher launcher(g, st);
-        mu_walk(g.sizes, g.n_sizes, launcher);
-        HIP_TRY(hipGetLastError());
-        return LRB_OK;
-    });
+        });
     } catch (const std::bad_alloc &) {
         lrb_set_error("out of memory%s%s", "", "");
         return LRB_ERR_NOMEM;
