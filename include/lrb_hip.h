@@ -547,7 +547,8 @@ int lrb_vae_debug_read(lrb_vae *v, int which, float *host, uint64_t count);
  *   y = (u - mean) / sqrt(var + eps) * w + b
  * x: rows x cols, the elements of a row side by side, rows x_stride elements apart; y: packed.  w, b: cols elements each or
  * NULL (1, 0), float32 or of x's type (w_type).  keep: rows x cols bytes, packed, or NULL.  d_mean, d_rstd: float32[rows],
- * what the backward pass needs, or both NULL.  Any number of rows and columns (below 2^29) from one on. */
+ * what the backward pass needs, or both NULL.  Any number of rows and columns (below 2^29) from one on.  What is written, here
+ * and in the backward pass, overlaps nothing else. */
 int lrb_layer_norm_fwd_dev(int device, void *stream, int x_type, int w_type, uint64_t rows, uint64_t cols, const void *d_x,
                            int64_t x_stride, const void *d_w, const void *d_b, float eps, float slope, const uint8_t *d_keep,
                            float keep_scale, void *d_y, float *d_mean, float *d_rstd);
@@ -565,8 +566,9 @@ int lrb_layer_norm_bwd_dev(int device, void *stream, int x_type, int w_type, uin
  *   m <- momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;  without m: u = g
  *   X = u / max(|u|_F, eps);  `steps` times X <- a X + (b A + c A^2) X, A = X X^T (X^T X of a tall matrix)
  *   p <- decay p + alpha X;  with decay = 0 p is not read
- * Strides are in elements, of (matrix, row, column), any values; p and m must not overlap each other, g, or another item's.
- * A matrix that holds an infinity or a NaN gives NaN throughout.  1 <= steps <= 32; a matrix below 2^31 elements with sides
+ * Strides are in elements, of (matrix, row, column), any values; p and m must not overlap each other, g (which p may be, with
+ * the same strides and type), or another item's.  A matrix that holds an infinity or a NaN gives NaN throughout, one of zeros
+ * X = 0.  1 <= steps <= 32; a matrix below 2^31 elements with sides
  * of at most 2^22.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
 typedef struct {
     void *p;

@@ -40,7 +40,7 @@ def _known_type(t, name):
 
 def _rows(t, cols):
     """t as rows x cols with the elements of a row side by side (a copy only where its strides allow no such view)."""
-    t = t.reshape(-1, cols)
+    t = t.resolve_neg().reshape(-1, cols)
     return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
 
 
@@ -49,7 +49,7 @@ def _address(t):
 
 
 def _packed(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
+    return t if t is None or t.is_contiguous() and not t.is_neg() else t.resolve_neg().contiguous()
 
 
 def _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, stats):
@@ -60,7 +60,7 @@ def _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, stats):
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
     if rows:
         stride = cols
-        if not x.is_contiguous():
+        if not x.is_contiguous() or x.is_neg():
             x = _rows(x, cols)
             stride = x.stride(0)
         weight, bias, keep = _packed(weight), _packed(bias), _packed(keep)
@@ -102,10 +102,10 @@ class _LayerNorm(torch.autograd.Function):
             ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(x_type, rows, cols)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
         x_stride = dy_stride = cols
-        if not x.is_contiguous():
+        if not x.is_contiguous() or x.is_neg():
             x = _rows(x, cols)
             x_stride = x.stride(0)
-        if not dy.is_contiguous():
+        if not dy.is_contiguous() or dy.is_neg():
             dy = _rows(dy, cols)
             dy_stride = dy.stride(0)
         weight, keep = _packed(weight), _packed(keep)
@@ -214,7 +214,14 @@ def _stack(t, name):
         raise ValueError(f"{name}: the leading axes of shape {tuple(t.shape)}, strides {t.stride()} are not evenly spaced") from None
 
 
+def _extent(t):
+    """The bytes from the first to behind the last element of t, which has some."""
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _written(t, name):
+    if t.is_neg():
+        raise ValueError(f"{name} is written, but it is a view with its sign turned")
     if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
         raise ValueError(f"{name} is written, but several of its elements share their memory (strides {t.stride()})")
 
@@ -226,7 +233,7 @@ def _check_iteration(steps, coefficients, eps):
         raise ValueError(f"coefficients: three finite numbers are wanted, not {coefficients}")
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps: {eps}")
-    if _lib.lib().lrb_muon_bound(int(steps), *coefficients) > _DIVERGED:
+    if not _lib.lib().lrb_muon_bound(int(steps), *coefficients) <= _DIVERGED:
         raise ValueError(f"coefficients {tuple(coefficients)}: a singular value may grow beyond {_DIVERGED:g} in {steps} steps")
 
 
@@ -246,7 +253,8 @@ def _orthogonal_plain(u, steps, coefficients, eps):
     x = u.float()
     turned = x.shape[-2] > x.shape[-1]
     x = x.transpose(-1, -2) if turned else x
-    x = x / torch.linalg.vector_norm(x, dim=(-2, -1), keepdim=True, dtype=torch.float64).clamp_min(eps).float()
+    norm = torch.linalg.vector_norm(x, dim=(-2, -1), keepdim=True, dtype=torch.float64).clamp_min(eps)
+    x = (x.double() / (norm + (norm == 0.0))).float()  # of float32's largest numbers the norm is beyond its range
     for _ in range(int(steps)):
         gram = x @ x.transpose(-1, -2)
         x = a * x + (b * gram + c * (gram @ gram)) @ x
@@ -255,12 +263,12 @@ def _orthogonal_plain(u, steps, coefficients, eps):
 
 @torch.no_grad()
 def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
-    """g / max(|g|_F, eps), then ``steps`` times X <- a X + (b A + c A^2) X with A = X X^T (of a tall matrix X^T X): the singular
-    vectors stay, the singular values go towards 1 (with the default coefficients into about 0.7 to 1.2).  Coefficients under which a singular
-    value from [0, 1] may grow beyond 64 on the way are refused.
+    """g / max(|g|_F, eps), then ``steps`` times X <- a X + (b A + c A^2) X with A = X X^T (of a tall matrix X^T X): the
+    singular vectors stay, the singular values go towards 1 (with the default coefficients into about 0.7 to 1.2).
+    Coefficients under which a singular value from [0, 1] may grow beyond 64 on the way are refused.
 
-    g: [..., rows, columns], any strides; each matrix by itself; one that holds an infinity or a NaN becomes NaN.
-    ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are as exact as
+    g: [..., rows, columns], any strides; each matrix by itself; one that holds an infinity or a NaN becomes NaN, one of
+    zeros stays.  ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are as exact as
     float32 ones for every type of g.  No gradient: an update is not differentiated."""
     _known_type(g, "g")
     if g.dim() < 2:
@@ -277,8 +285,13 @@ def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
             _stack(out, "out")
     if g.numel() == 0:
         return out
+    g = g.resolve_neg()
     if not g.is_cuda:
         return out.copy_(_orthogonal_plain(g, steps, coefficients, eps))
+    if out.data_ptr() != g.data_ptr() or out.stride() != g.stride() or out.dtype != g.dtype:
+        (g0, g1), (o0, o1) = _extent(g), _extent(out)
+        if g0 < o1 and o0 < g1:  # a matrix of out may lie over another matrix of g
+            g = g.clone()
     g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "g")
     o3 = _stack(out, "out")
     item = _ITEM.pack(o3.data_ptr(), g3.data_ptr(), 0, *o3.stride(), *g3.stride(), 0, 0, 0, *g3.shape,
@@ -298,8 +311,9 @@ def muon_step(params, grads, momenta=None, *, lr, momentum=0.95, nesterov=True, 
 
     params, grads, momenta: lists of [..., rows, columns] of one device, each of its own type and strides (momenta best in
     float32); leading axes are a stack of weights.  ``scale``: None for sqrt(max(1, rows / columns)), or a number.  The
-    weights of a list share their launches, so one call for all of a network's is best.  No two written tensors may overlap."""
-    params, grads = list(params), list(grads)
+    weights of a list share their launches, so one call for all of a network's is best.  No written tensor may overlap
+    another tensor of the call."""
+    params, grads = list(params), [g.resolve_neg() for g in grads]
     momenta = [None] * len(params) if momenta is None else list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(momenta)} momenta")

@@ -575,3 +575,65 @@ def test_a_run_after_a_fused_one_encodes_with_its_own_weights():
     vae.eval()
     with torch.no_grad():
         assert float((vae._encode(data)[0].cpu() - torch.from_numpy(mu)).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("shape", [(9, 32, 48), (5, 300, 200)])
+def test_out_that_lies_over_other_matrices(shape):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    for take in (lambda b: (b[:-1], b[1:]), lambda b: (b[1:], b[:-1]), lambda b: (b, b.flip(0)), lambda b: (b, b)):
+        buf = torch.randn(*shape, device="cuda", generator=gen)
+        g, out = take(buf)
+        want = train_ops.orthogonalize(g.clone())
+        assert torch.equal(train_ops.orthogonalize(g, out=out), want)
+    buf = torch.randn(shape[0], shape[0], 40, 24, device="cuda", generator=gen)  # a view that takes the stacks' axes in turn
+    want = train_ops.orthogonalize(buf[0].clone())
+    assert torch.equal(train_ops.orthogonalize(buf[0], out=buf[:, 0]), want)
+
+
+def test_views_with_their_sign_turned():
+    x, w, b, dy, _ = inputs(20, 33, torch.float32)
+    turned = torch._neg_view(x.t().contiguous()).t()
+    assert torch.equal(train_ops.layer_norm(turned, w, b), train_ops.layer_norm(-x, w, b))
+    assert torch.equal(train_ops.layer_norm(torch._neg_view(x), w, b), train_ops.layer_norm(-x, w, b))
+    assert torch.equal(train_ops.orthogonalize(torch._neg_view(x)), train_ops.orthogonalize(-x))
+
+
+def test_inside_inference_mode():
+    x, w, b, _, _ = inputs(20, 33, torch.float32)
+    want, moved = train_ops.layer_norm(x, w, b), x.clone()
+    turned = train_ops.orthogonalize(x)
+    train_ops.muon_step([moved], [x], lr=0.1)
+    with torch.inference_mode():
+        assert torch.equal(train_ops.layer_norm(x, w, b), want) and torch.equal(train_ops.orthogonalize(x), turned)
+        again = x.clone()
+        train_ops.muon_step([again], [x], lr=0.1)
+        assert torch.equal(again, moved)
+
+
+def test_threads_on_streams_of_their_own():
+    import threading
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    gs = [torch.randn(*s, device="cuda", generator=gen) for s in ((100, 150), (300, 200), (64, 64), (700, 520))]
+    want = [train_ops.orthogonalize(g) for g in gs]
+    got, failed = [None] * len(gs), []
+    torch.cuda.synchronize()
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    out = train_ops.orthogonalize(gs[k])
+                torch.cuda.current_stream().synchronize()
+                got[k] = out
+        except Exception as e:  # an assertion of a thread is not seen
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(gs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)

@@ -278,3 +278,23 @@ def test_vae_encode_takes_the_choices_from_the_environment(tmp_path, monkeypatch
     monkeypatch.setenv("LRB_VAE_OPTIMIZER", "none")
     with pytest.raises(ValueError, match="optimizer"):
         ae_utils.vae_encode(str(tmp_path), 3, [8, 8], 2, None, False)
+
+
+def test_orthogonalize_at_the_ends_of_the_range():
+    g = gradient_like(8, 12, torch.Generator().manual_seed(1))
+    huge = g / g.abs().max() * 3e38  # its norm is beyond float32
+    exact = orthogonal_ref(huge, 3, (1.5, -0.5, 0.0), 1e-7)
+    matrices_within(train_ops.orthogonalize(huge, 3, (1.5, -0.5, 0.0)), exact, orthogonal_tolerance(exact, huge, 3, (1.5, -0.5, 0.0), 1e-7))
+    assert not train_ops.orthogonalize(torch.zeros(3, 4), eps=0.0).any()
+    with pytest.raises(ValueError):
+        train_ops.orthogonalize(g, coefficients=(1e39, 0.0, 0.0))  # finite, but not in float32
+
+
+def test_views_with_their_sign_turned():
+    g = gradient_like(6, 9, torch.Generator().manual_seed(2))
+    turned = torch._neg_view(g)
+    assert turned.is_neg() and torch.equal(train_ops.orthogonalize(turned), train_ops.orthogonalize(-g))
+    with pytest.raises(ValueError):
+        train_ops.orthogonalize(g, out=torch._neg_view(torch.zeros(6, 9)))
+    with pytest.raises(ValueError):
+        train_ops.muon_step([torch._neg_view(torch.zeros(6, 9))], [g], lr=0.1)
