@@ -53,6 +53,14 @@ struct mu_item {
     float alpha, decay;
 };
 
+// An operation of the iteration: its number, its factors for a norm of at least eps, and the n x n buffers it reads and writes
+// (see mu_strip).  keep: the result in float32 too.
+struct mu_job {
+    int op;
+    float k[MU_COEF];
+    int u, v, old, old2, out, keep;
+};
+
 struct mu_args {
     char *ws;
     double *x0;     // [matrices][2] what u is multiplied by; 1 if the launch's own factors hold, 0 for those of the table
@@ -62,10 +70,9 @@ struct mu_args {
     float beta, eps, a, b, c;
     int nesterov;
     int flip;       // which of the two copies of X is read
-    // the operation: its number, its factors for a norm of at least eps, and the n x n buffers it reads and writes (see mu_strip)
-    int op;
-    float k[MU_COEF];
-    int u, v, old, old2, out, keep; // keep: the result in float32 too
+    int exact;      // the matrices are kept in float32 too
+    int jobs;       // operations of this launch: two symmetric products that do not need each other's results, or one
+    mu_job job[2];
     int n_sizes;                     // the iteration's blocks
     uint8_t sizes[MU_STEPS];
     // of a product's launch: the tiles from `direct` on are cut along k, `splits` workgroups each, whose sums go to `parts`
@@ -448,7 +455,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = tile[row][c + q];
         mu_split8(v, hi, lo);
-        __builtin_memcpy(w.x32 + (size_t)(i0 + row) * it.lp + j0 + c, v, 32);
+        if (a.exact) __builtin_memcpy(w.x32 + (size_t)(i0 + row) * it.lp + j0 + c, v, 32);
         *(mu_h8 *)(w.x + at) = hi;
         *(mu_h8 *)(w.x + at + 32) = lo;
 #pragma unroll
@@ -512,23 +519,32 @@ __device__ __forceinline__ void mu_update4(const mu_item &it, long long at, long
 struct mu_factors {
     float k0, k1, k2;
     // (asked for before the products, so that the results do not wait for it)
-    __device__ __forceinline__ mu_factors(const mu_args &a, int matrix) : k0(a.k[0]), k1(a.k[1]), k2(a.k[2])
+    __device__ __forceinline__ mu_factors(const mu_args &a, const mu_job &job, int matrix) : k0(job.k[0]), k1(job.k[1]), k2(job.k[2])
     {
         if (a.x0[2 * matrix + 1] == 0.0) {
-            const float *t = a.table + ((size_t)matrix * MU_OPS + a.op) * MU_COEF;
+            const float *t = a.table + ((size_t)matrix * MU_OPS + job.op) * MU_COEF;
             k0 = t[0], k1 = t[1], k2 = t[2];
         }
     }
 };
 template <int MODE, int NI>
-__device__ __forceinline__ void mu_strip(const mu_args &a, const mu_factors &f, const mu_item &it, int mat, const mu_mat &w, const mu_f16 (&acc)[NI], int i0, int j0,
-                                         bool mirror, float *lds, int lane)
+__device__ __forceinline__ void mu_strip(const mu_args &a, const mu_job &job, const mu_factors &f, const mu_item &it, int mat, const mu_mat &w,
+                                         const mu_f16 (&acc)[NI], int i0, int j0, bool mirror, float *lds, int lane)
 {
     constexpr int PITCH = MU_PITCH(NI), LANES = 8 * NI, ROWS = 64 / LANES; // lanes of a row, rows of a turn
     const int ld = MODE >= MU_APPLY ? it.lp : it.np;
-    const float *old = MODE >= MU_APPLY ? w.x32 : a.old >= 0 ? w.full(a.old) : nullptr, *old2 = MODE == MU_SYM && a.old2 >= 0 ? w.full(a.old2) : nullptr;
-    float *full = MODE == MU_APPLY ? w.x32 : MODE <= MU_SYM ? w.full(a.out) : nullptr;
-    mu_h *out = MODE == MU_APPLY ? w.x2 : w.half(a.out), *out_t = MODE == MU_APPLY ? w.xt2 : out;
+    const bool exact = a.exact, keep = exact && (MODE != MU_SYM || job.keep);
+    const bool has_old = MODE >= MU_APPLY || job.old >= 0, has_old2 = MODE == MU_SYM && job.old2 >= 0;
+    // the old entries in float32, or, where nothing is kept in float32, their halves
+    const float *old = MODE >= MU_APPLY ? w.x32 : w.full(job.old), *old2 = w.full(job.old2);
+    const mu_h *old_h = MODE >= MU_APPLY ? w.x : w.half(job.old), *old2_h = w.half(job.old2);
+    auto read_old = [=](const float *full, const mu_h *half, int i, int j) {
+        if (exact) return *(const float4 *)(full + (size_t)i * ld + j);
+        const mu_h4 hi = *(const mu_h4 *)(half + mu_at(i, j, ld)), lo = *(const mu_h4 *)(half + mu_at(i, j, ld) + 32);
+        return make_float4((float)hi[0] + (float)lo[0], (float)hi[1] + (float)lo[1], (float)hi[2] + (float)lo[2], (float)hi[3] + (float)lo[3]);
+    };
+    float *full = MODE == MU_APPLY ? w.x32 : w.full(job.out);
+    mu_h *out = MODE == MU_APPLY ? w.x2 : w.half(job.out), *out_t = MODE == MU_APPLY ? w.xt2 : out;
     const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1; // which way p is written
     mu_wave_sync();
 #pragma unroll
@@ -544,11 +560,10 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_factors &f, 
         const int c = (lane % LANES) * 4, i = i0 + r, j = j0 + c;
         if (i >= it.np || j >= ld) continue;
         float4 v = *(const float4 *)(lds + r * PITCH + c);
-        const size_t at = (size_t)i * ld + j;
-        const float4 o = MODE >= MU_APPLY || old ? *(const float4 *)(old + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float4 o = has_old ? read_old(old, old_h, i, j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         v = make_float4(f.k0 * o.x + f.k1 * v.x, f.k0 * o.y + f.k1 * v.y, f.k0 * o.z + f.k1 * v.z, f.k0 * o.w + f.k1 * v.w);
-        if (MODE == MU_SYM && old2) {
-            const float4 o2 = *(const float4 *)(old2 + at);
+        if (has_old2) {
+            const float4 o2 = read_old(old2, old2_h, i, j);
             v.x += f.k2 * o2.x, v.y += f.k2 * o2.y, v.z += f.k2 * o2.z, v.w += f.k2 * o2.w;
         }
         if (back) *(float4 *)(lds + r * PITCH + c) = v;
@@ -557,7 +572,7 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_factors &f, 
         } else {
             mu_h4 hi, lo;
             mu_split4(v.x, v.y, v.z, v.w, hi, lo);
-            if (MODE != MU_SYM || a.keep) *(float4 *)(full + at) = v;
+            if (keep) *(float4 *)(full + (size_t)i * ld + j) = v;
             *(mu_h4 *)(out + mu_at(i, j, ld)) = hi;
             *(mu_h4 *)(out + mu_at(i, j, ld) + 32) = lo;
         }
@@ -661,14 +676,17 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     }
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
-    const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
+    const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k];
+    const bool two = MODE == MU_SYM && a.jobs > 1; // both operations of a matrix side by side
+    const int mat = two ? local / per >> 1 : local / per;
+    const mu_job &job = a.job[two ? local / per & 1 : 0];
     int i0, j0;
     mu_place<MODE>(local % per, ti, tj, i0, j0);
     i0 *= T, j0 *= T;
     const mu_mat w = mu_planes(a, it, mat);
-    const mu_factors factors(a, it.first + mat);
+    const mu_factors factors(a, job, it.first + mat);
     const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
-    const mu_h *P = MODE == MU_GRAM ? w.x : w.half(a.u), *Q = MODE == MU_GRAM ? w.x : MODE == MU_SYM ? w.half(a.v) : w.xt;
+    const mu_h *P = MODE == MU_GRAM ? w.x : w.half(job.u), *Q = MODE == MU_GRAM ? w.x : MODE == MU_SYM ? w.half(job.v) : w.xt;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN, wj = wave % WN;
 
     // A load of a wave fills eight rows of a stage.  All addresses are a factor's first row of the tile (uniform) and an offset of
@@ -815,7 +833,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const bool mirror = MODE == MU_APPLY || i0 != j0;
 #pragma unroll
     for (int x = 0; x < MI; ++x)
-        mu_strip<MODE, NI>(a, factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane);
+        mu_strip<MODE, NI>(a, job, factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane);
 }
 
 // The tiles that were cut along k: their parts' sums, added up in order, a wave for each 32 rows of one of the tile's waves.
@@ -827,7 +845,10 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
     const int tile = a.direct + r, k = mu_find(a, tile);
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
-    const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k], mat = local / per;
+    const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k];
+    const bool two = MODE == MU_SYM && a.jobs > 1; // both operations of a matrix side by side
+    const int mat = two ? local / per >> 1 : local / per;
+    const mu_job &job = a.job[two ? local / per & 1 : 0];
     int i0, j0;
     mu_place<MODE>(local % per, ti, tj, i0, j0);
     i0 *= T, j0 *= T;
@@ -848,8 +869,8 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
                 acc[y][4 * q] += v.x, acc[y][4 * q + 1] += v.y, acc[y][4 * q + 2] += v.z, acc[y][4 * q + 3] += v.w;
             }
     const mu_mat w = mu_planes(a, it, mat);
-    const mu_factors factors(a, it.first + mat);
-    mu_strip<MODE, NI>(a, factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
+    const mu_factors factors(a, job, it.first + mat);
+    mu_strip<MODE, NI>(a, job, factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
 }
 
 // A matrix that fits one workgroup's LDS (128 x 208, 96 x 320, 64 x 512, 32 x 1,024 and less) goes through all its steps there, in one
@@ -1139,13 +1160,13 @@ struct mu_plan {
     uint64_t part_bytes() const { return splits > 1 ? (uint64_t)(tiles - direct) * splits * T * T * 4 : 0; }
 };
 
-static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
+static long long mu_tiles(const mu_args &a, bool symmetric, int jobs, int T, int *start)
 {
     long long sum = 0;
     for (int k = 0; k < a.n_items; ++k) {
         if (start) start[k] = (int)sum;
         const long long ti = (a.it[k].np + T - 1) / T, tj = (a.it[k].lp + T - 1) / T;
-        sum += a.it[k].count * (symmetric ? ti * (ti + 1) / 2 : ti * tj);
+        sum += a.it[k].count * (symmetric ? jobs * (ti * (ti + 1) / 2) : ti * tj);
     }
     if (start) start[a.n_items] = (int)sum;
     return sum;
@@ -1157,12 +1178,13 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
 // The cut: a round of 256 tiles gives every CU one; the tiles that are left over behind the last whole round are cut along k so
 // that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 14 units of 64 k of the
 // smallest tile, five of the middle one, two of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
-static mu_plan mu_lay_out(const mu_args &a, int mode)
+static mu_plan mu_lay_out(const mu_args &a, int mode, int jobs, bool exact)
 {
     const bool symmetric = mode <= MU_SYM;
+    const int counted = exact ? 1 : jobs;
     mu_plan p;
-    p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 400 ? 128 : 64;
-    p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
+    p.T = mu_tiles(a, symmetric, counted, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, counted, 128, nullptr) >= 400 ? 128 : 64;
+    p.tiles = mu_tiles(a, symmetric, jobs, p.T, nullptr);
     const long long rest = p.tiles % 256;
     p.direct = (int)p.tiles, p.splits = 1;
     if (rest == 0) return p;
@@ -1170,7 +1192,7 @@ static mu_plan mu_lay_out(const mu_args &a, int mode)
     long long before = 0;
     for (int k = 0; k < a.n_items; ++k) {
         const long long ti = (a.it[k].np + p.T - 1) / p.T, tj = (a.it[k].lp + p.T - 1) / p.T;
-        before += a.it[k].count * (symmetric ? ti * (ti + 1) / 2 : ti * tj);
+        before += a.it[k].count * (symmetric ? jobs * (ti * (ti + 1) / 2) : ti * tj);
         const long long u = (mode == MU_GRAM ? a.it[k].lp : a.it[k].np) / 64;
         if (before > p.tiles - rest && u < units) units = u;
     }
@@ -1195,11 +1217,11 @@ template <int T, int WM, int WN, int MODE> static void mu_launch_tiles(const mu_
 
 template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
 {
-    const mu_plan p = mu_lay_out(a, MODE);
-    mu_tiles(a, MODE <= MU_SYM, p.T, a.start);
+    const mu_plan p = mu_lay_out(a, MODE, a.jobs, a.exact);
+    mu_tiles(a, MODE <= MU_SYM, a.jobs, p.T, a.start);
     a.direct = p.direct, a.splits = p.splits;
     if (p.T == 256) mu_launch_tiles<256, 2, 4, MODE>(a, p, st);
-    else if (p.T == 128) mu_launch_tiles<128, 2, 2, MODE>(a, p, st);
+    else if (p.T == 128) mu_launch_tiles<128, 2, 4, MODE>(a, p, st);
     else mu_launch_tiles<64, 2, 2, MODE>(a, p, st);
 }
 
@@ -1224,11 +1246,13 @@ static void mu_blocks(mu_args &g)
         exact |= it.p_type == LRB_F32;
         most = most < n ? most : n;
     }
+    g.exact = 1;
     if (wide < 1.3 * square || wide < 5e8) return;
+    g.exact = exact;
     int left = g.steps;
     g.n_sizes = 0;
     while (left > 0) {
-        const int n = exact ? (g.n_sizes == 0 ? 2 : 1) : most;
+        const int n = g.exact ? (g.n_sizes == 0 ? 2 : 1) : most;
         g.sizes[g.n_sizes++] = (uint8_t)(n < left ? n : left);
         left -= n;
     }
@@ -1240,21 +1264,27 @@ struct mu_launcher {
     hipStream_t st;
     mu_chain chain;
     float factors[MU_OPS * MU_COEF];
-    int op = 0, A = 0, P = 1, S = 1, C = 2;
+    int op = 0, A = 0, P = 1, S = 1, C = 2, was = 1; // was: the buffer of the sum before, which a sum of the same launch reads
     mu_launcher(mu_args &args, hipStream_t stream) : g(args), st(stream), chain(g.a, g.b, g.c, 1.0, factors) { mu_walk(g.sizes, g.n_sizes, chain); }
     mu_launcher(const mu_launcher &) = delete;
-    int unused(int x, int y, int z) const // the least buffer that is none of these
+    int unused(int x, int y, int z, int w) const // the least buffer that is none of these
     {
         int b = 0;
-        while (b == x || b == y || b == z) ++b;
+        while (b == x || b == y || b == z || b == w) ++b;
         return b;
     }
     template <int MODE> void launch(int u, int v, int old, int old2, int out, bool keep = true)
     {
-        g.op = op;
-        memcpy(g.k, factors + op++ * MU_COEF, sizeof(g.k));
-        g.u = u, g.v = v, g.old = old, g.old2 = old2, g.out = out, g.keep = keep;
+        add(u, v, old, old2, out, keep);
         mu_launch_product<MODE>(g, st);
+        g.jobs = 0;
+    }
+    void add(int u, int v, int old, int old2, int out, bool keep) // one more operation of the next launch
+    {
+        mu_job &j = g.job[g.jobs++];
+        j.op = op;
+        memcpy(j.k, factors + op++ * MU_COEF, sizeof(j.k));
+        j.u = u, j.v = v, j.old = old, j.old2 = old2, j.out = out, j.keep = keep;
     }
     void gram()
     {
@@ -1263,19 +1293,20 @@ struct mu_launcher {
     }
     void poly(int k, int n)
     {
-        P = k ? unused(A, S, A) : 1;
+        P = k ? unused(A, S, S, S) : 1;
         launch<MU_SYM>(A, A, A, -1, P, n > 1); // of a single step's it is a factor only
-        if (k == 0) S = P;
+        if (k == 0) S = was = P;
     }
     void sum(int k, int n)
     {
-        const int to = unused(A, P, S);
-        launch<MU_SYM>(P, S, S, P, to, k + 1 < n);
-        S = to;
+        const int to = unused(A, P, S, S);
+        if (k + 1 < n) add(P, S, S, P, to, true); // with the turn that follows
+        else launch<MU_SYM>(P, S, S, P, to, false);
+        was = S, S = to;
     }
     void turn()
     {
-        C = unused(A, P, S);
+        C = unused(A, P, S, was);
         launch<MU_SYM>(P, A, A, -1, C);
     }
     void turn2() { launch<MU_SYM>(C, P, C, -1, A); }
@@ -1288,7 +1319,7 @@ struct mu_launcher {
 };
 
 // A run of items (or of some matrices of one) that fits the descriptors and MU_WS_MOST bytes, and what it takes.
-#define MU_BUFFERS 4 // n x n, of each matrix
+#define MU_BUFFERS 5 // n x n, of each matrix
 #define MU_WS_MOST (4ull << 30)
 #define MU_MATS_MOST 4096
 struct mu_group {
@@ -1305,10 +1336,11 @@ struct mu_group {
     {
         if (lds) return 0;
         uint64_t parts = 0;
-        for (int mode = MU_GRAM; mode <= MU_LAST; ++mode) {
-            const uint64_t b = mu_lay_out(a, mode).part_bytes();
-            parts = b > parts ? b : parts;
-        }
+        for (int mode = MU_GRAM; mode <= MU_LAST; ++mode)
+            for (int jobs = 1; jobs <= (mode == MU_SYM ? 2 : 1); ++jobs) {
+                const uint64_t b = mu_lay_out(a, mode, jobs, false).part_bytes(), e = mu_lay_out(a, mode, jobs, true).part_bytes();
+                parts = b > parts ? b : parts, parts = e > parts ? e : parts;
+            }
         return planes + parts + x0_bytes() + sums_bytes() + table_bytes();
     }
 };
