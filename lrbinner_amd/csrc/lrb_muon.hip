@@ -17,6 +17,12 @@
 // All products are of the form C[i][j] = sum_k P[i][k] Q[j][k] with k contiguous in both: A = X X^T and A^2 = A A^T as they
 // stand, B X from X's transpose, which the epilogue writes beside X.  One workgroup a T x T tile of C; of the symmetric
 // products the tiles on and above the diagonal are computed and mirrored.  Tiles of all weights of a call share a launch.
+// Where X is longer than wide several steps share one formation of X (mu_walk); a matrix that fits one workgroup's LDS goes
+// through all steps in one launch (mu_small_kernel).
+// Measured, where a library product of 8192 x 8192 float16 reaches 1.09 PFLOP/s: a 4096 x 4096 float32 weight 3.9 ms = 1.05
+// PFLOP/s of its three products (B X alone 1.17); a layer's four weights (2048 x 2048 twice, 5461 x 2048, 2048 x 5461,
+// bfloat16) 2.96 ms, of them 0.15 for the momentum and the splitting, at 4.6 and 5.3 TB/s; 8 x 1024 x 2048 0.98 ms;
+// 1025 x 511 175 us (26 launches that wait for each other); 128 x 168 50 us.
 #include <limits.h>
 #include <math.h>
 #include <string.h>
@@ -85,11 +91,12 @@ struct mu_args {
 };
 static_assert(sizeof(mu_args) <= 4096, "kernel arguments");
 
-// A matrix in the workspace: X and its transpose twice (read and written in turn), and four n x n buffers for A, B and what
+// A matrix in the workspace: X and its transpose twice (read and written in turn), and five n x n buffers for A, B and what
 // is made of them, as rows of 32 hi, the 32 lo of the same entries, the next 32 hi ...: 32 k of a row are one whole line of 128
 // bytes, which halves the requests that the L2 gets for a stage against separate planes of hi and lo (4096 x 4096, B X: 43 M ->
 // 21 M).  And X and the buffers in float32, for the terms that are not products (a X, b A ...): hi + lo is a rounding more than
 // float32 is, and these terms would pass it on.  Of symmetric matrices the float32 is there on and above the diagonal's tiles.
+// Blocks of steps whose results are all 16-bit (mu_blocks) do without it.
 __host__ __device__ inline unsigned long long mu_plane_x(const mu_item &it) { return 4ull * (unsigned long long)it.np * it.lp; }
 __host__ __device__ inline unsigned long long mu_plane_a(const mu_item &it) { return 4ull * (unsigned long long)it.np * it.np; }
 __host__ __device__ inline unsigned long long mu_bytes(const mu_item &it, int buffers) { return 5 * mu_plane_x(it) + 2 * buffers * mu_plane_a(it); }
@@ -271,6 +278,7 @@ __host__ __device__ double mu_scale(double r) // the power of two that takes ent
 //   turn()       k + 1 < n: C = a A + P A             (all of these are polynomials of the same A: they commute, and the
 //   turn2()                 A <- a C + C P             products are symmetric)
 //   apply(n)     X <- a^n X + S X
+// sum(k) and the turn() behind it share a launch: neither needs the other's result.
 // A block of one step is the iteration as it is written.  A longer one forms X and X X^T once for its n steps, and pays with
 // four symmetric n x n products a step more: for X of n x r n entries 1.5 r + 4.5 units of 2 n^3 for three steps against
 // 4.5 r + 1.5.
@@ -641,7 +649,12 @@ __host__ __device__ inline int mu_by_xcd(int xcd, int rank, int n)
 
 // One tile of a product.  LDS holds two stages of 32 k: T rows of P and T of Q, 128 bytes each; the eight 16-byte chunks of a
 // row (four of hi, four of lo) lie at chunk ^ ((row >> 1) & 7), which spreads the 16 rows that a quarter wave reads over all
-// 64 banks.  The loads go from global memory to LDS directly, one stage ahead of the products.
+// 64 banks.  The loads go from global memory to LDS directly, one stage ahead of the products (three for the smallest tile).
+// Bound: the matrix cores for the 256-tile (B X of 4096 x 4096: 352 us = 1.17 PFLOP/s; the chip lowers its clock under this
+// load: on zeros the whole call takes 2.9 ms, on numbers 3.9).  The 128-tile reaches 0.95 (four symmetric products of 2048: 115
+// us): it reads LDS twice as often for a product and has its loads only one shorter stage ahead.  Eight waves of 64 x 32 hide that better
+// than four of 64 x 64 (a layer's four weights 3.10 against 3.19 ms; two of 128 x 64: 3.38; eight with four stages: 3.27).  The
+// 64-tile is bound by its loads (eight symmetric products of 1024: 47 us).
 template <int T, int WM, int WN, int MODE>
 __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 {
@@ -1173,11 +1186,13 @@ static long long mu_tiles(const mu_args &a, bool symmetric, int jobs, int T, int
 }
 
 // The tile: the largest that still fills most of the chip (a larger tile loads less for each product): 256 CUs take one each of
-// 256, two each of 128.  (Eight symmetric products of 1024: 288 tiles of 128, 52 us each, 1088 of 64, 47.)  All symmetric
-// products take the same (their float32 is there on and above the diagonal's tiles only).
+// 256, two each of 128.  (Eight symmetric products of 1024: 288 tiles of 128 and 1088 of 64 both take 47 us; 576 tiles
+// of 128, two such products in a launch, 68.)  All symmetric products of a group that is kept in float32 take the same (it is
+// there on and above the diagonal's tiles only).
 // The cut: a round of 256 tiles gives every CU one; the tiles that are left over behind the last whole round are cut along k so
 // that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 14 units of 64 k of the
-// smallest tile, five of the middle one, two of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 + 12 with the last 16 cut.
+// smallest tile, five of the middle one, two of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 +
+// 12 with the last 16 cut (193 + 9 since a tile has eight waves).
 static mu_plan mu_lay_out(const mu_args &a, int mode, int jobs, bool exact)
 {
     const bool symmetric = mode <= MU_SYM;
@@ -1232,6 +1247,9 @@ template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
 // which has to stay below half a step of the result (5 steps for bfloat16: measured 2e-4 at the worst, of 1.7e-3 that the rounding
 // of the result makes; 4 for float16).  Float32 takes two steps at the beginning, where that is measured to lose nothing
 // (1.6e-6 against 1.6e-6, 2.1e-6 against 2.1e-6), and single ones from there on (two blocks of two: 1.2 to 2 times the error).
+// Where all results are 16-bit the matrices of such blocks are kept as halves only (2^-22 of an entry, far below the result's
+// rounding; 8 x 1024 x 2048, with the shared launches: 1.07 -> 1.00 ms).  Single steps keep float32: what they give is the
+// float32 result, rounded.
 static void mu_blocks(mu_args &g)
 {
     double square = 0.0, wide = 0.0;

@@ -36,15 +36,14 @@ struct ln_args {
     float eps, slope, keep_scale;
 };
 
-// A thread's V elements from column `col` on.  Rows need only their element's alignment: global loads of this target take any
-// address.  Where a row ends inside the V, the thread takes the row's last V instead: it then computes some elements that
+// A thread's V elements from column `col` on.  Rows need only their element's alignment: global loads of this target take
+// any address.  Where a row ends inside the V, the thread takes the row's last V instead: it then computes some elements that
 // its neighbour computes too, from the same operands in the same order, and both store the same bits; only what is summed
 // over the row has to leave them out (ln_chunk::own).  So no load or store is made element by element, which for rows of
-// 4095 16-bit elements cost as much as the rest (a forward pass over 8191 of them 48 us, so 26).  Rows of fewer than V columns (LN_TINY) go
-// element by element.
-// Rows of a multiple of V columns (LN_EVEN) have no such thread and are spared the selections (32,768 x 4096 bfloat16 forward: 97 us,
-// with them 114).  A thread whose columns all lie
-// past the end reads the row's last V too and stores nothing: with a branch between the loads of a row the same pass takes 129.
+// 4095 16-bit elements cost as much as the rest (a forward pass over 8191 of them: 48 us, so 27).  Rows of fewer than V
+// columns (LN_TINY) go element by element.  Rows of a multiple of V columns (LN_EVEN) have no such thread and are spared the
+// selections (32,768 x 4096 bfloat16 forward: 97 us, with them 114).  A thread whose columns all lie past the end reads the
+// row's last V too and stores nothing: with a branch between the loads of a row the same pass takes 129 us.
 enum { LN_EVEN = 0, LN_ODD = 1, LN_TINY = 2 };
 struct ln_chunk {
     int at, first;  // the first column; the first of the V elements that no neighbour has (V: none)

@@ -268,8 +268,8 @@ def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     Coefficients under which a singular value from [0, 1] may grow beyond 64 on the way are refused.
 
     g: [..., rows, columns], any strides; each matrix by itself; one that holds an infinity or a NaN becomes NaN, one of
-    zeros stays.  ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are as exact as
-    float32 ones for every type of g.  No gradient: an update is not differentiated."""
+    zeros stays.  ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are
+    as exact as float32 ones for every type of g.  No gradient: an update is not differentiated."""
     _known_type(g, "g")
     if g.dim() < 2:
         raise ValueError(f"g: a matrix is wanted, not shape {tuple(g.shape)}")
