@@ -652,9 +652,9 @@ __host__ __device__ inline int mu_by_xcd(int xcd, int rank, int n)
 // 64 banks.  The loads go from global memory to LDS directly, one stage ahead of the products (three for the smallest tile).
 // Bound: the matrix cores for the 256-tile (B X of 4096 x 4096: 352 us = 1.17 PFLOP/s; the chip lowers its clock under this
 // load: on zeros the whole call takes 2.9 ms, on numbers 3.9).  The 128-tile reaches 0.95 (four symmetric products of 2048: 115
-// us): it reads LDS twice as often for a product and has its loads only one shorter stage ahead.  Eight waves of 64 x 32 hide that better
-// than four of 64 x 64 (a layer's four weights 3.10 against 3.19 ms; two of 128 x 64: 3.38; eight with four stages: 3.27).  The
-// 64-tile is bound by its loads (eight symmetric products of 1024: 47 us).
+// us): it reads LDS twice as often for a product and has its loads only one shorter stage ahead.  Eight waves of 64 x 32 hide
+// that better than four of 64 x 64 (a layer's four weights 3.10 against 3.19 ms; two of 128 x 64: 3.38; eight with four stages:
+// 3.27).  The 64-tile is bound by its loads (eight symmetric products of 1024: 47 us).
 template <int T, int WM, int WN, int MODE>
 __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 {
