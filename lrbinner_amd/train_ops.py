@@ -75,6 +75,43 @@ def _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, stats):
     return y, stats
 
 
+def _ln_backward(ctx, dy):
+    x, weight, keep, stats = ctx.saved_tensors
+    bias_type, slope, keep_scale = ctx.more
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    w_type = weight.dtype if weight is not None else bias_type
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+    dw = torch.empty(cols, dtype=w_type, device=x.device) if need_w else None
+    db = torch.empty(cols, dtype=w_type, device=x.device) if need_b else None
+    lib = _lib.lib()
+    x_type = _TYPES[x.dtype]
+    ws, ws_bytes = None, 0
+    if need_w or need_b:
+        ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(x_type, rows, cols)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    x_stride = dy_stride = cols
+    if not x.is_contiguous() or x.is_neg():
+        x = _rows(x, cols)
+        x_stride = x.stride(0)
+    if not dy.is_contiguous() or dy.is_neg():
+        dy = _rows(dy, cols)
+        dy_stride = dy.stride(0)
+    weight, keep = _packed(weight), _packed(keep)
+    index, at = x.device.index, stats.data_ptr() or None
+    rc = lib.lrb_layer_norm_bwd_dev(
+        index, _stream(index), x_type, 0 if w_type is None else _TYPES[w_type], rows, cols, x.data_ptr() or None, x_stride,
+        dy.data_ptr() or None, dy_stride, _address(weight), at, at and at + 4 * rows, slope, _address(keep) or None, keep_scale,
+        _address(dx) or None, _address(dw), _address(db), _address(ws), ws_bytes)
+    if rc:
+        check("lrb_layer_norm_bwd_dev", rc)
+    return dx, dw, db, None, None, None, None
+
+
+_ln_backward_of_a_graph = once_differentiable(_ln_backward)  # refuses a second derivative
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, keep, eps, slope, keep_scale):
@@ -84,39 +121,10 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, keep, stats = ctx.saved_tensors
-        bias_type, slope, keep_scale = ctx.more
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        cols = x.shape[-1]
-        rows = x.numel() // cols
-        w_type = weight.dtype if weight is not None else bias_type
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-        dw = torch.empty(cols, dtype=w_type, device=x.device) if need_w else None
-        db = torch.empty(cols, dtype=w_type, device=x.device) if need_b else None
-        lib = _lib.lib()
-        x_type = _TYPES[x.dtype]
-        ws, ws_bytes = None, 0
-        if need_w or need_b:
-            ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(x_type, rows, cols)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-        x_stride = dy_stride = cols
-        if not x.is_contiguous() or x.is_neg():
-            x = _rows(x, cols)
-            x_stride = x.stride(0)
-        if not dy.is_contiguous() or dy.is_neg():
-            dy = _rows(dy, cols)
-            dy_stride = dy.stride(0)
-        weight, keep = _packed(weight), _packed(keep)
-        index, at = x.device.index, stats.data_ptr() or None
-        rc = lib.lrb_layer_norm_bwd_dev(
-            index, _stream(index), x_type, 0 if w_type is None else _TYPES[w_type], rows, cols, x.data_ptr() or None, x_stride,
-            dy.data_ptr() or None, dy_stride, _address(weight), at, at and at + 4 * rows, slope, _address(keep) or None, keep_scale,
-            _address(dx) or None, _address(dw), _address(db), _address(ws), ws_bytes)
-        if rc:
-            check("lrb_layer_norm_bwd_dev", rc)
-        return dx, dw, db, None, None, None, None
+        # gradients are enabled here only where a graph of the backward pass is asked for (the wrapper costs a small operator
+        # 5 us of a hundred)
+        return _ln_backward_of_a_graph(ctx, dy) if torch.is_grad_enabled() else _ln_backward(ctx, dy)
 
 
 def _ln_plain(x, weight, bias, keep, eps, slope, keep_scale):

@@ -637,3 +637,14 @@ def test_threads_on_streams_of_their_own():
     assert not failed
     for g, w in zip(got, want):
         assert torch.equal(g, w)
+
+
+def test_second_derivatives_are_refused():
+    x, w, b, dy, _ = inputs(6, 20, torch.float32)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    plain = torch.autograd.grad(train_ops.layer_norm(*leaves), leaves, dy)
+    graph = torch.autograd.grad(train_ops.layer_norm(*leaves), leaves, dy, create_graph=True)
+    for g, e in zip(graph, plain):
+        assert torch.equal(g, e)
+    with pytest.raises(RuntimeError):  # (of gradients that hang on dy: by autograd itself, these do not)
+        graph[0].sum().backward()
