@@ -524,20 +524,28 @@ __device__ __forceinline__ void mu_update4(const mu_item &it, long long at, long
 // whole row segments, and once more by columns for the mirrored or transposed side.
 //   MU_GRAM, MU_SYM: buffer `out` = k0 old + k1 sum + k2 old2 (buffers; -1: none)      MU_APPLY: X = k0 X + k1 sum; MU_LAST: p
 #define MU_PITCH(NI) (32 * (NI) + 4)
+// The factors of an operation.  What is loaded for them is asked for before the products and looked at behind them.
 struct mu_factors {
-    float k0, k1, k2;
-    // (asked for before the products, so that the results do not wait for it)
-    __device__ __forceinline__ mu_factors(const mu_args &a, const mu_job &job, int matrix) : k0(job.k[0]), k1(job.k[1]), k2(job.k[2])
+    const mu_job &job;
+    double ready; // not 0: the launch's own factors hold
+    float t0, t1, t2;
+    __device__ __forceinline__ mu_factors(const mu_args &a, const mu_job &j, int matrix) : job(j)
     {
-        if (a.x0[2 * matrix + 1] == 0.0) {
-            const float *t = a.table + ((size_t)matrix * MU_OPS + job.op) * MU_COEF;
-            k0 = t[0], k1 = t[1], k2 = t[2];
-        }
+        const float *t = a.table + ((size_t)matrix * MU_OPS + j.op) * MU_COEF;
+        ready = a.x0[2 * matrix + 1], t0 = t[0], t1 = t[1], t2 = t[2];
     }
+    __device__ __forceinline__ float k0() const { return ready != 0.0 ? job.k[0] : t0; }
+    __device__ __forceinline__ float k1() const { return ready != 0.0 ? job.k[1] : t1; }
+    __device__ __forceinline__ float k2() const { return ready != 0.0 ? job.k[2] : t2; }
 };
-template <int MODE, int NI>
+
+// The old entries in float32 that a lane combines with its part of a strip of 32 x 32, asked for before the products.
+struct mu_early {
+    float4 o[4];
+};
+template <int MODE, int NI, bool EARLY>
 __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_job &job, const mu_factors &f, const mu_item &it, int mat, const mu_mat &w,
-                                         const mu_f16 (&acc)[NI], int i0, int j0, bool mirror, float *lds, int lane)
+                                         const mu_f16 (&acc)[NI], int i0, int j0, bool mirror, float *lds, int lane, const mu_early &early)
 {
     constexpr int PITCH = MU_PITCH(NI), LANES = 8 * NI, ROWS = 64 / LANES; // lanes of a row, rows of a turn
     const int ld = MODE >= MU_APPLY ? it.lp : it.np;
@@ -563,16 +571,17 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_job &job, co
                 make_float4(acc[y][4 * q], acc[y][4 * q + 1], acc[y][4 * q + 2], acc[y][4 * q + 3]);
     mu_wave_sync();
     const bool back = MODE == MU_LAST ? !by_rows : mirror;
+    const float k0 = f.k0(), k1 = f.k1(), k2 = f.k2();
 #pragma unroll(MODE == MU_LAST ? 1 : 4)
-    for (int r = lane / LANES; r < 32; r += ROWS) {
-        const int c = (lane % LANES) * 4, i = i0 + r, j = j0 + c;
+    for (int turn = 0; turn < 32 / ROWS; ++turn) {
+        const int r = turn * ROWS + lane / LANES, c = (lane % LANES) * 4, i = i0 + r, j = j0 + c;
         if (i >= it.np || j >= ld) continue;
         float4 v = *(const float4 *)(lds + r * PITCH + c);
-        const float4 o = has_old ? read_old(old, old_h, i, j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        v = make_float4(f.k0 * o.x + f.k1 * v.x, f.k0 * o.y + f.k1 * v.y, f.k0 * o.z + f.k1 * v.z, f.k0 * o.w + f.k1 * v.w);
+        const float4 o = EARLY && exact ? early.o[turn & 3] : has_old ? read_old(old, old_h, i, j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v = make_float4(k0 * o.x + k1 * v.x, k0 * o.y + k1 * v.y, k0 * o.z + k1 * v.z, k0 * o.w + k1 * v.w);
         if (has_old2) {
             const float4 o2 = read_old(old2, old2_h, i, j);
-            v.x += f.k2 * o2.x, v.y += f.k2 * o2.y, v.z += f.k2 * o2.z, v.w += f.k2 * o2.w;
+            v.x += k2 * o2.x, v.y += k2 * o2.y, v.z += k2 * o2.z, v.w += k2 * o2.w;
         }
         if (back) *(float4 *)(lds + r * PITCH + c) = v;
         if (MODE == MU_LAST) {
@@ -718,6 +727,15 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const int k_end = part ? (int)((long long)units * (unit % a.splits + 1) / a.splits) * 64 : K;
     const char *const base_p = (const char *)(P + (size_t)i0 * 2 * K), *const base_q = (const char *)(Q + (size_t)j0 * 2 * K);
 
+    constexpr bool EARLY = T == 64 && (MODE == MU_SYM || MODE == MU_APPLY);
+    mu_early early;
+    if (EARLY && a.exact) { // (rows and columns of a 64-tile all lie inside)
+        const float *old = MODE == MU_APPLY ? w.x32 : job.old >= 0 ? w.full(job.old) : nullptr;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            early.o[q] = old ? *(const float4 *)(old + (size_t)(i0 + wi * 32 + lane / 8 + 8 * q) * (MODE == MU_APPLY ? it.lp : it.np) + j0 + wj * 32 + lane % 8 * 4)
+                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
     mu_f16 acc[MI][NI];
 #pragma unroll
     for (int x = 0; x < MI; ++x)
@@ -846,7 +864,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const bool mirror = MODE == MU_APPLY || i0 != j0;
 #pragma unroll
     for (int x = 0; x < MI; ++x)
-        mu_strip<MODE, NI>(a, job, factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane);
+        mu_strip<MODE, NI, EARLY>(a, job, factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane, early);
 }
 
 // The tiles that were cut along k: their parts' sums, added up in order, a wave for each 32 rows of one of the tile's waves.
@@ -883,7 +901,8 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
             }
     const mu_mat w = mu_planes(a, it, mat);
     const mu_factors factors(a, job, it.first + mat);
-    mu_strip<MODE, NI>(a, job, factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane);
+    mu_strip<MODE, NI, false>(a, job, factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane,
+                              mu_early());
 }
 
 // A matrix that fits one workgroup's LDS (128 x 208, 96 x 320, 64 x 512, 32 x 1,024 and less) goes through all its steps there, in one
