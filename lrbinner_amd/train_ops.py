@@ -56,11 +56,12 @@ def _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, stats):
     """y, and with `stats` the float32 [2, rows] of means and 1 / deviations that the backward pass takes."""
     cols = x.shape[-1]
     rows = x.numel() // cols
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dense = x.is_contiguous() and not x.is_neg()
+    y = torch.empty_like(x) if dense else torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
     if rows:
         stride = cols
-        if not x.is_contiguous() or x.is_neg():
+        if not dense:
             x = _rows(x, cols)
             stride = x.stride(0)
         weight, bias, keep = _packed(weight), _packed(bias), _packed(keep)
@@ -81,25 +82,32 @@ def _ln_backward(ctx, dy):
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     cols = x.shape[-1]
     rows = x.numel() // cols
-    w_type = weight.dtype if weight is not None else bias_type
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-    dw = torch.empty(cols, dtype=w_type, device=x.device) if need_w else None
-    db = torch.empty(cols, dtype=w_type, device=x.device) if need_b else None
+    device = x.device
+    w_type, dx, dw, db = bias_type, None, None, None
+    weight, keep = _packed(weight), _packed(keep)
+    dense = x.is_contiguous() and not x.is_neg()
+    if need_x:
+        dx = torch.empty_like(x) if dense else torch.empty_like(x, memory_format=torch.contiguous_format)
+    if weight is not None:
+        w_type = weight.dtype
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(weight) if need_b else None
+    elif need_b:
+        db = torch.empty(cols, dtype=w_type, device=device)
     lib = _lib.lib()
     x_type = _TYPES[x.dtype]
     ws, ws_bytes = None, 0
     if need_w or need_b:
         ws_bytes = lib.lrb_layer_norm_bwd_ws_bytes(x_type, rows, cols)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     x_stride = dy_stride = cols
-    if not x.is_contiguous() or x.is_neg():
+    if not dense:
         x = _rows(x, cols)
         x_stride = x.stride(0)
     if not dy.is_contiguous() or dy.is_neg():
         dy = _rows(dy, cols)
         dy_stride = dy.stride(0)
-    weight, keep = _packed(weight), _packed(keep)
-    index, at = x.device.index, stats.data_ptr() or None
+    index, at = device.index, stats.data_ptr() or None
     rc = lib.lrb_layer_norm_bwd_dev(
         index, _stream(index), x_type, 0 if w_type is None else _TYPES[w_type], rows, cols, x.data_ptr() or None, x_stride,
         dy.data_ptr() or None, dy_stride, _address(weight), at, at and at + 4 * rows, slope, _address(keep) or None, keep_scale,
