@@ -648,3 +648,22 @@ def test_second_derivatives_are_refused():
         assert torch.equal(g, e)
     with pytest.raises(RuntimeError):  # (of gradients that hang on dy: by autograd itself, these do not)
         graph[0].sum().backward()
+
+
+# 128-tiles, and 256-tiles, of which two products of a block share a launch; of an uneven number of steps
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("count,rows,cols", [(7, 1000, 2100), (4, 2048, 2700), (5, 1901, 900)])
+def test_orthogonalize_stacks_in_blocks_of_steps(count, rows, cols, kind):
+    g = gradient_like(rows, cols, torch.Generator().manual_seed(9), "cuda", (count,)).to(TYPES[kind])
+    g[1] *= 1e-12  # below eps: factors of its own
+    for steps in (3, 5, 8):
+        got = check_orthogonal(g, steps=steps)
+        assert torch.equal(got, train_ops.orthogonalize(g, steps=steps))
+
+
+def test_muon_step_in_blocks_of_steps_on_weights_of_two_types():
+    shapes = [(700, 2100), (1500, 600), (2, 640, 1500), (100, 90)]
+    for kinds in (("bf16", "bf16", "f16", "bf16"), ("bf16", "f32", "f16", "f32")):
+        p, g, m = weights(shapes, [TYPES[k] for k in kinds])
+        check_muon(p, g, m)
+        check_muon(p, g, None)
