@@ -7,7 +7,8 @@ of weights (momentum, iteration and update in shared launches), and ``Muon`` is 
 
 On the GPU the arithmetic is csrc/lrb_norm.hip and csrc/lrb_muon.hip behind the C ABI of include/lrb_hip.h; calls go to
 torch's current stream of the tensors' device, their workspace comes from torch's allocator (so calls may be captured in a
-HIP graph), and there is no fallback where the library is missing.  On CPU tensors the same definitions run as torch
+HIP graph; a captured backward pass, as any of torch's, wants leaves that no living eager graph holds), and there is no
+fallback where the library is missing.  On CPU tensors the same definitions run as torch
 operations, as the network itself does without ``--cuda``.
 
 Float32, bfloat16 and float16; what is summed is summed in float32 or more, and results are rounded once."""
