@@ -17,8 +17,10 @@
 // All products are of the form C[i][j] = sum_k P[i][k] Q[j][k] with k contiguous in both: A = X X^T and A^2 = A A^T as they
 // stand, B X from X's transpose, which the epilogue writes beside X.  One workgroup a T x T tile of C; of the symmetric
 // products the tiles on and above the diagonal are computed and mirrored.  Tiles of all weights of a call share a launch.
-// Where X is longer than wide several steps share one formation of X (mu_walk); a matrix that fits one workgroup's LDS goes
-// through all steps in one launch (mu_small_kernel).
+// Every step forms A from the X before it, for every type of p: a 16-bit result is the float32 result, rounded.  (Where X is longer
+// than wide fewer products would do if A were carried over several steps by the polynomial it goes through; the rounding
+// errors of the small singular values' part of A would then grow by a^2 a step instead of a.)  A matrix that fits one workgroup's LDS
+// goes through all steps in one launch (mu_small_kernel).
 // Measured, where a library product of 8192 x 8192 float16 reaches 1.09 PFLOP/s: a 4096 x 4096 float32 weight 3.9 ms = 1.05
 // PFLOP/s of its three products (B X alone 1.17); a layer's four weights (2048 x 2048 twice, 5461 x 2048, 2048 x 5461,
 // bfloat16) 2.96 ms, of them 0.15 for the momentum and the splitting, at 4.6 and 5.3 TB/s; 8 x 1024 x 2048 0.98 ms;
@@ -41,9 +43,8 @@ typedef float mu_f16 __attribute__((ext_vector_type(16)));
 
 #define MU_ITEMS 14       // weights of one launch (their descriptors travel as kernel arguments)
 #define MU_STEPS 32       // longest iteration
-#define MU_BLOCK_STEPS 5  // most steps between two formations of X
-#define MU_COEF 3         // factors of an operation
-#define MU_OPS 128        // operations of the longest iteration: 3 of a single step, 4 n - 1 of a block of n
+#define MU_COEF 2         // factors of an operation: of the old entry, and of the sum of products
+#define MU_OPS 3          // operations of a step
 #define MU_TOP 57344.0    // the largest entry that a factor is scaled to: 7/8 of fp16's largest number
 #define MU_BK 32          // k of one stage in LDS
 
@@ -59,68 +60,53 @@ struct mu_item {
     float alpha, decay;
 };
 
-// An operation of the iteration: its number, its factors for a norm of at least eps, and the n x n buffers it reads and writes
-// (see mu_strip).  keep: the result in float32 too.
-struct mu_job {
-    int op;
-    float k[MU_COEF];
-    int u, v, old, old2, out, keep;
-};
-
 struct mu_args {
     char *ws;
     double *x0;     // [matrices][2] what u is multiplied by; 1 if the launch's own factors hold, 0 for those of the table
-    float *table;   // [matrices][MU_OPS][MU_COEF]
+    float *table;   // [matrices][steps][MU_OPS][MU_COEF]
     double *part;   // [tiles of 64 x 64 of all matrices] sums of squares
     int n_items, steps;
     float beta, eps, a, b, c;
     int nesterov;
     int flip;       // which of the two copies of X is read
-    int exact;      // the matrices are kept in float32 too
-    int jobs;       // operations of this launch: two symmetric products that do not need each other's results, or one
-    mu_job job[2];
-    int n_sizes;                     // the iteration's blocks
-    uint8_t sizes[MU_STEPS];
+    int op;         // the operation of this launch, counted through the steps, and its factors for a norm of at least eps
+    float k[MU_COEF];
     // of a product's launch: the tiles from `direct` on are cut along k, `splits` workgroups each, whose sums go to `parts`
     int direct, splits;
     float *parts;
     double sx;                       // the scale of X at the start for a norm of at least eps
-    float std[MU_STEPS * 3 * MU_COEF]; // and all factors, of single steps (for the small matrices)
+    float std[MU_STEPS * MU_OPS * MU_COEF]; // and all factors
     int start[MU_ITEMS + 1]; // first tile of each item in this launch
     mu_item it[MU_ITEMS];
 };
 static_assert(sizeof(mu_args) <= 4096, "kernel arguments");
 
-// A matrix in the workspace: X and its transpose twice (read and written in turn), and five n x n buffers for A, B and what
-// is made of them, as rows of 32 hi, the 32 lo of the same entries, the next 32 hi ...: 32 k of a row are one whole line of 128
-// bytes, which halves the requests that the L2 gets for a stage against separate planes of hi and lo (4096 x 4096, B X: 43 M ->
-// 21 M).  And X and the buffers in float32, for the terms that are not products (a X, b A ...): hi + lo is a rounding more than
-// float32 is, and these terms would pass it on.  Of symmetric matrices the float32 is there on and above the diagonal's tiles.
-// Blocks of steps whose results are all 16-bit (mu_blocks) do without it.
+// A matrix in the workspace: X and its transpose twice (read and written in turn), A and B, as rows of 32 hi, the 32 lo of the
+// same entries, the next 32 hi ...: 32 k of a row are one whole line of 128 bytes, which halves the requests that the L2 gets for
+// a stage against separate planes of hi and lo (4096 x 4096, B X: 43 M -> 21 M).  And X and A in float32, for the terms that are
+// not products (a X, b A): hi + lo is a rounding more than float32 is, and these terms would pass it on.  A's float32 is there on
+// and above the diagonal's tiles.
 __host__ __device__ inline unsigned long long mu_plane_x(const mu_item &it) { return 4ull * (unsigned long long)it.np * it.lp; }
 __host__ __device__ inline unsigned long long mu_plane_a(const mu_item &it) { return 4ull * (unsigned long long)it.np * it.np; }
-__host__ __device__ inline unsigned long long mu_bytes(const mu_item &it, int buffers) { return 5 * mu_plane_x(it) + 2 * buffers * mu_plane_a(it); }
+__host__ __device__ inline unsigned long long mu_bytes(const mu_item &it) { return 5 * mu_plane_x(it) + 3 * mu_plane_a(it); }
 
 struct mu_mat {
-    mu_h *x, *xt, *x2, *xt2;
-    float *x32;
-    char *buffers;
-    unsigned long long pa;
-    __device__ __forceinline__ mu_h *half(int b) const { return (mu_h *)(buffers + 2 * b * pa); }
-    __device__ __forceinline__ float *full(int b) const { return (float *)(buffers + (2 * b + 1) * pa); }
+    mu_h *x, *xt, *x2, *xt2, *a, *b;
+    float *x32, *a32;
 };
 __device__ __forceinline__ mu_mat mu_planes(const mu_args &a, const mu_item &it, int mat)
 {
     char *w = a.ws + it.off + (unsigned long long)mat * it.step;
-    const unsigned long long px = mu_plane_x(it);
+    const unsigned long long px = mu_plane_x(it), pa = mu_plane_a(it);
     mu_mat r;
     r.x = (mu_h *)(w + (a.flip ? 2 * px : 0));
     r.xt = (mu_h *)(w + (a.flip ? 3 * px : px));
     r.x2 = (mu_h *)(w + (a.flip ? 0 : 2 * px));
     r.xt2 = (mu_h *)(w + (a.flip ? px : 3 * px));
     r.x32 = (float *)(w + 4 * px);
-    r.buffers = w + 5 * px;
-    r.pa = mu_plane_a(it);
+    r.a = (mu_h *)(w + 5 * px);
+    r.b = (mu_h *)(w + 5 * px + pa);
+    r.a32 = (float *)(w + 5 * px + 2 * pa);
     return r;
 }
 
@@ -270,94 +256,48 @@ __host__ __device__ double mu_scale(double r) // the power of two that takes ent
     return ldexp(1.0, e - 1);
 }
 
-// The operations of an iteration in blocks of sizes[0], sizes[1] ... steps, in their order:
-//   gram()       A = X X^T
-//   then for every step k of a block of n
-//   poly(k)      P = b A + c A^2
-//   sum(k)       k > 0: S <- a S + a^k P + P S        (a^(k+1) I + S is the product of all (a I + P) so far; S = P for k = 0)
-//   turn()       k + 1 < n: C = a A + P A             (all of these are polynomials of the same A: they commute, and the
-//   turn2()                 A <- a C + C P             products are symmetric)
-//   apply(n)     X <- a^n X + S X
-// sum(k) and the turn() behind it share a launch: neither needs the other's result.
-// A block of one step is the iteration as it is written.  A longer one forms X and X X^T once for its n steps, and pays with
-// four symmetric n x n products a step more: for X of n x r n entries 1.5 r + 4.5 units of 2 n^3 for three steps against
-// 4.5 r + 1.5.
-template <typename V> __host__ __device__ inline void mu_walk(const uint8_t *sizes, int n_sizes, V &v)
+// The operations of an iteration, in their order:
+//   gram()   A = X X^T
+//   poly()   B = b A + c A^2
+//   apply()  X <- a X + B X
+template <typename V> __host__ __device__ inline void mu_walk(int steps, V &v)
 {
-    for (int q = 0; q < n_sizes; ++q) {
-        const int n = sizes[q];
+    for (int k = 0; k < steps; ++k) {
         v.gram();
-        for (int k = 0; k < n; ++k) {
-            v.poly(k, n);
-            if (k > 0) v.sum(k, n);
-            if (k + 1 < n) {
-                v.turn();
-                v.turn2();
-            }
-        }
-        v.apply(n, q + 1 == n_sizes);
+        v.poly();
+        v.apply(k + 1 == steps);
     }
 }
 
-// Writes the factors of every operation: of the old entry, the sum of products, and the second old entry.  Scales are powers
-// of two, from bounds on the largest singular values.
+// Writes the factors of every operation: of the old entry, and of the sum of products.  Scales are powers of two, from bounds on
+// the largest singular values.
 struct mu_chain {
-    double a, b, c, r, sx, ra = 0.0, sa = 0.0, sp = 0.0, ss = 0.0, sc = 0.0, product = 1.0;
+    double a, b, c, r, sx, ra = 0.0, sa = 0.0, sb = 0.0;
     float *t;
     static constexpr double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
     __host__ __device__ mu_chain(double a_, double b_, double c_, double r_, float *t_) : a(a_), b(b_), c(c_), r(r_ * slack), t(t_) { sx = mu_scale(r); }
-    __host__ __device__ void put(double k0, double k1, double k2)
+    __host__ __device__ void put(double k0, double k1)
     {
-        t[0] = (float)k0, t[1] = (float)k1, t[2] = (float)k2;
+        t[0] = (float)k0, t[1] = (float)k1;
         t += MU_COEF;
-    }
-    __host__ __device__ double largest(double first) const // max |first + b t + c t^2| over [0, ra]
-    {
-        double m = fmax(fabs(first), fabs(first + b * ra + c * ra * ra));
-        if (c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < ra) m = fmax(m, fabs(first - b * b / (4.0 * c)));
-        return m * slack;
     }
     __host__ __device__ void gram()
     {
         ra = r * r * slack, sa = mu_scale(ra);
-        put(0.0, sa / (sx * sx), 0.0);
+        put(0.0, sa / (sx * sx));
     }
-    __host__ __device__ void poly(int k, int)
+    __host__ __device__ void poly()
     {
-        sp = mu_scale(largest(0.0));
-        put(b * (sp / sa), c * (sp / sa) / sa, 0.0);
-        product = (k ? product : 1.0) * largest(a);
-        if (k == 0) ss = sp;
+        double m = fabs(b * ra + c * ra * ra); // max |b t + c t^2| over [0, ra]
+        if (c != 0.0 && -b / (2.0 * c) > 0.0 && -b / (2.0 * c) < ra) m = fmax(m, fabs(b * b / (4.0 * c)));
+        sb = mu_scale(m * slack);
+        put(b * (sb / sa), c * (sb / sa) / sa);
     }
-    __host__ __device__ void sum(int k, int)
+    __host__ __device__ void apply(bool last)
     {
-        double power = 1.0;
-        for (int q = 0; q < k; ++q) power *= a;
-        const double s = mu_scale(fabs(power * a) + product);
-        put(a * (s / ss), s / sp / ss, power * (s / sp));
-        ss = s;
-    }
-    __host__ __device__ void turn()
-    {
-        const double next = mu_largest_odd(a, b, c, r) * slack;
-        sc = mu_scale(r * next * slack);
-        put(a * (sc / sa), sc / sp / sa, 0.0);
-        r = next;
-    }
-    __host__ __device__ void turn2()
-    {
-        ra = r * r * slack;
-        const double s = mu_scale(ra);
-        put(a * (s / sc), s / sc / sp, 0.0);
-        sa = s;
-    }
-    __host__ __device__ void apply(int n, bool last)
-    {
-        double power = 1.0;
-        for (int q = 0; q < n; ++q) power *= a;
         r = mu_largest_odd(a, b, c, r) * slack;
         const double s = last ? 1.0 : mu_scale(r);
-        put(power * (s / sx), s / ss / sx, 0.0);
+        put(a * (s / sx), s / sb / sx);
         sx = s;
     }
 };
@@ -395,9 +335,9 @@ __global__ __launch_bounds__(256) void mu_table_kernel(mu_args a)
     const mu_norm n = mu_start(red[0] + red[1] + red[2] + red[3], a.eps);
     double scale = a.sx;
     if (n.r != 1.0) {
-        mu_chain chain(a.a, a.b, a.c, n.r, a.table + (size_t)blockIdx.x * MU_OPS * MU_COEF);
+        mu_chain chain(a.a, a.b, a.c, n.r, a.table + (size_t)blockIdx.x * a.steps * MU_OPS * MU_COEF);
         scale = chain.sx;
-        mu_walk(a.sizes, a.n_sizes, chain);
+        mu_walk(a.steps, chain);
     }
     a.x0[2 * blockIdx.x] = n.x0 * scale;
     a.x0[2 * blockIdx.x + 1] = n.r == 1.0 ? 1.0 : 0.0;
@@ -463,7 +403,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = tile[row][c + q];
         mu_split8(v, hi, lo);
-        if (a.exact) __builtin_memcpy(w.x32 + (size_t)(i0 + row) * it.lp + j0 + c, v, 32);
+        __builtin_memcpy(w.x32 + (size_t)(i0 + row) * it.lp + j0 + c, v, 32);
         *(mu_h8 *)(w.x + at) = hi;
         *(mu_h8 *)(w.x + at + 32) = lo;
 #pragma unroll
@@ -522,21 +462,20 @@ __device__ __forceinline__ void mu_update4(const mu_item &it, long long at, long
 // What becomes of 32 x 32 NI entries of a product, of which a wave holds the sums: acc[y][4 q + e] of a lane is row (lane & 31),
 // column 32 y + 8 q + 4 (lane >> 5) + e.  They go through `lds` (32 rows of MU_PITCH) to be read, combined and written in
 // whole row segments, and once more by columns for the mirrored or transposed side.
-//   MU_GRAM, MU_SYM: buffer `out` = k0 old + k1 sum + k2 old2 (buffers; -1: none)      MU_APPLY: X = k0 X + k1 sum; MU_LAST: p
+//   MU_GRAM: A = k1 sum      MU_SYM: B = k0 A + k1 sum      MU_APPLY: X = k0 X + k1 sum; MU_LAST: p
 #define MU_PITCH(NI) (32 * (NI) + 4)
 // The factors of an operation.  What is loaded for them is asked for before the products and looked at behind them.
 struct mu_factors {
-    const mu_job &job;
+    const mu_args &a;
     double ready; // not 0: the launch's own factors hold
-    float t0, t1, t2;
-    __device__ __forceinline__ mu_factors(const mu_args &a, const mu_job &j, int matrix) : job(j)
+    float t0, t1;
+    __device__ __forceinline__ mu_factors(const mu_args &args, int matrix) : a(args)
     {
-        const float *t = a.table + ((size_t)matrix * MU_OPS + j.op) * MU_COEF;
-        ready = a.x0[2 * matrix + 1], t0 = t[0], t1 = t[1], t2 = t[2];
+        const float *t = a.table + ((size_t)matrix * a.steps * MU_OPS + a.op) * MU_COEF;
+        ready = a.x0[2 * matrix + 1], t0 = t[0], t1 = t[1];
     }
-    __device__ __forceinline__ float k0() const { return ready != 0.0 ? job.k[0] : t0; }
-    __device__ __forceinline__ float k1() const { return ready != 0.0 ? job.k[1] : t1; }
-    __device__ __forceinline__ float k2() const { return ready != 0.0 ? job.k[2] : t2; }
+    __device__ __forceinline__ float k0() const { return ready != 0.0 ? a.k[0] : t0; }
+    __device__ __forceinline__ float k1() const { return ready != 0.0 ? a.k[1] : t1; }
 };
 
 // The old entries in float32 that a lane combines with its part of a strip of 32 x 32, asked for before the products: a launch of
@@ -545,23 +484,14 @@ struct mu_early {
     float4 o[4];
 };
 template <int MODE, int NI, bool EARLY>
-__device__ __forceinline__ void mu_strip(const mu_args &a, const mu_job &job, const mu_factors &f, const mu_item &it, int mat, const mu_mat &w,
+__device__ __forceinline__ void mu_strip(const mu_factors &f, const mu_item &it, int mat, const mu_mat &w,
                                          const mu_f16 (&acc)[NI], int i0, int j0, bool mirror, float *lds, int lane, const mu_early &early)
 {
     constexpr int PITCH = MU_PITCH(NI), LANES = 8 * NI, ROWS = 64 / LANES; // lanes of a row, rows of a turn
     const int ld = MODE >= MU_APPLY ? it.lp : it.np;
-    const bool exact = a.exact, keep = exact && (MODE != MU_SYM || job.keep);
-    const bool has_old = MODE >= MU_APPLY || job.old >= 0, has_old2 = MODE == MU_SYM && job.old2 >= 0;
-    // the old entries in float32, or, where nothing is kept in float32, their halves
-    const float *old = MODE >= MU_APPLY ? w.x32 : w.full(job.old), *old2 = w.full(job.old2);
-    const mu_h *old_h = MODE >= MU_APPLY ? w.x : w.half(job.old), *old2_h = w.half(job.old2);
-    auto read_old = [=](const float *full, const mu_h *half, int i, int j) {
-        if (exact) return *(const float4 *)(full + (size_t)i * ld + j);
-        const mu_h4 hi = *(const mu_h4 *)(half + mu_at(i, j, ld)), lo = *(const mu_h4 *)(half + mu_at(i, j, ld) + 32);
-        return make_float4((float)hi[0] + (float)lo[0], (float)hi[1] + (float)lo[1], (float)hi[2] + (float)lo[2], (float)hi[3] + (float)lo[3]);
-    };
-    float *full = MODE == MU_APPLY ? w.x32 : w.full(job.out);
-    mu_h *out = MODE == MU_APPLY ? w.x2 : w.half(job.out), *out_t = MODE == MU_APPLY ? w.xt2 : out;
+    const float *old = MODE >= MU_APPLY ? w.x32 : w.a32;
+    float *full = MODE == MU_APPLY ? w.x32 : w.a32; // (MU_GRAM; B is a factor only)
+    mu_h *out = MODE == MU_APPLY ? w.x2 : MODE == MU_GRAM ? w.a : w.b, *out_t = MODE == MU_APPLY ? w.xt2 : out;
     const bool by_rows = it.ps[2] == 1 || it.ps[1] != 1; // which way p is written
     mu_wave_sync();
 #pragma unroll
@@ -572,25 +502,21 @@ __device__ __forceinline__ void mu_strip(const mu_args &a, const mu_job &job, co
                 make_float4(acc[y][4 * q], acc[y][4 * q + 1], acc[y][4 * q + 2], acc[y][4 * q + 3]);
     mu_wave_sync();
     const bool back = MODE == MU_LAST ? !by_rows : mirror;
-    const float k0 = f.k0(), k1 = f.k1(), k2 = f.k2();
+    const float k0 = f.k0(), k1 = f.k1();
 #pragma unroll(MODE == MU_LAST ? 1 : 4)
     for (int turn = 0; turn < 32 / ROWS; ++turn) {
         const int r = turn * ROWS + lane / LANES, c = (lane % LANES) * 4, i = i0 + r, j = j0 + c;
         if (i >= it.np || j >= ld) continue;
         float4 v = *(const float4 *)(lds + r * PITCH + c);
-        const float4 o = EARLY && exact ? early.o[turn & 3] : has_old ? read_old(old, old_h, i, j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float4 o = EARLY ? early.o[turn & 3] : MODE == MU_GRAM ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *(const float4 *)(old + (size_t)i * ld + j);
         v = make_float4(k0 * o.x + k1 * v.x, k0 * o.y + k1 * v.y, k0 * o.z + k1 * v.z, k0 * o.w + k1 * v.w);
-        if (has_old2) {
-            const float4 o2 = read_old(old2, old2_h, i, j);
-            v.x += k2 * o2.x, v.y += k2 * o2.y, v.z += k2 * o2.z, v.w += k2 * o2.w;
-        }
         if (back) *(float4 *)(lds + r * PITCH + c) = v;
         if (MODE == MU_LAST) {
             if (by_rows && i < it.n && j < it.l) mu_update4(it, mat * it.ps[0] + i * it.ps[1] + j * it.ps[2], it.ps[2], min(4, it.l - j), v);
         } else {
             mu_h4 hi, lo;
             mu_split4(v.x, v.y, v.z, v.w, hi, lo);
-            if (keep) *(float4 *)(full + (size_t)i * ld + j) = v;
+            if (MODE == MU_GRAM || MODE == MU_APPLY) *(float4 *)(full + (size_t)i * ld + j) = v;
             *(mu_h4 *)(out + mu_at(i, j, ld)) = hi;
             *(mu_h4 *)(out + mu_at(i, j, ld) + 32) = lo;
         }
@@ -700,16 +626,14 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
     const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k];
-    const bool two = MODE == MU_SYM && a.jobs > 1; // both operations of a matrix side by side
-    const int mat = two ? local / per >> 1 : local / per;
-    const mu_job &job = a.job[two ? local / per & 1 : 0];
+    const int mat = local / per;
     int i0, j0;
     mu_place<MODE>(local % per, ti, tj, i0, j0);
     i0 *= T, j0 *= T;
     const mu_mat w = mu_planes(a, it, mat);
-    const mu_factors factors(a, job, it.first + mat);
+    const mu_factors factors(a, it.first + mat);
     const int K = MODE == MU_GRAM ? it.lp : it.np, jrows = MODE >= MU_APPLY ? it.lp : it.np;
-    const mu_h *P = MODE == MU_GRAM ? w.x : w.half(job.u), *Q = MODE == MU_GRAM ? w.x : MODE == MU_SYM ? w.half(job.v) : w.xt;
+    const mu_h *P = MODE == MU_GRAM ? w.x : MODE == MU_SYM ? w.a : w.b, *Q = MODE == MU_GRAM ? w.x : MODE == MU_SYM ? w.a : w.xt;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN, wj = wave % WN;
 
     // A load of a wave fills eight rows of a stage.  All addresses are a factor's first row of the tile (uniform) and an offset of
@@ -730,12 +654,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 
     constexpr bool EARLY = T == 64 && (MODE == MU_SYM || MODE == MU_APPLY);
     mu_early early;
-    if (EARLY && a.exact) { // (rows and columns of a 64-tile all lie inside)
-        const float *old = MODE == MU_APPLY ? w.x32 : job.old >= 0 ? w.full(job.old) : nullptr;
+    if (EARLY) { // (rows and columns of a 64-tile all lie inside)
+        const float *old = MODE == MU_APPLY ? w.x32 : w.a32;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            early.o[q] = old ? *(const float4 *)(old + (size_t)(i0 + wi * 32 + lane / 8 + 8 * q) * (MODE == MU_APPLY ? it.lp : it.np) + j0 + wj * 32 + lane % 8 * 4)
-                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            early.o[q] = *(const float4 *)(old + (size_t)(i0 + wi * 32 + lane / 8 + 8 * q) * (MODE == MU_APPLY ? it.lp : it.np) + j0 + wj * 32 + lane % 8 * 4);
     }
     mu_f16 acc[MI][NI];
 #pragma unroll
@@ -865,7 +788,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
     const bool mirror = MODE == MU_APPLY || i0 != j0;
 #pragma unroll
     for (int x = 0; x < MI; ++x)
-        mu_strip<MODE, NI, EARLY>(a, job, factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane, early);
+        mu_strip<MODE, NI, EARLY>(factors, it, mat, w, acc[x], i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, mirror, lds, lane, early);
 }
 
 // The tiles that were cut along k: their parts' sums, added up in order, a wave for each 32 rows of one of the tile's waves.
@@ -878,9 +801,7 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
     const mu_item &it = a.it[k];
     const int ti = (it.np + T - 1) / T, tj = MODE >= MU_APPLY ? (it.lp + T - 1) / T : ti;
     const int per = MODE >= MU_APPLY ? ti * tj : ti * (ti + 1) / 2, local = tile - a.start[k];
-    const bool two = MODE == MU_SYM && a.jobs > 1; // both operations of a matrix side by side
-    const int mat = two ? local / per >> 1 : local / per;
-    const mu_job &job = a.job[two ? local / per & 1 : 0];
+    const int mat = local / per;
     int i0, j0;
     mu_place<MODE>(local % per, ti, tj, i0, j0);
     i0 *= T, j0 *= T;
@@ -901,8 +822,8 @@ template <int T, int WM, int WN, int MODE> __global__ __launch_bounds__(64) void
                 acc[y][4 * q] += v.x, acc[y][4 * q + 1] += v.y, acc[y][4 * q + 2] += v.z, acc[y][4 * q + 3] += v.w;
             }
     const mu_mat w = mu_planes(a, it, mat);
-    const mu_factors factors(a, job, it.first + mat);
-    mu_strip<MODE, NI, false>(a, job, factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane,
+    const mu_factors factors(a, it.first + mat);
+    mu_strip<MODE, NI, false>(factors, it, mat, w, acc, i0 + (wi * MI + x) * 32, j0 + wj * NI * 32, MODE == MU_APPLY || i0 != j0, lds, lane,
                               mu_early());
 }
 
@@ -994,7 +915,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     const mu_args &a = *(const mu_args *)__builtin_amdgcn_kernarg_segment_ptr();
     extern __shared__ __attribute__((aligned(16))) char mu_lds[];
     __shared__ double red[MU_SMALL_WAVES];
-    __shared__ float own[MU_STEPS * 3 * MU_COEF];
+    __shared__ float own[MU_STEPS * MU_OPS * MU_COEF];
     int k = 0;
     while (k + 1 < a.n_items && (int)blockIdx.x >= a.it[k + 1].first) ++k;
     const mu_item &it = a.it[k];
@@ -1039,14 +960,14 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     const mu_norm n = mu_start(s, a.eps);
     double x0 = n.x0;
     if (n.r == 1.0) { // (all threads have the same s)
-        if ((int)threadIdx.x < a.steps * 3 * MU_COEF) own[threadIdx.x] = a.std[threadIdx.x];
+        if ((int)threadIdx.x < a.steps * MU_OPS * MU_COEF) own[threadIdx.x] = a.std[threadIdx.x];
         x0 *= a.sx;
     } else { // a norm below eps
         lrb_barrier(); // red has been read
         if (threadIdx.x == 0) {
             mu_chain chain(a.a, a.b, a.c, n.r, own);
             red[0] = chain.sx;
-            mu_walk(a.sizes, a.n_sizes, chain);
+            mu_walk(a.steps, chain);
         }
         lrb_barrier();
         x0 *= red[0];
@@ -1071,7 +992,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     while (ti < nt && tj >= nt - ti) tj -= nt - ti++;
     tj += ti;
     const bool sym = ti < nt;
-    for (int step = 0; step < a.steps; ++step, coef += 3 * MU_COEF) {
+    for (int step = 0; step < a.steps; ++step, coef += MU_OPS * MU_COEF) {
         // the addresses below are made anew in every step: kept over the steps, all of them together spill
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
@@ -1130,7 +1051,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
                 for (int h = 0; h < 2; ++h, p += 32, q += 32) mu_three(mu_by_row(p, 64), mu_by_row(q, 64), acc);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = coef[3] * full[e] + coef[4] * acc[e];
+            for (int e = 0; e < 16; ++e) acc[e] = coef[2] * full[e] + coef[3] * acc[e];
         }
         lrb_barrier();
         if (sym) mu_put_block(A + mu_block(ti, tj, nt), lane, acc);
@@ -1153,8 +1074,8 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                x[0][e] = coef[6] * x[0][e] + coef[7] * acc[e];
-                x[1][e] = coef[6] * x[1][e] + coef[7] * other[e];
+                x[0][e] = coef[4] * x[0][e] + coef[5] * acc[e];
+                x[1][e] = coef[4] * x[1][e] + coef[5] * other[e];
             }
         }
         lrb_barrier();
@@ -1193,33 +1114,31 @@ struct mu_plan {
     uint64_t part_bytes() const { return splits > 1 ? (uint64_t)(tiles - direct) * splits * T * T * 4 : 0; }
 };
 
-static long long mu_tiles(const mu_args &a, bool symmetric, int jobs, int T, int *start)
+static long long mu_tiles(const mu_args &a, bool symmetric, int T, int *start)
 {
     long long sum = 0;
     for (int k = 0; k < a.n_items; ++k) {
         if (start) start[k] = (int)sum;
         const long long ti = (a.it[k].np + T - 1) / T, tj = (a.it[k].lp + T - 1) / T;
-        sum += a.it[k].count * (symmetric ? jobs * (ti * (ti + 1) / 2) : ti * tj);
+        sum += a.it[k].count * (symmetric ? ti * (ti + 1) / 2 : ti * tj);
     }
     if (start) start[a.n_items] = (int)sum;
     return sum;
 }
 
 // The tile: the largest that still fills most of the chip (a larger tile loads less for each product): 256 CUs take one each of
-// 256, two each of 128.  (Eight symmetric products of 1024: 288 tiles of 128 and 1088 of 64 both take 47 us; 576 tiles
-// of 128, two such products in a launch, 68.)  All symmetric products of a group that is kept in float32 take the same (it is
-// there on and above the diagonal's tiles only).
+// 256, two each of 128.  (Eight symmetric products of 1024: 288 tiles of 128 and 1088 of 64 both take 47 us.)  Both symmetric products take the same (A's
+// float32 is there on and above the diagonal's tiles only).
 // The cut: a round of 256 tiles gives every CU one; the tiles that are left over behind the last whole round are cut along k so
 // that all CUs share them, if that saves more than the launch that joins the parts takes (about 5 us: 14 units of 64 k of the
 // smallest tile, five of the middle one, two of the largest).  4096 x 4096, symmetric product of 528 tiles: 302 us whole, 231 +
 // 12 with the last 16 cut (193 + 9 since a tile has eight waves).
-static mu_plan mu_lay_out(const mu_args &a, int mode, int jobs, bool exact)
+static mu_plan mu_lay_out(const mu_args &a, int mode)
 {
     const bool symmetric = mode <= MU_SYM;
-    const int counted = exact ? 1 : jobs;
     mu_plan p;
-    p.T = mu_tiles(a, symmetric, counted, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, counted, 128, nullptr) >= 400 ? 128 : 64;
-    p.tiles = mu_tiles(a, symmetric, jobs, p.T, nullptr);
+    p.T = mu_tiles(a, symmetric, 256, nullptr) >= 200 ? 256 : mu_tiles(a, symmetric, 128, nullptr) >= 400 ? 128 : 64;
+    p.tiles = mu_tiles(a, symmetric, p.T, nullptr);
     const long long rest = p.tiles % 256;
     p.direct = (int)p.tiles, p.splits = 1;
     if (rest == 0) return p;
@@ -1227,7 +1146,7 @@ static mu_plan mu_lay_out(const mu_args &a, int mode, int jobs, bool exact)
     long long before = 0;
     for (int k = 0; k < a.n_items; ++k) {
         const long long ti = (a.it[k].np + p.T - 1) / p.T, tj = (a.it[k].lp + p.T - 1) / p.T;
-        before += a.it[k].count * (symmetric ? jobs * (ti * (ti + 1) / 2) : ti * tj);
+        before += a.it[k].count * (symmetric ? ti * (ti + 1) / 2 : ti * tj);
         const long long u = (mode == MU_GRAM ? a.it[k].lp : a.it[k].np) / 64;
         if (before > p.tiles - rest && u < units) units = u;
     }
@@ -1252,112 +1171,35 @@ template <int T, int WM, int WN, int MODE> static void mu_launch_tiles(const mu_
 
 template <int MODE> static void mu_launch_product(mu_args &a, hipStream_t st)
 {
-    const mu_plan p = mu_lay_out(a, MODE, a.jobs, a.exact);
-    mu_tiles(a, MODE <= MU_SYM, a.jobs, p.T, a.start);
+    const mu_plan p = mu_lay_out(a, MODE);
+    mu_tiles(a, MODE <= MU_SYM, p.T, a.start);
     a.direct = p.direct, a.splits = p.splits;
     if (p.T == 256) mu_launch_tiles<256, 2, 4, MODE>(a, p, st);
     else if (p.T == 128) mu_launch_tiles<128, 2, 4, MODE>(a, p, st);
     else mu_launch_tiles<64, 2, 2, MODE>(a, p, st);
 }
 
-// How many steps a block takes.  It is longer than one where X is longer than wide (from 1.3 on it saves a tenth and more of the
-// products) and large (below, its launches cost more than that), and as long as the result's type allows.  What a block of n
-// steps loses: A is carried from step to step instead of being formed anew, and its rounding errors in the directions of small
-// singular values, 2^-24 of the largest, grow by a^2 a step; with (3.4445, -4.775, 2.0315) that is at most a^(2 n - 2) 2^-24,
-// which has to stay below half a step of the result (5 steps for bfloat16: measured 2e-4 at the worst, of 1.7e-3 that the rounding
-// of the result makes; 4 for float16).  Float32 takes two steps at the beginning, where that is measured to lose nothing
-// (1.6e-6 against 1.6e-6, 2.1e-6 against 2.1e-6), and single ones from there on (two blocks of two: 1.2 to 2 times the error).
-// Where all results are 16-bit the matrices of such blocks are kept as halves only (2^-22 of an entry, far below the result's
-// rounding; 8 x 1024 x 2048, with the shared launches: 1.07 -> 1.00 ms).  Single steps keep float32: what they give is the
-// float32 result, rounded.
-static void mu_blocks(mu_args &g)
-{
-    double square = 0.0, wide = 0.0;
-    int most = MU_BLOCK_STEPS;
-    bool exact = false;
-    const double a2 = fabs((double)g.a) > 1.0 ? 2.0 * log2(fabs((double)g.a)) : 0.0;
-    for (int k = 0; k < g.n_items; ++k) {
-        const mu_item &it = g.it[k];
-        square += (double)it.count * it.np * it.np * it.np, wide += (double)it.count * it.np * it.np * it.lp;
-        const double spare = it.p_type == LRB_BF16 ? 16.0 : it.p_type == LRB_F16 ? 13.0 : 0.0; // log2 of half a step over 2^-24
-        const int n = a2 > 0.0 ? 1 + (int)fmin(spare / a2, 30.0) : MU_BLOCK_STEPS;
-        exact |= it.p_type == LRB_F32;
-        most = most < n ? most : n;
-    }
-    g.exact = 1;
-    if (wide < 1.3 * square || wide < 5e8) return;
-    g.exact = exact;
-    int left = g.steps;
-    g.n_sizes = 0;
-    while (left > 0) {
-        const int n = g.exact ? (g.n_sizes == 0 ? 2 : 1) : most;
-        g.sizes[g.n_sizes++] = (uint8_t)(n < left ? n : left);
-        left -= n;
-    }
-}
-
-// Launches the operations of an iteration, and says which of the four n x n buffers hold what.
+// Launches the operations of an iteration.
 struct mu_launcher {
     mu_args &g;
     hipStream_t st;
-    mu_chain chain;
-    float factors[MU_OPS * MU_COEF];
-    int op = 0, A = 0, P = 1, S = 1, C = 2, was = 1; // was: the buffer of the sum before, which a sum of the same launch reads
-    mu_launcher(mu_args &args, hipStream_t stream) : g(args), st(stream), chain(g.a, g.b, g.c, 1.0, factors) { mu_walk(g.sizes, g.n_sizes, chain); }
-    mu_launcher(const mu_launcher &) = delete;
-    int unused(int x, int y, int z, int w) const // the least buffer that is none of these
+    template <int MODE> void launch()
     {
-        int b = 0;
-        while (b == x || b == y || b == z || b == w) ++b;
-        return b;
-    }
-    template <int MODE> void launch(int u, int v, int old, int old2, int out, bool keep = true)
-    {
-        add(u, v, old, old2, out, keep);
+        memcpy(g.k, g.std + g.op * MU_COEF, sizeof(g.k));
         mu_launch_product<MODE>(g, st);
-        g.jobs = 0;
+        ++g.op;
     }
-    void add(int u, int v, int old, int old2, int out, bool keep) // one more operation of the next launch
+    void gram() { launch<MU_GRAM>(); }
+    void poly() { launch<MU_SYM>(); }
+    void apply(bool last)
     {
-        mu_job &j = g.job[g.jobs++];
-        j.op = op;
-        memcpy(j.k, factors + op++ * MU_COEF, sizeof(j.k));
-        j.u = u, j.v = v, j.old = old, j.old2 = old2, j.out = out, j.keep = keep;
-    }
-    void gram()
-    {
-        A = 0;
-        launch<MU_GRAM>(0, 0, -1, -1, A);
-    }
-    void poly(int k, int n)
-    {
-        P = k ? unused(A, S, S, S) : 1;
-        launch<MU_SYM>(A, A, A, -1, P, n > 1); // of a single step's it is a factor only
-        if (k == 0) S = was = P;
-    }
-    void sum(int k, int n)
-    {
-        const int to = unused(A, P, S, S);
-        if (k + 1 < n) add(P, S, S, P, to, true); // with the turn that follows
-        else launch<MU_SYM>(P, S, S, P, to, false);
-        was = S, S = to;
-    }
-    void turn()
-    {
-        C = unused(A, P, S, was);
-        launch<MU_SYM>(P, A, A, -1, C);
-    }
-    void turn2() { launch<MU_SYM>(C, P, C, -1, A); }
-    void apply(int, bool last)
-    {
-        if (last) launch<MU_LAST>(S, 0, -1, -1, 0);
-        else launch<MU_APPLY>(S, 0, -1, -1, 0);
+        if (last) launch<MU_LAST>();
+        else launch<MU_APPLY>();
         g.flip ^= 1;
     }
 };
 
 // A run of items (or of some matrices of one) that fits the descriptors and MU_WS_MOST bytes, and what it takes.
-#define MU_BUFFERS 5 // n x n, of each matrix
 #define MU_WS_MOST (4ull << 30)
 #define MU_MATS_MOST 4096
 struct mu_group {
@@ -1369,16 +1211,15 @@ struct mu_group {
     // sizes of what lies behind the planes
     uint64_t x0_bytes() const { return ((uint64_t)mats * 16 + 255) / 256 * 256; }
     uint64_t sums_bytes() const { return ((uint64_t)tiles * 8 + 255) / 256 * 256; }
-    uint64_t table_bytes() const { return ((uint64_t)mats * MU_OPS * MU_COEF * 4 + 255) / 256 * 256; }
+    uint64_t table_bytes() const { return ((uint64_t)mats * MU_STEPS * MU_OPS * MU_COEF * 4 + 255) / 256 * 256; }
     uint64_t bytes() const
     {
         if (lds) return 0;
         uint64_t parts = 0;
-        for (int mode = MU_GRAM; mode <= MU_LAST; ++mode)
-            for (int jobs = 1; jobs <= (mode == MU_SYM ? 2 : 1); ++jobs) {
-                const uint64_t b = mu_lay_out(a, mode, jobs, false).part_bytes(), e = mu_lay_out(a, mode, jobs, true).part_bytes();
-                parts = b > parts ? b : parts, parts = e > parts ? e : parts;
-            }
+        for (int mode = MU_GRAM; mode <= MU_LAST; ++mode) {
+            const uint64_t b = mu_lay_out(a, mode).part_bytes();
+            parts = b > parts ? b : parts;
+        }
         return planes + parts + x0_bytes() + sums_bytes() + table_bytes();
     }
 };
@@ -1401,7 +1242,7 @@ template <typename F> static int mu_each_group(const lrb_muon_item *items, int n
             const int lds = mu_small_bytes(it.n, it.l);
             if ((lds != 0) != (small != 0)) continue;
             it.np = (it.n + 63) / 64 * 64, it.lp = (it.l + 63) / 64 * 64;
-            it.step = mu_bytes(it, MU_BUFFERS);
+            it.step = mu_bytes(it);
             for (int d = 0; d < 3; ++d) {
                 const int from = d && turned ? 3 - d : d;
                 it.ps[d] = s.p_stride[from], it.gs[d] = s.g_stride[from], it.ms[d] = s.m_stride[from];
@@ -1500,20 +1341,16 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
     lrb_on_device on(device);
     HIP_TRY(on.err);
     hipStream_t st = (hipStream_t)stream;
-    float std[MU_STEPS * 3 * MU_COEF] = {};
-    uint8_t ones[MU_STEPS];
-    memset(ones, 1, sizeof(ones));
+    float std[MU_STEPS * MU_OPS * MU_COEF] = {};
     mu_chain chain(a, b, c, 1.0, std);
     const double sx = chain.sx;
-    mu_walk(ones, steps, chain);
+    mu_walk(steps, chain);
     try {
         return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
             mu_args &g = gr.a;
             g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
             g.sx = sx;
             memcpy(g.std, std, sizeof(std));
-            memcpy(g.sizes, ones, sizeof(ones));
-            g.n_sizes = steps;
             if (gr.lds) {
                 // (a bit a device, set behind the call: a thread that finds it may launch)
                 static std::atomic<uint64_t> raised{0};
@@ -1532,12 +1369,11 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
             g.part = (double *)at, at += gr.sums_bytes();
             g.table = (float *)at, at += gr.table_bytes();
             g.parts = (float *)at;
-            mu_blocks(g);
             hipLaunchKernelGGL(mu_momentum_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
             hipLaunchKernelGGL(mu_table_kernel, dim3(gr.mats), dim3(256), 0, st, g);
             hipLaunchKernelGGL(mu_split_kernel, dim3((unsigned)gr.tiles), dim3(256), 0, st, g);
-            mu_launcher launcher(g, st);
-            mu_walk(g.sizes, g.n_sizes, launcher);
+            mu_launcher launcher{g, st};
+            mu_walk(steps, launcher);
             HIP_TRY(hipGetLastError());
             return LRB_OK;
         });

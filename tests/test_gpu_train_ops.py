@@ -667,3 +667,18 @@ def test_muon_step_in_blocks_of_steps_on_weights_of_two_types():
         p, g, m = weights(shapes, [TYPES[k] for k in kinds])
         check_muon(p, g, m)
         check_muon(p, g, None)
+
+
+# long enough that A could be carried over several steps: it is formed anew for each, whatever the result's type
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", [(700, 2100), (1500, 600), (7, 1000, 2100), (90, 130), (300, 200)])
+def test_a_16_bit_result_is_the_float32_result_rounded(shape, kind):
+    t = TYPES[kind]
+    g = gradient_like(*shape[-2:], torch.Generator().manual_seed(3), "cuda", shape[:-2]).to(t)
+    for steps in (2, 5):
+        assert torch.equal(train_ops.orthogonalize(g, steps=steps), train_ops.orthogonalize(g.float(), steps=steps).to(t))
+    p, m = torch.randn(*shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(t), g.float()
+    q, n = p.float(), m.clone()
+    train_ops.muon_step([p], [g], [m], lr=0.1)
+    train_ops.muon_step([q], [g.float()], [n], lr=0.1)
+    assert torch.equal(p, q.to(t)) and torch.equal(m, n)
