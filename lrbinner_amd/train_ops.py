@@ -264,6 +264,23 @@ def _muon_call(device, items, momentum, nesterov, steps, coefficients, eps):
                                            a, b, c, eps, ws.data_ptr() if ws_bytes else None, ws_bytes))
 
 
+def _muon_items(params, grads, momenta, lr, decay, scale):
+    """The C ABI's items, and the tensors whose memory they point at: these have to live until the launches are made."""
+    items, held = [], []
+    for p, g, m in zip(params, grads, momenta):
+        if not p.numel():
+            continue
+        p3, m3 = _stack(p, "params"), None if m is None else _stack(m, "momenta")
+        g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "grads")  # a copy where the leading axes ask for one
+        held += [p3, g3, m3]
+        count, rows, cols = p3.shape
+        by = math.sqrt(max(1.0, rows / cols)) if scale is None else scale
+        items.append(_ITEM.pack(p3.data_ptr(), g3.data_ptr(), 0 if m is None else m3.data_ptr(), *p3.stride(), *g3.stride(),
+                                *((0, 0, 0) if m is None else m3.stride()), count, rows, cols, _TYPES[p.dtype], _TYPES[g.dtype],
+                                0 if m is None else _TYPES[m.dtype], -lr * by, decay, 0))
+    return items, held
+
+
 def _orthogonal_plain(u, steps, coefficients, eps):
     """In float32, whatever u's type; u: [..., rows, columns]."""
     a, b, c = coefficients
@@ -369,19 +386,10 @@ def muon_step(params, grads, momenta=None, *, lr, momentum=0.95, nesterov=True, 
             by = math.sqrt(max(1.0, p.shape[-2] / p.shape[-1])) if scale is None else scale
             p.copy_(decay * p.float() - lr * by * _orthogonal_plain(u, steps, coefficients, eps))
         return
-    items = []
-    for p, g, m in zip(params, grads, momenta):
-        if not p.numel():
-            continue
-        p3, m3 = _stack(p, "params"), None if m is None else _stack(m, "momenta")
-        g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "grads")
-        count, rows, cols = p3.shape
-        by = math.sqrt(max(1.0, rows / cols)) if scale is None else scale
-        items.append(_ITEM.pack(p3.data_ptr(), g3.data_ptr(), 0 if m is None else m3.data_ptr(), *p3.stride(), *g3.stride(),
-                                *((0, 0, 0) if m is None else m3.stride()), count, rows, cols, _TYPES[p.dtype], _TYPES[g.dtype],
-                                0 if m is None else _TYPES[m.dtype], -lr * by, decay, 0))
+    items, held = _muon_items(params, grads, momenta, lr, decay, scale)
     if items:
         _muon_call(device, items, momentum, nesterov, steps, coefficients, eps)
+    del held  # (its memory is the stream's: what takes it next runs behind the launches)
     torch.autograd.graph.increment_version([t for t in params + momenta if t is not None])
 
 

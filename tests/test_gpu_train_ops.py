@@ -682,3 +682,16 @@ def test_a_16_bit_result_is_the_float32_result_rounded(shape, kind):
     train_ops.muon_step([p], [g], [m], lr=0.1)
     train_ops.muon_step([q], [g.float()], [n], lr=0.1)
     assert torch.equal(p, q.to(t)) and torch.equal(m, n)
+
+
+def test_muon_step_on_gradients_that_are_copied():
+    gen = torch.Generator().manual_seed(6)
+    grads = [gradient_like(20, 30, gen, "cuda", (3, 4)).transpose(0, 1) for _ in range(4)]
+    grads += [gradient_like(200, 300, gen, "cuda", (4, 1)).expand(4, 3, 200, 300) for _ in range(3)]
+    params = [torch.randn(g.shape, generator=gen).cuda() for g in grads]
+    momenta = [torch.zeros(g.shape, device="cuda") for g in grads]
+    others = [[t.clone() for t in x] for x in (params, momenta)]
+    train_ops.muon_step(params, grads, momenta, lr=0.1)
+    train_ops.muon_step(others[0], [g.contiguous() for g in grads], others[1], lr=0.1)
+    for got, want in zip((params, momenta), others):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -298,3 +298,24 @@ def test_views_with_their_sign_turned():
         train_ops.orthogonalize(g, out=torch._neg_view(torch.zeros(6, 9)))
     with pytest.raises(ValueError):
         train_ops.muon_step([torch._neg_view(torch.zeros(6, 9))], [g], lr=0.1)
+
+
+def _four_axes(device):
+    """Gradients of one shape whose leading axes cannot be flattened without a copy, and the same ones packed."""
+    gen = torch.Generator().manual_seed(6)
+    grads = [gradient_like(20, 30, gen, device, (3, 4)).transpose(0, 1) for _ in range(4)]
+    grads += [gradient_like(20, 30, gen, device, (4, 1)).expand(4, 3, 20, 30) for _ in range(2)]
+    return grads, [g.contiguous() for g in grads]
+
+
+def test_muon_items_point_at_memory_that_lives():
+    grads, packed = _four_axes("cpu")
+    params = [torch.zeros(4, 3, 20, 30) for _ in grads]
+    items, held = train_ops._muon_items(params, grads, [None] * len(grads), 0.1, 1.0, None)
+    noise = [torch.full((12, 20, 30), 7.0) for _ in range(12)]  # takes what was given back
+    for item, g in zip(items, packed):
+        _, at, _, *strides = train_ops._ITEM.unpack(item)[:9]
+        assert strides[3:6] == [600, 30, 1]
+        there = np.ctypeslib.as_array((C.c_float * g.numel()).from_address(at))
+        assert np.array_equal(there, g.numpy().ravel())
+    del noise, held
