@@ -6,14 +6,18 @@
 //   du  = rstd * (g - mean(g) - hat * mean(g * hat)),  dx = du * du/dx
 //   dw  = sum over rows of dy * hat,  db = sum over rows of dy
 //
-// Bound: memory.  A row is read once and stays in registers between its reductions (the mean first, then the mean of the
-// squared differences: no cancellation of large squares), so a forward pass moves x and y and a backward pass x, dy and dx.
+// Bound: memory.  A row is read once and stays in registers between its reductions, so a forward pass moves x and y and a backward
+// pass x, dy and dx.  The mean comes first, then together the sums of the differences from it and of their squares: the former
+// is what rounding (of the sum, and of 1 / cols) has left out of the mean, and corrects it and the variance.  A row of equal
+// elements has variance 0 and gives b, and a mean far above the deviation costs no more than the mean's last bit.  Elements are
+// divided by `cols` before they are added up: the sum of a row may be beyond float32 where its mean is not.
 // TPR threads take a row, each `C` chunks of 16 bytes; the same thread meets the same columns in every row it visits, so
 // w and b are loaded once per thread and the weight's gradient is summed in registers: one partial row per workgroup is
 // written and a second kernel adds the partial rows in a fixed order (no atomics: the same bits run after run).
 // Everything between load and store is float32.
 // Measured (32,768 x 4096 bfloat16): forward 97 us = 5.5 TB/s, backward 164 us = 4.9 TB/s and 12 us for the join (a copy: 5.1).
 #include <limits.h>
+#include <math.h>
 
 #include "lrb_device.h"
 
@@ -146,7 +150,8 @@ template <int TPR> __device__ __forceinline__ float ln_sum(float v, float *red, 
     return v;
 }
 
-// two sums behind one barrier; `red`: 4 x (TPR / 64) floats
+// Two sums behind one barrier; `red`: 4 x (TPR / 64) floats.  (Where one sum and then two are made of every row, the one has the
+// first quarter of `red` and the two its second half.)
 template <int TPR> __device__ __forceinline__ void ln_sum2(float &v, float &w, float *red, int &flip)
 {
     constexpr int W = TPR < 64 ? TPR : 64;
@@ -173,11 +178,20 @@ template <int TPR> __device__ __forceinline__ void ln_sum2(float &v, float &w, f
     }
 }
 
+// 1 / deviation from the means of the differences from `mean` and of their squares; `mean` is put right.  A NaN stays one, and
+// squares beyond float32 give 0.
+__device__ __forceinline__ float ln_statistics(float off, float squares, float eps, float &mean)
+{
+    mean += off;
+    const float var = squares < INFINITY ? fmaxf(squares - off * off, 0.0f) : squares;
+    return 1.0f / sqrtf(var + eps);
+}
+
 template <typename T, int TPR, int C, bool ACT, int EDGE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_fwd_kernel(ln_args a)
 {
     constexpr int V = ln_vec<T>::V, THREADS = TPR < 256 ? 256 : TPR, RPG = THREADS / TPR;
-    __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
+    __shared__ float red[4 * (TPR > 64 ? TPR / 64 : 1)];
     int flip = 0;
     const int lane = threadIdx.x % TPR, cols = a.cols;
     const float inv = 1.0f / (float)cols;
@@ -219,17 +233,19 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_fwd_kernel(ln_args a
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s += LN_OWN(c, i) ? u[c][i] : 0.0f;
-        const float mean = ln_sum<TPR>(s, red, flip) * inv;
+            for (int i = 0; i < V; ++i) s = fmaf(LN_OWN(c, i) ? u[c][i] : 0.0f, inv, s);
+        float mean = ln_sum<TPR>(s, red, flip), s2 = 0.0f;
         s = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float e = u[c][i] - mean;
-                s += LN_OWN(c, i) ? e * e : 0.0f;
+                s = fmaf(LN_OWN(c, i) ? e : 0.0f, inv, s);
+                s2 += LN_OWN(c, i) ? e * e : 0.0f;
             }
-        const float rstd = 1.0f / sqrtf(ln_sum<TPR>(s, red, flip) * inv + a.eps);
+        ln_sum2<TPR>(s, s2, red, flip);
+        const float rstd = ln_statistics(s, s2 * inv, a.eps, mean);
         if (!live) continue;
         if (a.mean && lane == 0) {
             a.mean[row] = mean;
@@ -386,20 +402,22 @@ template <typename T> __device__ __forceinline__ float ln_w_at(const void *w, in
 
 template <typename T, bool ACT> __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(ln_args a)
 {
-    __shared__ float red[32];
+    __shared__ float red[64];
     int flip = 0;
     const float inv = 1.0f / (float)a.cols;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *x = (const T *)a.x + row * a.x_stride;
         float s = 0.0f, f;
-        for (int c = threadIdx.x; c < a.cols; c += 1024) s += ln_at<T, ACT>(a, x, row, c, f);
-        const float mean = ln_sum<1024>(s, red, flip) * inv;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) s = fmaf(ln_at<T, ACT>(a, x, row, c, f), inv, s);
+        float mean = ln_sum<1024>(s, red, flip), s2 = 0.0f;
         s = 0.0f;
         for (int c = threadIdx.x; c < a.cols; c += 1024) {
             const float e = ln_at<T, ACT>(a, x, row, c, f) - mean;
-            s += e * e;
+            s = fmaf(e, inv, s);
+            s2 += e * e;
         }
-        const float rstd = 1.0f / sqrtf(ln_sum<1024>(s, red, flip) * inv + a.eps);
+        ln_sum2<1024>(s, s2, red, flip);
+        const float rstd = ln_statistics(s, s2 * inv, a.eps, mean);
         if (a.mean && threadIdx.x == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;

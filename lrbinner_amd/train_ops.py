@@ -142,7 +142,8 @@ def _ln_plain(x, weight, bias, keep, eps, slope, keep_scale):
         u = torch.where(u > 0, u, slope * u)
         if keep is not None:
             u = torch.where(keep.bool(), u * keep_scale, torch.zeros_like(u))
-    centred = u - u.mean(-1, keepdim=True)
+    centred = u - (u / u.shape[-1]).sum(-1, keepdim=True)  # (the sum of u may be beyond float32)
+    centred = centred - centred.mean(-1, keepdim=True)  # what rounding has left out of the mean
     y = centred / torch.sqrt((centred * centred).mean(-1, keepdim=True) + eps)
     if weight is not None:
         y = y * weight.float()

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from lrbinner_amd import ae_utils, train_ops
-from train_ops_ref import HALF_STEP, gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
+from train_ops_ref import HALF_STEP, far_row_tolerance, gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
 
 pytestmark = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -695,3 +695,32 @@ def test_muon_step_on_gradients_that_are_copied():
     train_ops.muon_step(others[0], [g.contiguous() for g in grads], others[1], lr=0.1)
     for got, want in zip((params, momenta), others):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# rows in every layout over threads
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("cols", [7, 41, 61, 700, 1000, 4095, 10007, 16385, 20001])
+def test_layer_norm_rows_of_equal_elements(cols, kind):
+    t = TYPES[kind]
+    x, w, b, dy, keep = inputs(9, cols, t)
+    values = [1.0, 0.1, 1e3, 1e5 if kind != "f16" else 6e4, -7.7]
+    for r, v in enumerate(values):
+        x[r + 2] = v
+    y = train_ops.layer_norm(x, w, b)
+    for r in range(len(values)):  # no variance: what is left is the bias
+        assert torch.equal(y[r + 2], b.to(t)), values[r]
+    if kind != "f16":
+        x[4] = 3e34
+        assert torch.equal(train_ops.layer_norm(x, w, b)[4], b.to(t))
+    # ... and of the activation's rows
+    y = train_ops.layer_norm(x[2:4], w, b, slope=0.01, keep=keep[2:4] | True, keep_scale=1.25)
+    assert torch.equal(y, b.to(t).expand(2, cols))
+
+
+@pytest.mark.parametrize("cols", [61, 700, 4095, 10007, 16385, 20001])
+def test_layer_norm_rows_far_from_zero(cols):
+    x, w, b, dy, _ = inputs(6, cols, torch.float32)
+    x += torch.tensor([[0.0], [1e3], [-1e4], [1e5], [3e6], [-1e7]], device="cuda")
+    c = x.double() - x.double().mean(1, keepdim=True)
+    want = c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-5) * w.double() + b.double()
+    within(train_ops.layer_norm(x, w, b), want, far_row_tolerance(x, w, 1e-5) + 2.0 ** -24 * want.abs())

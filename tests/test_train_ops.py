@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lrbinner_amd import _lib, ae_utils, train_ops
-from train_ops_ref import gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
+from train_ops_ref import far_row_tolerance, gradient_like, matrices_within, norm_ref, orthogonal_ref, orthogonal_tolerance, within
 
 
 def make(rows, cols, seed=0, dtype=torch.float32):
@@ -319,3 +319,17 @@ def test_muon_items_point_at_memory_that_lives():
         there = np.ctypeslib.as_array((C.c_float * g.numel()).from_address(at))
         assert np.array_equal(there, g.numpy().ravel())
     del noise, held
+
+
+def test_rows_far_from_zero():
+    for cols in (41, 61, 1000, 4095):
+        for value in (1.0, 0.1, 1e3, 1e5, -3e34, 3e38):
+            x, w, b, _, _ = make(3, cols)
+            x[1] = value  # no variance: what is left is the bias
+            assert torch.equal(train_ops.layer_norm(x, w, b)[1], b)
+    x, w, b, _, _ = make(5, 700)
+    x += torch.tensor([[0.0], [1e3], [-1e4], [1e5], [3e6]])
+    y = train_ops.layer_norm(x, w, b)
+    c = x.double() - x.double().mean(1, keepdim=True)
+    want = c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-5) * w.double() + b.double()
+    within(y, want, far_row_tolerance(x, w, 1e-5) + 2.0 ** -24 * want.abs())

@@ -125,3 +125,27 @@ def matrices_within(got, want, tol, half_step=0.0, what=""):
     off = torch.linalg.vector_norm(got.double() - want, dim=(-2, -1))
     most = tol + 1.1 * half_step * torch.linalg.vector_norm(want, dim=(-2, -1)) + math.sqrt(want.shape[-1] * want.shape[-2]) * 6e-8 * (half_step > 2.0 ** -20)
     assert bool((off <= most).all()), f"{what}: off by {float((off / most).max()):.3g} times the tolerance"
+
+
+def far_row_tolerance(x, w, eps):
+    """Of y for float32 rows whose mean may lie far above their deviation, up to 20,001 columns.
+
+    The mean of the first pass is off by at most gamma |u| on average (48 + cols / 1024 roundings, as above), which every
+    difference from it carries.  The mean of these differences, gamma of their own size off, is added, and the mean rounded: it is
+    then off by U |mean| + gamma mean |u - first mean|.  The differences of the second pass are float32 numbers, off by U of
+    themselves; the variance is (3 + cols / 1024) gamma-like roundings of the mean square of the first pass's differences, of which
+    the square of the first mean's error is taken off again."""
+    x = x.detach().double()
+    gamma = (48 + x.shape[-1] / 1024) * U
+    mean = x.mean(-1, keepdim=True)
+    c = x - mean
+    first = gamma * x.abs().mean(-1, keepdim=True)        # error of the first mean
+    d_mean = U * (mean.abs() + first) + gamma * (c.abs().mean(-1, keepdim=True) + first)
+    var = c.square().mean(-1, keepdim=True)
+    d_var = 3 * gamma * (var + first ** 2) + d_mean ** 2
+    rstd = 1 / torch.sqrt(var + eps)
+    # 1 / sqrt falls the fastest at its lower end
+    low = torch.rsqrt((var - d_var).clamp_min(0) + eps)
+    d_rstd = low - rstd + 4 * U * low
+    d_hat = low * d_mean + (c.abs() + d_mean) * d_rstd + 4 * U * (c.abs() + d_mean) * low
+    return 1.1 * (w.detach().double().abs() * d_hat) + 4 * U * (c * rstd * w.double()).abs() + 1e-30
