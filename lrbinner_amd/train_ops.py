@@ -8,7 +8,8 @@ of weights (momentum, iteration and update in shared launches), and ``Muon`` is 
 On the GPU the arithmetic is csrc/lrb_norm.hip and csrc/lrb_muon.hip behind the C ABI of include/lrb_hip.h; calls go to
 torch's current stream of the tensors' device, their workspace comes from torch's allocator (so calls may be captured in a
 HIP graph; a captured backward pass, as any of torch's, wants leaves that no living eager graph holds), and there is no
-fallback where the library is missing.  On CPU tensors the same definitions run as torch
+fallback where the library is missing.  Launches on addresses are nothing that torch.jit.trace, make_fx or forward-mode
+gradients could follow: under these a call raises RuntimeError.  On CPU tensors the same definitions run as torch
 operations, as the network itself does without ``--cuda``.
 
 Float32, bfloat16 and float16; what is summed is summed in float32 or more, and results are rounded once."""
@@ -17,6 +18,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -30,6 +32,26 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 # hipStream_t of torch's current stream on a device, by its index (a call of torch.cuda.current_stream costs a small
 # operator as much as its launch)
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
+_key_included, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+
+
+def _has_proxy_mode():
+    """Whether make_fx or torch.export is at work.  (Asked only where some mode is: its module takes long to import.)"""
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
+
+
+def _refuse_unseen(name, *tensors):
+    """Raises where torch records or differentiates, by the operations it sees, what is about to be launched unseen."""
+    if torch.compiler.is_dynamo_compiling():  # torch.compile steps aside for the launch by itself
+        return
+    if _tracing_state() is not None or (_dispatch_modes() or _key_included(_PRE_DISPATCH)) and _has_proxy_mode():
+        raise RuntimeError(f"{name}: a call on the GPU cannot be traced (its kernels would not be in the trace)")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name}: forward-mode gradients are not given on the GPU")
 
 
 def _known_type(t, name):
@@ -193,6 +215,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, slope=1.0, keep=None, kee
         keep_scale = 1.0
     if not x.is_cuda:
         return _ln_plain(x, weight, bias, keep, eps, slope, keep_scale)
+    _refuse_unseen("layer_norm", x, weight, bias)
     if grad and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, keep, eps, slope, keep_scale)
     return _ln_forward(x, weight, bias, keep, eps, slope, keep_scale, False)[0]
@@ -323,6 +346,7 @@ def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     g = g.resolve_neg()
     if not g.is_cuda:
         return out.copy_(_orthogonal_plain(g, steps, coefficients, eps))
+    _refuse_unseen("orthogonalize", g, out)
     if out.data_ptr() != g.data_ptr() or out.stride() != g.stride() or out.dtype != g.dtype:
         (g0, g1), (o0, o1) = _extent(g), _extent(out)
         if g0 < o1 and o0 < g1:  # a matrix of out may lie over another matrix of g
@@ -387,6 +411,7 @@ def muon_step(params, grads, momenta=None, *, lr, momentum=0.95, nesterov=True, 
             by = math.sqrt(max(1.0, p.shape[-2] / p.shape[-1])) if scale is None else scale
             p.copy_(decay * p.float() - lr * by * _orthogonal_plain(u, steps, coefficients, eps))
         return
+    _refuse_unseen("muon_step", *params, *grads, *momenta)
     items, held = _muon_items(params, grads, momenta, lr, decay, scale)
     if items:
         _muon_call(device, items, momentum, nesterov, steps, coefficients, eps)

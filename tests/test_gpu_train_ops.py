@@ -724,3 +724,54 @@ def test_layer_norm_rows_far_from_zero(cols):
     c = x.double() - x.double().mean(1, keepdim=True)
     want = c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-5) * w.double() + b.double()
     within(train_ops.layer_norm(x, w, b), want, far_row_tolerance(x, w, 1e-5) + 2.0 ** -24 * want.abs())
+
+
+def test_what_torch_would_not_see_is_refused():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, _, _ = inputs(6, 20, torch.float32)
+    m = train_ops.LayerNorm(20, device="cuda")
+
+    def step(v):
+        p = torch.zeros_like(v)
+        train_ops.muon_step([p], [v], lr=0.1)
+        return p
+
+    calls = (lambda v: train_ops.layer_norm(v, w, b), m, lambda v: train_ops.orthogonalize(v), step)
+    for call in calls:
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(RuntimeError, match="traced"):
+                    torch.jit.trace(call, (x,))
+                for more in ({}, dict(pre_dispatch=True)):
+                    with pytest.raises(RuntimeError, match="traced"):
+                        make_fx(call, **more)(x)
+                with forward_ad.dual_level():
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(forward_ad.make_dual(x, torch.ones_like(x)))
+                with pytest.raises(RuntimeError):
+                    torch.func.vmap(call)(x.unsqueeze(0))
+                with pytest.raises(RuntimeError):
+                    torch.func.jvp(call, (x,), (x,))
+                call(x)
+    with torch.no_grad(), forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            train_ops.layer_norm(x, forward_ad.make_dual(w, torch.ones_like(w)), b)
+        assert torch.equal(train_ops.layer_norm(x, w, b), calls[0](x))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_layer_norm_in_a_compiled_function(grad):
+    x, w, b, dy, _ = inputs(6, 20, torch.float32)
+    leaves = [t.requires_grad_(grad) for t in (x, w, b)]
+    compiled = torch.compile(lambda *a: train_ops.layer_norm(*a) * 2, backend="eager")
+    want = train_ops.layer_norm(*leaves) * 2
+    for _ in range(2):
+        got = compiled(*leaves)
+        assert torch.equal(got, want)
+        if grad:
+            for g, e in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy, retain_graph=True)):
+                assert torch.equal(g, e)
+    turned = torch.compile(lambda v: train_ops.orthogonalize(v) * 2, backend="eager")
+    for _ in range(2):
+        assert torch.equal(turned(x), train_ops.orthogonalize(x) * 2)

@@ -333,3 +333,33 @@ def test_rows_far_from_zero():
     c = x.double() - x.double().mean(1, keepdim=True)
     want = c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-5) * w.double() + b.double()
     within(y, want, far_row_tolerance(x, w, 1e-5) + 2.0 ** -24 * want.abs())
+
+
+def test_what_torch_would_not_see_is_refused():
+    """(What a call on the GPU asks before its launch; on the CPU torch sees everything.)"""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(3, 4)
+
+    def asks(v):
+        train_ops._refuse_unseen("layer_norm", v, None)
+        return v + 1
+
+    asks(x)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(asks, (x,))
+    for more in ({}, dict(tracing_mode="fake"), dict(tracing_mode="symbolic"), dict(pre_dispatch=True)):
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(asks, **more)(x)
+    with forward_ad.dual_level():
+        asks(x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            asks(forward_ad.make_dual(x, torch.ones_like(x)))
+    asks(x)
+    # the CPU's forms can be traced, and have forward-mode gradients
+    m = train_ops.LayerNorm(4, slope=0.1)
+    with torch.no_grad():
+        traced, other = torch.jit.trace(m, (x,)), torch.randn(3, 4)
+        assert torch.allclose(traced(other), m(other)) and torch.allclose(make_fx(m)(x)(other), m(other))
+    with forward_ad.dual_level():
+        assert forward_ad.unpack_dual(m(forward_ad.make_dual(x, torch.ones_like(x)))).tangent is not None
