@@ -19,7 +19,6 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, check
@@ -140,7 +139,25 @@ def _ln_backward(ctx, dy):
     return dx, dw, db, None, None, None, None
 
 
-_ln_backward_of_a_graph = once_differentiable(_ln_backward)  # refuses a second derivative
+class _Once(torch.autograd.Function):
+    """The first `count` tensors, as functions of all of them that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tensors[:count]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("layer_norm: second derivatives are not given on the GPU")
+
+
+def _ln_backward_of_a_graph(ctx, dy):
+    # (torch's once_differentiable looks at dy alone: the gradient of a sum, say, would pass for a constant)
+    with torch.no_grad():
+        grads = _ln_backward(ctx, dy)
+    given = [g for g in grads if g is not None]
+    given = iter(_Once.apply(len(given), *given, dy, *ctx.saved_tensors[:2]))
+    return tuple(None if g is None else next(given) for g in grads)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -153,8 +170,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        # gradients are enabled here only where a graph of the backward pass is asked for (the wrapper costs a small operator
-        # 5 us of a hundred)
+        # gradients are enabled here only where a graph of the backward pass is asked for
         return _ln_backward_of_a_graph(ctx, dy) if torch.is_grad_enabled() else _ln_backward(ctx, dy)
 
 
@@ -180,7 +196,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, slope=1.0, keep=None, kee
     u is x, or with ``slope`` (of a LeakyReLU; 0 a ReLU) or ``keep`` (bool or uint8, of x's shape, a dropout's draw)
     keep * keep_scale * leaky_relu(x); what is dropped counts as 0 whatever it holds.  ``weight`` and ``bias``: one element a
     column, float32 or of x's type (both alike), or None.  x may have any leading axes and strides; a copy is made only
-    where the elements of a row are not side by side, or the rows not evenly spaced.  The statistics are float32."""
+    where the elements of a row are not side by side, or the rows not evenly spaced.  The statistics are float32.  On the GPU the
+    gradients may be asked for with ``create_graph``, but not differentiated: that raises RuntimeError."""
     dtype, shape, device = x.dtype, x.shape, x.device
     if dtype not in _TYPES:
         _known_type(x, "x")

@@ -775,3 +775,21 @@ def test_layer_norm_in_a_compiled_function(grad):
     turned = torch.compile(lambda v: train_ops.orthogonalize(v) * 2, backend="eager")
     for _ in range(2):
         assert torch.equal(turned(x), train_ops.orthogonalize(x) * 2)
+
+
+def test_a_penalty_on_the_gradient_is_refused():
+    x, w, b, dy, _ = inputs(6, 20, torch.float32)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    plain = torch.autograd.grad(train_ops.layer_norm(*leaves).square().sum(), leaves)
+    for of in ((x,), (w,), leaves):
+        y = train_ops.layer_norm(*leaves)
+        grads = torch.autograd.grad(y.sum(), of, create_graph=True)  # (the gradient of a sum depends on no leaf)
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            (y.sum() + sum(g.square().sum() for g in grads)).backward()
+    # a graph of the backward pass that nobody differentiates costs nothing but itself
+    y = train_ops.layer_norm(*leaves)
+    grads = torch.autograd.grad(y.square().sum(), leaves, create_graph=True)
+    for g, e in zip(grads, plain):
+        assert torch.equal(g, e)
+    only = torch.autograd.grad(train_ops.layer_norm(x.detach(), w.detach(), b).sum(), b, create_graph=True)[0]
+    assert torch.equal(only, torch.full_like(b, 6.0)) and not only.requires_grad
