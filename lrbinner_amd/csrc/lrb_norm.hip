@@ -127,8 +127,12 @@ __device__ __forceinline__ void ln_load_keep(const uint8_t *__restrict__ p, ln_c
     }
 }
 
-// u of the block's activation; k: keep_scale or 0
-__device__ __forceinline__ float ln_act(float x, float slope, float k) { return k == 0.0f ? 0.0f : x * (x > 0.0f ? k : slope * k); }
+// u of the block's activation; k: keep_scale or 0.  With slope 0 what is below 0 gives 0, -inf among it.
+__device__ __forceinline__ float ln_act(float x, float slope, float k)
+{
+    const float f = x > 0.0f ? k : slope * k;
+    return k == 0.0f || (f == 0.0f && x < 0.0f) ? 0.0f : x * f;
+}
 
 // The sum over the TPR threads of a row, in every one of them.  `red`: 2 x (TPR / 64) floats of the workgroup, used in turn
 // (`flip`) so that one barrier a reduction is enough.

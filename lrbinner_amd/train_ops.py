@@ -177,7 +177,7 @@ class _LayerNorm(torch.autograd.Function):
 def _ln_plain(x, weight, bias, keep, eps, slope, keep_scale):
     u = x.float()
     if keep is not None or slope != 1.0:
-        u = torch.where(u > 0, u, slope * u)
+        u = torch.relu(u) if slope == 0.0 else torch.where(u > 0, u, slope * u)  # (0 times -inf is no 0)
         if keep is not None:
             u = torch.where(keep.bool(), u * keep_scale, torch.zeros_like(u))
     centred = u - (u / u.shape[-1]).sum(-1, keepdim=True)  # (the sum of u may be beyond float32)

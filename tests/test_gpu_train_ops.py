@@ -793,3 +793,21 @@ def test_a_penalty_on_the_gradient_is_refused():
         assert torch.equal(g, e)
     only = torch.autograd.grad(train_ops.layer_norm(x.detach(), w.detach(), b).sum(), b, create_graph=True)[0]
     assert torch.equal(only, torch.full_like(b, 6.0)) and not only.requires_grad
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("cols", [3, 40, 700, 9000, 18000])
+def test_slope_0_is_a_relu(cols, kind):
+    x, w, b, dy, keep = inputs(5, cols, TYPES[kind])
+    x[1, 1], x[2, 2], x[3, 0] = -math.inf, math.nan, -0.0
+    live = [0, 1, 3, 4]
+    for more in ({}, dict(keep=keep, keep_scale=1.25)):
+        y, dx = both_passes(x, w, b, dy, slope=0.0, **more)[:2]
+        # (not the bits of a call on relu(x) without slope: another instance of the kernel, whose float32 operations may be
+        # fused otherwise.  The tolerances hold for both.)
+        part = {k: v[live] if k == "keep" else v for k, v in more.items()}
+        want, tol = norm_ref(torch.relu(x[live]), w, b, 1e-5, dy[live], **part)
+        within(y[live], want[0], tol[0], "y")
+        above = (x[live] > 0).double()
+        within(dx[live], want[1] * above, tol[1] * above, "dx")
+        assert "keep" in more or bool(y[2].isnan().all())

@@ -363,3 +363,12 @@ def test_what_torch_would_not_see_is_refused():
         assert torch.allclose(traced(other), m(other)) and torch.allclose(make_fx(m)(x)(other), m(other))
     with forward_ad.dual_level():
         assert forward_ad.unpack_dual(m(forward_ad.make_dual(x, torch.ones_like(x)))).tangent is not None
+
+
+def test_slope_0_is_a_relu():
+    x, w, b, dy, keep = make(5, 40)
+    x[1, 3], x[2, 7], x[3, 9] = -math.inf, math.nan, -0.0
+    y = train_ops.layer_norm(x, w, b, slope=0.0)
+    want = train_ops.layer_norm(torch.relu(x), w, b)
+    assert torch.equal(y.nan_to_num(77.0), want.nan_to_num(77.0))
+    assert bool(y[2].isnan().all()) and bool(torch.isfinite(y[[0, 1, 3, 4]]).all())
