@@ -585,7 +585,7 @@ typedef struct {
 #define LRB_MUON_DIVERGED 64.0
 double lrb_muon_bound(int steps, float a, float b, float c);
 uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items);
-int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items, int n_items, float momentum, int nesterov, int steps,
+int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items, int n_items, double momentum, int nesterov, int steps,
                  float a, float b, float c, float eps, void *d_ws, uint64_t ws_bytes);
 
 /* ---- host side: ingest and profile text -------------------------------- */

@@ -147,7 +147,7 @@ PROTOTYPES = {
                                          vp, C.c_float, vp, C.c_float, vp, vp, vp, vp, C.c_uint64]),
     "lrb_muon_bound": (C.c_double, [C.c_int, C.c_float, C.c_float, C.c_float]),
     "lrb_muon_ws_bytes": (C.c_uint64, [vp, C.c_int]),
-    "lrb_muon_dev": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_float, C.c_int, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float, vp,
+    "lrb_muon_dev": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_double, C.c_int, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float, vp,
                                C.c_uint64]),
     "lrb_vae_debug_read": (C.c_int, [vp, C.c_int, C.POINTER(C.c_float), C.c_uint64]),
     "lrb_reader_open": (C.c_int, [C.c_char_p, C.POINTER(vp)]),

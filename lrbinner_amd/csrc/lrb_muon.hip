@@ -66,7 +66,8 @@ struct mu_args {
     float *table;   // [matrices][steps][MU_OPS][MU_COEF]
     double *part;   // [tiles of 64 x 64 of all matrices] sums of squares
     int n_items, steps;
-    float beta, eps, a, b, c;
+    float beta, rest; // the momentum, and 1 - momentum rounded by itself: 1 - beta of 0.999 would be off by 1e-5 of it
+    float eps, a, b, c;
     int nesterov;
     int flip;       // which of the two copies of X is read
     int op;         // the operation of this launch, counted through the steps, and its factors for a norm of at least eps
@@ -174,7 +175,7 @@ __device__ __forceinline__ void mu_write(T *p, long long at, long long piece, lo
 // u in R pieces of four along the side on which g is contiguous: piece r lies in line `line(r)` of the other side, from `at` on.
 // UPDATE also writes the momentum back (each entry by one thread); u is made of what is kept.
 template <bool UPDATE, int R, typename L>
-__device__ __forceinline__ void mu_u(float beta, int nesterov, const mu_item &it, int mat, bool along_j, L line, int at, float (&u)[4 * R])
+__device__ __forceinline__ void mu_u(float beta, float rest, int nesterov, const mu_item &it, int mat, bool along_j, L line, int at, float (&u)[4 * R])
 {
     const int lines = along_j ? it.n : it.l, len = along_j ? it.l : it.n;
     const long long g_fast = along_j ? it.gs[2] : it.gs[1], g_slow = along_j ? it.gs[1] : it.gs[2];
@@ -188,13 +189,13 @@ __device__ __forceinline__ void mu_u(float beta, int nesterov, const mu_item &it
     mu_read<R>(it.m, it.m_type, m_at, gap * m_slow, m_fast, count, m);
     if (UPDATE) {
 #pragma unroll
-        for (int e = 0; e < 4 * R; ++e) m[e] = beta * m[e] + (1.0f - beta) * u[e];
+        for (int e = 0; e < 4 * R; ++e) m[e] = beta * m[e] + rest * u[e];
         if (it.m_type == LRB_F32) mu_write<float, R>((float *)it.m, m_at, gap * m_slow, m_fast, count, m);
         else if (it.m_type == LRB_BF16) mu_write<__bf16, R>((__bf16 *)it.m, m_at, gap * m_slow, m_fast, count, m);
         else mu_write<mu_h, R>((mu_h *)it.m, m_at, gap * m_slow, m_fast, count, m);
     }
 #pragma unroll
-    for (int e = 0; e < 4 * R; ++e) u[e] = nesterov ? (1.0f - beta) * u[e] + beta * m[e] : m[e];
+    for (int e = 0; e < 4 * R; ++e) u[e] = nesterov ? rest * u[e] + beta * m[e] : m[e];
 }
 
 // v times a double, rounded once or nearly so (to 2^-24 (1 + 2^-23)) without double arithmetic for each entry: the factor is
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256) void mu_momentum_kernel(mu_args a)
     // sixteen threads a line of 64, four lines of a thread 16 apart
     float u[16];
     const int line = (along_j ? i0 : j0) + (threadIdx.x >> 4), at = (along_j ? j0 : i0) + (threadIdx.x & 15) * 4;
-    mu_u<true, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, at, u);
+    mu_u<true, 4>(a.beta, a.rest, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, at, u);
 #pragma unroll
     for (int e = 0; e < 16; ++e) s += (double)u[e] * u[e];
 #pragma unroll
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(256) void mu_split_kernel(mu_args a)
     const mu_factor scale(a.x0[2 * (it.first + mat)]);
     float u[16];
     const int first = threadIdx.x >> 4, x = (threadIdx.x & 15) * 4, line = (along_j ? i0 : j0) + first;
-    mu_u<false, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, (along_j ? j0 : i0) + x, u);
+    mu_u<false, 4>(a.beta, a.rest, a.nesterov, it, mat, along_j, [=](int r) { return line + 16 * r; }, (along_j ? j0 : i0) + x, u);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -935,7 +936,7 @@ __global__ __launch_bounds__(64 * MU_SMALL_WAVES) void mu_small_kernel(mu_args b
     for (int tile = xj; tile < last; tile += groups) {
         const int i0 = xi * 32, j0 = tile * 32, x = lane % 8 * 4, line = (along_j ? i0 : j0) + lane / 8;
         float u[16];
-        mu_u<true, 4>(a.beta, a.nesterov, it, mat, along_j, [=](int r) { return line + 8 * r; }, (along_j ? j0 : i0) + x, u);
+        mu_u<true, 4>(a.beta, a.rest, a.nesterov, it, mat, along_j, [=](int r) { return line + 8 * r; }, (along_j ? j0 : i0) + x, u);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = i0 + (along_j ? 8 * r + lane / 8 : x), j = j0 + (along_j ? x : 8 * r + lane / 8);
@@ -1326,7 +1327,7 @@ extern "C" uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items)
     return most;
 }
 
-extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items, int n_items, float momentum, int nesterov, int steps,
+extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items, int n_items, double momentum, int nesterov, int steps,
                             float a, float b, float c, float eps, void *d_ws, uint64_t ws_bytes)
 {
     ARG_TRY(n_items >= 0 && (n_items == 0 || items != nullptr));
@@ -1348,7 +1349,7 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
     try {
         return mu_each_group(items, n_items, [&](mu_group &gr) -> int {
             mu_args &g = gr.a;
-            g.steps = steps, g.beta = momentum, g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
+            g.steps = steps, g.beta = (float)momentum, g.rest = (float)(1.0 - momentum), g.nesterov = nesterov, g.eps = eps, g.a = a, g.b = b, g.c = c;
             g.sx = sx;
             memcpy(g.std, std, sizeof(std));
             if (gr.lds) {

@@ -811,3 +811,13 @@ def test_slope_0_is_a_relu(cols, kind):
         above = (x[live] > 0).double()
         within(dx[live], want[1] * above, tol[1] * above, "dx")
         assert "keep" in more or bool(y[2].isnan().all())
+
+
+@pytest.mark.parametrize("shape", [(40, 60), (300, 500)])
+@pytest.mark.parametrize("momentum", [0.95, 0.999, 0.9999, 0.0])
+def test_the_share_of_the_gradient_is_exact(shape, momentum):
+    g = gradient_like(*shape, torch.Generator().manual_seed(2), "cuda")
+    p, m = torch.zeros(*shape, device="cuda"), torch.zeros(*shape, device="cuda")
+    train_ops.muon_step([p], [g], [m], lr=0.1, momentum=momentum)
+    # 1 - momentum rounded to float32, and the product; float32's smallest number
+    within(m, (1.0 - momentum) * g.double(), 2.02 * 2.0 ** -24 * (1.0 - momentum) * g.double().abs() + 2.0 ** -149)
