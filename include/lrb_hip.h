@@ -580,8 +580,9 @@ typedef struct {
     float alpha, decay;
     int32_t reserved;
 } lrb_muon_item;
-/* How large a singular value from [0, 1] may become in `steps` steps with these coefficients; LRB_ERR_ARG from lrb_muon_dev
- * where that is more than LRB_MUON_DIVERGED (the factors' 16-bit halves are scaled by this bound). */
+/* How large a singular value from [0, 1] may become in `steps` steps with these coefficients, or one from [0, 1 + 1 / 512],
+ * as large as it is made by roundings, where that is beyond LRB_MUON_DIVERGED; LRB_ERR_ARG from lrb_muon_dev where the answer is more
+ * than LRB_MUON_DIVERGED (the factors' 16-bit halves are scaled by this bound). */
 #define LRB_MUON_DIVERGED 64.0
 double lrb_muon_bound(int steps, float a, float b, float c);
 uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items);

@@ -272,10 +272,11 @@ template <typename V> __host__ __device__ inline void mu_walk(int steps, V &v)
 
 // Writes the factors of every operation: of the old entry, and of the sum of products.  Scales are powers of two, from bounds on
 // the largest singular values.
+#define MU_SLACK (1.0 + 1.0 / 512.0) // for the roundings on the way: the bounds hold for exact factors
 struct mu_chain {
     double a, b, c, r, sx, ra = 0.0, sa = 0.0, sb = 0.0;
     float *t;
-    static constexpr double slack = 1.0 + 1.0 / 512.0; // for the roundings on the way: the bounds hold for exact factors
+    static constexpr double slack = MU_SLACK;
     __host__ __device__ mu_chain(double a_, double b_, double c_, double r_, float *t_) : a(a_), b(b_), c(c_), r(r_ * slack), t(t_) { sx = mu_scale(r); }
     __host__ __device__ void put(double k0, double k1)
     {
@@ -1302,14 +1303,23 @@ static bool mu_items_fit(const lrb_muon_item *items, int n)
     return true;
 }
 
-extern "C" double lrb_muon_bound(int steps, float a, float b, float c)
+static double mu_bound(int steps, double a, double b, double c, double slack)
 {
-    double r = 1.0, most = 1.0;
+    double r = slack, most = 1.0;
     for (int k = 0; k < steps && k < MU_STEPS && r <= 1e9; ++k) {
-        r = mu_largest_odd(a, b, c, r);
+        r = mu_largest_odd(a, b, c, r) * slack;
         most = most >= r ? most : r; // a NaN stays
     }
     return most;
+}
+
+// Where the exact bound is small, but the one with the slack that the factors' scales are made from is not (x^5 keeps 1 where it
+// is, and takes what is beyond it away), a rounding could grow as the latter says, and the scales would leave nothing of a 16-bit
+// factor: then the latter is the answer.
+extern "C" double lrb_muon_bound(int steps, float a, float b, float c)
+{
+    const double exact = mu_bound(steps, a, b, c, 1.0), slack = mu_bound(steps, a, b, c, MU_SLACK);
+    return exact <= LRB_MUON_DIVERGED && !(slack <= LRB_MUON_DIVERGED) ? slack : exact;
 }
 
 extern "C" uint64_t lrb_muon_ws_bytes(const lrb_muon_item *items, int n_items)

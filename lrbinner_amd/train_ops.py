@@ -340,7 +340,8 @@ def _orthogonal_plain(u, steps, coefficients, eps):
 def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     """g / max(|g|_F, eps), then ``steps`` times X <- a X + (b A + c A^2) X with A = X X^T (of a tall matrix X^T X): the
     singular vectors stay, the singular values go towards 1 (with the default coefficients into about 0.7 to 1.2).
-    Coefficients under which a singular value from [0, 1] may grow beyond 64 on the way are refused.
+    Coefficients under which a singular value from [0, 1], or one that rounding has put above 1 by 1 / 512, may grow beyond 64 on
+    the way are refused.
 
     g: [..., rows, columns], any strides; each matrix by itself; one that holds an infinity or a NaN becomes NaN, one of
     zeros stays.  ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are

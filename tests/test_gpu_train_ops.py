@@ -821,3 +821,13 @@ def test_the_share_of_the_gradient_is_exact(shape, momentum):
     train_ops.muon_step([p], [g], [m], lr=0.1, momentum=momentum)
     # 1 - momentum rounded to float32, and the product; float32's smallest number
     within(m, (1.0 - momentum) * g.double(), 2.02 * 2.0 ** -24 * (1.0 - momentum) * g.double().abs() + 2.0 ** -149)
+
+
+# (short sides up to 16: there the tolerance counts how the iteration passes a rounding on)
+@pytest.mark.parametrize("shape", [(12, 40), (12, 3000), (3000, 16)])
+def test_coefficients_that_keep_a_singular_value_at_its_border(shape):
+    g = torch.outer(torch.randn(shape[0], generator=torch.Generator().manual_seed(1)), torch.linspace(-1, 1, shape[1])).cuda()
+    for steps, c in ((2, (0.0, 0.0, 1.0)), (3, (0.0, 0.0, 1.0)), (4, (0.5, 0.0, 0.5)), (32, (1.0, 0.0, 0.0)), (32, (1.5, -0.5, 0.0))):
+        check_orthogonal(g, steps=steps, coefficients=c)
+    with pytest.raises(ValueError, match="grow beyond"):
+        train_ops.orthogonalize(g, steps=8, coefficients=(0.0, 0.0, 1.0))

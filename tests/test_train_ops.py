@@ -372,3 +372,17 @@ def test_slope_0_is_a_relu():
     want = train_ops.layer_norm(torch.relu(x), w, b)
     assert torch.equal(y.nan_to_num(77.0), want.nan_to_num(77.0))
     assert bool(y[2].isnan().all()) and bool(torch.isfinite(y[[0, 1, 3, 4]]).all())
+
+
+def test_coefficients_under_which_roundings_grow_are_refused():
+    g = torch.outer(torch.arange(1.0, 5.0), torch.arange(1.0, 7.0))
+    unit = g / g.norm()  # of rank one: its singular value is 1, which x^5 keeps
+    assert float((train_ops.orthogonalize(g, steps=3, coefficients=(0.0, 0.0, 1.0)) - unit).abs().max()) < 2e-5
+    assert _lib.lib().lrb_muon_bound(3, 0.0, 0.0, 1.0) == 1.0
+    for steps, c in ((8, (0.0, 0.0, 1.0)), (32, (0.0, 0.0, -1.0)), (12, (0.5, 0.0, 0.5)), (20, (0.0, 1.0, 0.0))):
+        assert _lib.lib().lrb_muon_bound(steps, *c) > 64.0
+        with pytest.raises(ValueError, match="grow beyond"):
+            train_ops.orthogonalize(g, steps=steps, coefficients=c)
+    for steps, c in ((32, train_ops.COEFFICIENTS), (32, (1.5, -0.5, 0.0)), (32, (15 / 8, -10 / 8, 3 / 8)), (32, (2.0, -1.5, 0.5)),
+                     (32, (1.0, 0.0, 0.0))):
+        assert _lib.lib().lrb_muon_bound(steps, *c) < 1.5
