@@ -568,8 +568,8 @@ int lrb_layer_norm_bwd_dev(int device, void *stream, int x_type, int w_type, uin
  *   p <- decay p + alpha X;  with decay = 0 p is not read
  * Strides are in elements, of (matrix, row, column), any values; p and m must not overlap each other, g (which p may be, with
  * the same strides and type), or another item's.  A matrix that holds an infinity or a NaN gives NaN throughout, one of zeros
- * X = 0.  1 <= steps <= 32; a matrix below 2^31 elements with sides
- * of at most 2^22.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
+ * X = 0.  1 <= steps <= 32; sides of at
+ * most 2^22, and rows x cols below 2^31 with both rounded up to multiples of 64.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
 typedef struct {
     void *p;
     const void *g;

@@ -1295,8 +1295,8 @@ static bool mu_items_fit(const lrb_muon_item *items, int n)
         const lrb_muon_item &s = items[k];
         if (s.count < 0 || s.rows < 0 || s.cols < 0) return false;
         if (s.count == 0 || s.rows == 0 || s.cols == 0) continue;
-        // a side below 2^22 and planes below 2^31 entries: the kernels' 32-bit indices hold
-        if (s.rows > (1 << 22) || s.cols > (1 << 22) || (s.rows + 63) * (s.cols + 63) > INT_MAX) return false;
+        // sides up to 2^22 and planes below 2^31 entries, both sides padded to 64: the kernels' 32-bit indices hold
+        if (s.rows > (1 << 22) || s.cols > (1 << 22) || (s.rows + 63) / 64 * 64 * ((s.cols + 63) / 64 * 64) > INT_MAX) return false;
         if (!s.p || !s.g || s.p_type < LRB_F32 || s.p_type > LRB_F16 || s.g_type < LRB_F32 || s.g_type > LRB_F16) return false;
         if (s.m && (s.m_type < LRB_F32 || s.m_type > LRB_F16)) return false;
     }

@@ -260,6 +260,14 @@ _ITEM = struct.Struct("=3Q9q3q3i2fi")  # lrb_muon_item
 _DIVERGED = 64.0                       # LRB_MUON_DIVERGED
 
 
+def _check_size(t, name):
+    """What lrb_muon_dev takes (the lengths of its kernels' indices)."""
+    rows, cols = t.shape[-2:]
+    if rows > 1 << 22 or cols > 1 << 22 or (rows + 63) // 64 * 64 * ((cols + 63) // 64 * 64) >= 1 << 31:
+        raise ValueError(f"{name}: sides up to 2^22, and fewer than 2^31 elements with both rounded up to multiples of 64 are wanted "
+                         f"on the GPU, not {rows} x {cols}")
+
+
 def _stack(t, name):
     """t as matrices x rows x columns, without a copy."""
     if t.dim() == 2:
@@ -311,6 +319,7 @@ def _muon_items(params, grads, momenta, lr, decay, scale):
     for p, g, m in zip(params, grads, momenta):
         if not p.numel():
             continue
+        _check_size(p, "params")
         p3, m3 = _stack(p, "params"), None if m is None else _stack(m, "momenta")
         g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "grads")  # a copy where the leading axes ask for one
         held += [p3, g3, m3]
@@ -365,6 +374,7 @@ def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     if not g.is_cuda:
         return out.copy_(_orthogonal_plain(g, steps, coefficients, eps))
     _refuse_unseen("orthogonalize", g, out)
+    _check_size(g, "g")
     if out.data_ptr() != g.data_ptr() or out.stride() != g.stride() or out.dtype != g.dtype:
         (g0, g1), (o0, o1) = _extent(g), _extent(out)
         if g0 < o1 and o0 < g1:  # a matrix of out may lie over another matrix of g

@@ -386,3 +386,19 @@ def test_coefficients_under_which_roundings_grow_are_refused():
     for steps, c in ((32, train_ops.COEFFICIENTS), (32, (1.5, -0.5, 0.0)), (32, (15 / 8, -10 / 8, 3 / 8)), (32, (2.0, -1.5, 0.5)),
                      (32, (1.0, 0.0, 0.0))):
         assert _lib.lib().lrb_muon_bound(steps, *c) < 1.5
+
+
+def test_the_largest_sizes():
+    L = _lib.lib()
+    for rows, cols, fits in ((46336, 46336, True), (46340, 46340, False), (448, 1 << 22, True), (500, 1 << 22, False), (1, 1 << 22, True),
+                             (1, (1 << 22) + 1, False), ((1 << 22) + 1, 1, False), (1 << 22, 511, False), (1 << 22, 448, True),
+                             (65536, 32704, True), (65536, 32705, False)):
+        item = C.create_string_buffer(train_ops._ITEM.pack(64, 64, 0, 0, cols, 1, 0, cols, 1, 0, 0, 0, 1, rows, cols, 0, 0, 0, 1.0, 0.0, 0))
+        assert (L.lrb_muon_ws_bytes(item, 1) > 0) == fits, (rows, cols)
+        t = torch.empty(rows, cols, device="meta")
+        if fits:
+            train_ops._check_size(t, "g")
+        else:
+            assert L.lrb_muon_dev(0, None, item, 1, 0.0, 0, 5, 1.5, -0.5, 0.0, 0.0, 256, 1 << 60) == 1
+            with pytest.raises(ValueError, match="2.31"):
+                train_ops._check_size(t, "g")
