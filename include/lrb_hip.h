@@ -569,7 +569,9 @@ int lrb_layer_norm_bwd_dev(int device, void *stream, int x_type, int w_type, uin
  * Strides are in elements, of (matrix, row, column), any values; p and m must not overlap each other, g (which p may be, with
  * the same strides and type), or another item's.  A matrix that holds an infinity or a NaN gives NaN throughout, one of zeros
  * X = 0.  1 <= steps <= 32; sides of at
- * most 2^22, and rows x cols below 2^31 with both rounded up to multiples of 64.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256. */
+ * most 2^22, and rows x cols below 2^31 with both rounded up to multiples of 64.  d_ws: lrb_muon_ws_bytes bytes, aligned to 256: none
+ * for matrices that fit a workgroup's LDS (128 x 208, 96 x 320, 64 x 512, 32 x 1024 and less), else 4 n (5 l + 3 n) for a matrix of
+ * short side n and long side l (padded to 64), of a stack or list those of up to 4 GiB at a time, and up to 64 MiB besides. */
 typedef struct {
     void *p;
     const void *g;

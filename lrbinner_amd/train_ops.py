@@ -354,7 +354,9 @@ def orthogonalize(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
 
     g: [..., rows, columns], any strides; each matrix by itself; one that holds an infinity or a NaN becomes NaN, one of
     zeros stays.  ``out``: a tensor of g's shape, g itself among them (by default a new one of g's type).  The products are
-    as exact as float32 ones for every type of g.  No gradient: an update is not differentiated."""
+    as exact as float32 ones for every type of g.  No gradient: an update is not differentiated.  On the GPU a matrix that does not fit
+    a workgroup's LDS (128 x 208, 32 x 1024 ...) takes a workspace of 8 times its float32 size if it is square, 5 times if it is
+    long; the matrices of a stack up to 4 GiB at a time."""
     _known_type(g, "g")
     if g.dim() < 2:
         raise ValueError(f"g: a matrix is wanted, not shape {tuple(g.shape)}")

@@ -402,3 +402,22 @@ def test_the_largest_sizes():
             assert L.lrb_muon_dev(0, None, item, 1, 0.0, 0, 5, 1.5, -0.5, 0.0, 0.0, 256, 1 << 60) == 1
             with pytest.raises(ValueError, match="2.31"):
                 train_ops._check_size(t, "g")
+
+
+def test_the_workspace_is_what_is_said():
+    L = _lib.lib()
+
+    def asks(*shapes):
+        items = b"".join(train_ops._ITEM.pack(64, 64, 0, r * c, c, 1, r * c, c, 1, 0, 0, 0, n, r, c, 0, 0, 0, 1.0, 0.0, 0) for n, r, c in shapes)
+        return L.lrb_muon_ws_bytes(C.create_string_buffer(items, len(items)), len(shapes))
+
+    def said(n, rows, cols):
+        s, l = sorted(((rows + 63) // 64 * 64, (cols + 63) // 64 * 64))
+        return 4 * n * s * (5 * l + 3 * s)
+
+    for shapes in ([(1, 4096, 4096)], [(1, 511, 1025)], [(8, 1024, 2048)], [(1, 16384, 16384)], [(1, 2048, 2048), (1, 5461, 2048), (2, 300, 70)]):
+        most = sum(said(*s) for s in shapes)
+        assert most <= asks(*shapes) <= most + (64 << 20) + (1 << 20) + most // 64, shapes
+    assert (2 << 30) < asks((1000, 1024, 1024)) <= (4 << 30) + (128 << 20)
+    for shape in ((128, 208), (320, 96), (64, 512), (1024, 32), (1, 1)):
+        assert asks((3, *shape)) == 0
