@@ -8,6 +8,7 @@
 
 #include "lrb_hip.h"
 #include "lrb_internal.h"
+#include "lrb_once.h"
 
 struct lrb_ctx {
     int device;
@@ -106,18 +107,11 @@ struct lrb_on_device {
     lrb_on_device &operator=(const lrb_on_device &) = delete;
 };
 
-// hipFuncSetAttribute is per DEVICE: a launch site remembers which devices it has raised its kernel's limit on
-// (the C ABI allows contexts on several GPUs in one process).  A race between two threads sets the attribute twice.
-struct lrb_per_device_once {
-    bool done[64] = {};
-    bool need(int dev)
-    {
-        if (dev < 0 || dev >= 64) return true;
-        if (done[dev]) return false;
-        done[dev] = true;
-        return true;
-    }
-};
+// The largest dynamic LDS of a kernel's launches on a device, asked for once (in a `static lrb_per_device_once` of the launch site).
+inline hipError_t lrb_raise_lds(lrb_per_device_once &done, int device, const void *kernel, int bytes)
+{
+    return done.once(device, [=] { return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+}
 
 // *p = at least `bytes` of device memory owned by the context (slot is reused, contents
 // are not preserved when it grows)

@@ -128,9 +128,7 @@ int fmt_launch(lrb_ctx *c, const uint32_t *d_vals, const uint32_t *d_per_row, ui
     const uint32_t width = MODE == 0 ? 9u * dim + 1u : 9u * dim;
     const size_t smem = (size_t)FMT_ROWS * width;
     static lrb_per_device_once raised[2];
-    if (smem > 48 * 1024 && raised[MODE].need(c->device)) {
-        HIP_TRY(hipFuncSetAttribute((const void *)fmt_rows_kernel<MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    }
+    if (smem > 48 * 1024) HIP_TRY(lrb_raise_lds(raised[MODE], c->device, (const void *)fmt_rows_kernel<MODE>, 160 * 1024));
     const uint64_t blocks = (n + FMT_ROWS - 1) / FMT_ROWS;
     ARG_TRY(blocks <= 0x7FFFFFFFull);
     hipLaunchKernelGGL(fmt_rows_kernel<MODE>, dim3((unsigned)blocks), dim3(256), smem, c->stream, d_vals, d_per_row, n, dim, k, d_text,

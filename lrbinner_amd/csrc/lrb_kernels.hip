@@ -2008,10 +2008,7 @@ static int launch_k1(lrb_ctx *c, const uint32_t *d_codes, const uint64_t *d_code
     const uint32_t dimpad = (c->dim[K] + 63u) & ~63u;
     const size_t smem = (size_t)4 * BINS * SUBS * 4 + (size_t)4 * dimpad * 4 + BINS * 2;
     static lrb_per_device_once attr_done;
-    if (attr_done.need(c->device)) {
-        HIP_TRY(hipFuncSetAttribute((const void *)k1_count_kernel<K, SUBS, WPS, TW>,
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    }
+    HIP_TRY(lrb_raise_lds(attr_done, c->device, (const void *)k1_count_kernel<K, SUBS, WPS, TW>, (int)smem));
     int per_cu = (int)((160 * 1024) / smem);
     if (per_cu > 2 * WPS) per_cu = 2 * WPS; // 4 waves per block, WPS waves per SIMD
     if (per_cu > 8) per_cu = 8;
@@ -2171,10 +2168,7 @@ static int k1_lane_launch(lrb_ctx *c, int k, const uint32_t *d_codes_t, const ui
         // walking everything measured slower: they fall into step and flush together)
         constexpr size_t smem = 65536 + 1024;   // histogram + tail / output row / class tables of the flush
         static lrb_per_device_once attr_s2;
-        if (attr_s2.need(c->device)) {
-            HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(&k1_lane4s2_kernel<8, 2>),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        }
+        HIP_TRY(lrb_raise_lds(attr_s2, c->device, reinterpret_cast<const void *>(&k1_lane4s2_kernel<8, 2>), (int)smem));
         ARG_TRY(ngroups <= 0x3FFFFFFFull);
         hipLaunchKernelGGL((k1_lane4s2_kernel<8, 2>), dim3((unsigned)(2 * ngroups)), dim3(512), smem, c->stream, ct,
                            d_group_off, d_order, d_lens, n, d_counts);
@@ -2182,10 +2176,7 @@ static int k1_lane_launch(lrb_ctx *c, int k, const uint32_t *d_codes_t, const ui
         // k = 5: two half-groups per CU, 2 x (64 KB, eight waves) -- one's flush (2 KB of output per read) overlaps
         // the other's tally; a whole group per CU (128 KB, sixteen waves) measured 1.98 ms against 1.61 ms per 1 M reads
         static lrb_per_device_once attr_set;
-        if (attr_set.need(c->device)) {
-            HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(&k1_lane4_kernel<5, 8, 2, true>),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, 65536 + 2560));
-        }
+        HIP_TRY(lrb_raise_lds(attr_set, c->device, reinterpret_cast<const void *>(&k1_lane4_kernel<5, 8, 2, true>), 65536 + 2560));
         ARG_TRY(ngroups <= 0x3FFFFFFFull);
         // 64 KB of histogram + the flush's tables (output row per column 256 B, class table 2 KB)
         hipLaunchKernelGGL((k1_lane4_kernel<5, 8, 2, true>), dim3((unsigned)(2 * ngroups)), dim3(512), 65536 + 2560, c->stream, ct,
@@ -3019,9 +3010,7 @@ extern "C" int lrb_packed_kmer_counts_many_dev(lrb_ctx *c, const lrb_packed *con
     }
     constexpr size_t smem = 65536 + 1024;   // (k1_lane_launch: histogram + tail / output row / class tables of the flush)
     static lrb_per_device_once attr_many;
-    if (attr_many.need(c->device))
-        HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(&k1_lane4s2_kernel<8, 2, false, 4, true>),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    HIP_TRY(lrb_raise_lds(attr_many, c->device, reinterpret_cast<const void *>(&k1_lane4s2_kernel<8, 2, false, 4, true>), (int)smem));
     hipLaunchKernelGGL((k1_lane4s2_kernel<8, 2, false, 4, true>), dim3((unsigned)(2 * groups)), dim3(512), smem, c->stream,
                        reinterpret_cast<const uint4 *>(base), (const uint64_t *)d_pairs, (const uint32_t *)d_order,
                        (const uint32_t *)d_lens, groups * 64, d_counts, (uint64_t *)nullptr);

@@ -1268,8 +1268,7 @@ extern "C" int lrb_k15_lists_part_dev(lrb_ctx *c, const uint32_t *d_codes, const
                            d_bounds);
         {
             static lrb_per_device_once ring_attr;
-            if (ring_attr.need(c->device))
-                HIP_TRY(hipFuncSetAttribute((const void *)wl_part_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, WLR_SMEM_BYTES));
+            HIP_TRY(lrb_raise_lds(ring_attr, c->device, (const void *)wl_part_kernel, WLR_SMEM_BYTES));
             // (one workgroup a CU: the rings take 128 of its 160 KB)
             const unsigned gr = (unsigned)(nunits < (uint32_t)c->n_cu ? nunits : (uint32_t)c->n_cu);
             hipLaunchKernelGGL(wl_part_kernel, dim3(gr), dim3(1024), WLR_SMEM_BYTES, c->stream, d_codes, d_mask, d_code_off,
@@ -1322,9 +1321,7 @@ extern "C" int lrb_k15_lists_tally_dev(lrb_ctx *c, const uint32_t *d_codes, cons
     const uint64_t ngroups = (n + reads_per_group - 1) / reads_per_group;
     ARG_TRY(ngroups <= 0x7FFFFFFFull / WL_MAX_UNITS);
     static lrb_per_device_once attr_done;
-    if (attr_done.need(c->device)) {
-        HIP_TRY(hipFuncSetAttribute((const void *)wl_tally_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 131072));
-    }
+    HIP_TRY(lrb_raise_lds(attr_done, c->device, (const void *)wl_tally_kernel, 131072));
     hipLaunchKernelGGL(wl_tally_kernel, dim3(WL_BUCKETS), dim3(1024), 131072, c->stream, d_lists, d_bounds, d_gbase,
                        (uint32_t)ngroups, d_half);
     HIP_TRY(hipGetLastError());
@@ -1342,9 +1339,7 @@ static int wl_sweep_launch(lrb_ctx *c, unsigned grid, size_t smem, const uint32_
 {
     constexpr int EW = (DBV && BITS == 8) ? 8 : 12, MD = EW == 8 ? 3 : 2;
     static lrb_per_device_once once_;
-    if (once_.need(c->device))
-        HIP_TRY(hipFuncSetAttribute((const void *)wl_sweep_kernel<4, EW, MD, DBV, BITS, NP>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    163840));
+    HIP_TRY(lrb_raise_lds(once_, c->device, (const void *)wl_sweep_kernel<4, EW, MD, DBV, BITS, NP>, 163840));
     hipLaunchKernelGGL((wl_sweep_kernel<4, EW, MD, DBV, BITS, NP>), dim3(grid), dim3(64 * (4 + EW)), smem, c->stream, d_lists, d_bounds,
                        d_gbase, n, reads_per_group, (uint32_t)ngroups, (const uint8_t *)d_use, (uint32_t)bins, d_hist, d_sums);
     return LRB_OK;

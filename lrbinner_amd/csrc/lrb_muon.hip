@@ -30,7 +30,6 @@
 #include <string.h>
 
 #include <algorithm>
-#include <atomic>
 #include <new>
 #include <vector>
 
@@ -1363,13 +1362,8 @@ extern "C" int lrb_muon_dev(int device, void *stream, const lrb_muon_item *items
             g.sx = sx;
             memcpy(g.std, std, sizeof(std));
             if (gr.lds) {
-                // (a bit a device, set behind the call: a thread that finds it may launch)
-                static std::atomic<uint64_t> raised{0};
-                const uint64_t bit = device < 64 ? 1ull << device : 0;
-                if (!(raised.load(std::memory_order_acquire) & bit)) {
-                    HIP_TRY(hipFuncSetAttribute((const void *)mu_small_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MU_SMALL_LDS));
-                    raised.fetch_or(bit, std::memory_order_release);
-                }
+                static lrb_per_device_once raised;
+                HIP_TRY(lrb_raise_lds(raised, device, (const void *)mu_small_kernel, MU_SMALL_LDS));
                 hipLaunchKernelGGL(mu_small_kernel, dim3(gr.mats), dim3(64 * MU_SMALL_WAVES), gr.lds, st, g);
                 HIP_TRY(hipGetLastError());
                 return LRB_OK;

@@ -187,3 +187,43 @@ def test_drop_in_executables_are_built_and_parse_their_argv():
         assert r.returncode != 0 and "usage" in r.stderr
         ldd = subprocess.run(["ldd", exe], capture_output=True, text=True).stdout
         assert "lrbinner_amd/bin/../liblrb_hip.so" in ldd or "liblrb_hip.so =>" in ldd
+
+
+def test_a_device_is_done_when_the_call_has_succeeded(tmp_path):
+    """lrb_once.h: no thread passes before one call has come back, and a call that fails is made again."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lrbinner_amd", "csrc")
+    (tmp_path / "once.cpp").write_text("""
+        #include "lrb_once.h"
+        #include <chrono>
+        #include <thread>
+        #include <vector>
+        static lrb_per_device_once site;
+        static std::atomic<int> raised{0}, calls{0}, early{0};
+        int main()
+        {
+            std::vector<std::thread> threads;
+            for (int k = 0; k < 8; ++k)
+                threads.emplace_back([k] {
+                    std::this_thread::sleep_for(std::chrono::milliseconds(10 * k));
+                    site.once(3, [] {
+                        ++calls;
+                        std::this_thread::sleep_for(std::chrono::milliseconds(45));
+                        raised = 1;
+                        return 0;
+                    });
+                    if (!raised) ++early;
+                });
+            for (auto &t : threads) t.join();
+            const int before = calls;
+            if (early || before < 1 || site.once(3, [] { ++calls; return 7; }) != 0 || calls != before) return 1;
+            int tries = 0;  // a failure is no success, and another device is another one
+            if (site.once(4, [&] { return ++tries, 5; }) != 5 || site.once(4, [&] { return ++tries, 0; }) != 0 || tries != 2) return 2;
+            for (int dev : {-1, 64, 1000})  // beyond what is remembered: every time
+                for (int k = 0; k < 2; ++k) site.once(dev, [&] { return ++tries, 0; });
+            return tries == 8 ? 0 : 3;
+        }
+    """)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-pthread", "-I", csrc, "-o", str(tmp_path / "once"), str(tmp_path / "once.cpp")])
+    assert subprocess.run([str(tmp_path / "once")]).returncode == 0
