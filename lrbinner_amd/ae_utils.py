@@ -12,6 +12,7 @@ part), every epoch draws one device-side permutation, and loss bookkeeping
 stays on the device until the epoch ends.  The dense layers are genuine GEMMs
 and run on the matrix cores through rocBLAS/hipBLASLt.
 """
+import contextlib
 import json
 import logging
 import os
@@ -218,6 +219,20 @@ class VAE(nn.Module):
         optimizer.step()
         sums += torch.stack([loss.detach(), e_cov.detach(), e_comp.detach(), kld.detach()])
 
+    @contextlib.contextmanager
+    def _fresh_leaves(self):
+        """Other Parameters over the same memory, for a training that is captured: a backward pass that meets the accumulation nodes of a
+        graph that the caller still holds (they belong to the caller's stream) cannot be recorded."""
+        owners = [(m, name, p) for m in self.modules() for name, p in m._parameters.items() if p is not None]
+        fresh = {}
+        for m, name, p in owners:
+            m._parameters[name] = fresh.setdefault(id(p), nn.Parameter(p.detach(), requires_grad=p.requires_grad))
+        try:
+            yield
+        finally:
+            for m, name, p in owners:
+                m._parameters[name] = p
+
     def _optimizer(self, name, lrate, muon_lrate, capturable):
         if name == 'adam':
             return optim.Adam(self.parameters(), lr=lrate, capturable=capturable)
@@ -251,7 +266,13 @@ class VAE(nn.Module):
             use_graph = on_gpu and os.environ.get("LRB_VAE_GRAPH", "1") != "0" \
                 and self.constraints is None
         self.release_native()  # what an earlier run left for encode() would be out of date
-        optimizer = self._optimizer(optimizer, lrate, muon_lrate, bool(use_graph))
+        with self._fresh_leaves() if use_graph else contextlib.nullcontext():
+            self._trainmodel_torch(data, nepochs, steps, batch_size, use_graph,
+                                   self._optimizer(optimizer, lrate, muon_lrate, bool(use_graph)))
+        if save_path is not None:
+            self.save(save_path)
+
+    def _trainmodel_torch(self, data, nepochs, steps, batch_size, use_graph, optimizer):
         n = data.shape[0]
         graphs = {}  # batch size -> (graph, static index buffer)
         for epoch in range(nepochs):
@@ -303,8 +324,6 @@ class VAE(nn.Module):
                 logger.debug(f'Epoch: {epoch + 1:4} Loss: {s[0]:.6f}\tEC: {s[1]:.7f}\t'
                              f'EP: {s[2]:.6f}\tKLD: {s[3]:.4f}\tBatchsize: {batch_size}')
         self._sums = None
-        if save_path is not None:
-            self.save(save_path)
 
     def _trainmodel_native(self, data, nepochs, lrate, steps, batch_size, save_path):
         """The same schedule on the fused HIP step (include/lrb_hip.h K7, csrc/lrb_vae.hip):

@@ -831,3 +831,31 @@ def test_coefficients_that_keep_a_singular_value_at_its_border(shape):
         check_orthogonal(g, steps=steps, coefficients=c)
     with pytest.raises(ValueError, match="grow beyond"):
         train_ops.orthogonalize(g, steps=8, coefficients=(0.0, 0.0, 1.0))
+
+
+class _Counted(torch.cuda.CUDAGraph):
+    replays = 0
+
+    def replay(self):
+        _Counted.replays += 1
+        super().replay()
+
+
+@pytest.mark.parametrize("norm,optimizer", [("layer", "muon"), ("layer", "adam"), ("batch", "muon")])
+@pytest.mark.parametrize("held", [False, True])
+def test_the_vae_s_step_is_captured(norm, optimizer, held, monkeypatch):
+    """Also where the caller holds a graph of the same weights."""
+    torch.manual_seed(0)
+    data = torch.rand(3000, 168, device="cuda")
+    vae = ae_utils.VAE(32, 136, norm=norm, device="cuda")
+    before = [p.detach().clone() for p in vae.parameters()]
+    outputs = vae(data[:100]) if held else None
+    mine = list(vae.parameters())
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", _Counted)
+    _Counted.replays = 0
+    vae.trainmodel(data, nepochs=4, batchsteps=[2], batch_size=256, optimizer=optimizer)
+    # 11 batches of 256 and 5 of 512 an epoch, of which the first epoch of each size gives three to the warm-up
+    assert _Counted.replays == 2 * 11 + 2 * 5 - 2 * 3
+    for p, q, was in zip(vae.parameters(), mine, before):
+        assert p is q and bool(torch.isfinite(p).all()) and not torch.equal(p, was)
+    del outputs

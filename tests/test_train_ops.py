@@ -421,3 +421,25 @@ def test_the_workspace_is_what_is_said():
     assert (2 << 30) < asks((1000, 1024, 1024)) <= (4 << 30) + (128 << 20)
     for shape in ((128, 208), (320, 96), (64, 512), (1024, 32), (1, 1)):
         assert asks((3, *shape)) == 0
+
+
+def test_a_captured_training_has_leaves_of_its_own():
+    vae = ae_utils.VAE(10, 32, latent_dims=3, hidden_layers=[8], norm="layer")
+    held = list(vae.parameters())
+    x = torch.rand(5, 42)
+    recon, mu, sigma = vae(x)  # a graph of the caller's, alive
+    node = lambda p: torch.autograd.graph.get_gradient_edge(p).node
+    before = [node(p) for p in held]
+    with pytest.raises(KeyError), vae._fresh_leaves():
+        fresh = list(vae.parameters())
+        assert len(fresh) == len(held) and not any(a is b for a, b in zip(fresh, held))
+        assert all(a.data_ptr() == b.data_ptr() and a.requires_grad for a, b in zip(fresh, held))
+        assert not any(node(p) in before for p in fresh)
+        vae.calc_loss(x, *vae(x))[0].backward()
+        assert all(p.grad is not None for p in fresh) and all(p.grad is None for p in held)
+        with torch.no_grad():
+            vae.outputlayer.weight.zero_()
+        raise KeyError
+    assert all(a is b for a, b in zip(vae.parameters(), held)) and not bool(vae.outputlayer.weight.any())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        recon.sum().backward()  # the caller's graph knows that its weights have changed
