@@ -477,7 +477,7 @@ class Muon(torch.optim.Optimizer):
         super().load_state_dict(state_dict)  # casts the state to the parameters' type: the momentum stays float32
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         for i, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
-            if i in state_dict["state"]:
+            if "momentum" in state_dict["state"].get(i, ()):
                 self.state[p]["momentum"] = state_dict["state"][i]["momentum"].to(device=p.device, dtype=torch.float32, copy=True)
 
     @torch.no_grad()
@@ -491,12 +491,11 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                state = self.state[p]
-                if "momentum" not in state:
+                if "momentum" not in self.state.get(p, ()):
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("Muon: take one step before the capture, or each replay clears the momentum")
-                    state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-                by_device.setdefault(p.device, []).append((p, p.grad, state["momentum"]))
+                    self.state[p]["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                by_device.setdefault(p.device, []).append((p, p.grad, self.state[p]["momentum"]))
             for of in by_device.values():
                 muon_step(*zip(*of), lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
                           weight_decay=group["weight_decay"], steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])

@@ -859,3 +859,13 @@ def test_the_vae_s_step_is_captured(norm, optimizer, held, monkeypatch):
     for p, q, was in zip(vae.parameters(), mine, before):
         assert p is q and bool(torch.isfinite(p).all()) and not torch.equal(p, was)
     del outputs
+
+
+def test_a_refused_step_leaves_no_state(monkeypatch):
+    w = torch.nn.Parameter(torch.ones(3, 4, device="cuda"))
+    w.grad = torch.ones_like(w)
+    opt = train_ops.Muon([w])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        opt.step()
+    assert not opt.state_dict()["state"]

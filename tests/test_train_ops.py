@@ -443,3 +443,16 @@ def test_a_captured_training_has_leaves_of_its_own():
     assert all(a is b for a, b in zip(vae.parameters(), held)) and not bool(vae.outputlayer.weight.any())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         recon.sum().backward()  # the caller's graph knows that its weights have changed
+
+
+def test_a_state_without_a_momentum_is_loaded():
+    """As a refused first step left it."""
+    w = torch.nn.Parameter(torch.ones(3, 4))
+    opt = train_ops.Muon([w])
+    opt.state[w]
+    saved = opt.state_dict()
+    again = train_ops.Muon([w])
+    again.load_state_dict(saved)
+    w.grad = torch.randn(3, 4)
+    again.step()
+    assert again.state[w]["momentum"].shape == (3, 4)
