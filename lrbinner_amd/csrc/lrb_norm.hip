@@ -156,22 +156,20 @@ template <int TPR> __device__ __forceinline__ float ln_sum(float v, float *red, 
 
 // Two sums behind one barrier; `red`: 4 x (TPR / 64) floats.  (Where one sum and then two are made of every row, the one has the
 // first quarter of `red` and the two its second half.)
+// The lanes of a pair take one of the two sums each, so that both go through as many exchanges as one would.
 template <int TPR> __device__ __forceinline__ void ln_sum2(float &v, float &w, float *red, int &flip)
 {
     constexpr int W = TPR < 64 ? TPR : 64;
+    const bool odd = threadIdx.x & 1;
+    float mine = odd ? w : v, other = odd ? v : w;
+    mine += __shfl_xor(other, 1, 64);
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-        v += __shfl_xor(v, o, 64);
-        w += __shfl_xor(w, o, 64);
-    }
+    for (int o = W / 2; o > 1; o >>= 1) mine += __shfl_xor(mine, o, 64);
     if (TPR > 64) {
         constexpr int NW = TPR / 64;
         float *r = red + flip * 2 * NW;
         flip ^= 1;
-        if ((threadIdx.x & 63) == 0) {
-            r[threadIdx.x >> 6] = v;
-            r[NW + (threadIdx.x >> 6)] = w;
-        }
+        if ((threadIdx.x & 63) < 2) r[(odd ? NW : 0) + (threadIdx.x >> 6)] = mine;
         lrb_barrier();
         v = w = 0.0f;
 #pragma unroll
@@ -179,6 +177,10 @@ template <int TPR> __device__ __forceinline__ void ln_sum2(float &v, float &w, f
             v += r[i];
             w += r[NW + i];
         }
+    } else {
+        other = __shfl_xor(mine, 1, 64);
+        v = odd ? other : mine;
+        w = odd ? mine : other;
     }
 }
 
@@ -244,9 +246,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_fwd_kernel(ln_args a
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float e = u[c][i] - mean;
-                s = fmaf(LN_OWN(c, i) ? e : 0.0f, inv, s);
-                s2 += LN_OWN(c, i) ? e * e : 0.0f;
+                const float e = LN_OWN(c, i) ? u[c][i] - mean : 0.0f;
+                s = fmaf(e, inv, s);
+                s2 = fmaf(e, e, s2);
             }
         ln_sum2<TPR>(s, s2, red, flip);
         const float rstd = ln_statistics(s, s2 * inv, a.eps, mean);
