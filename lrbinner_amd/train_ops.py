@@ -319,11 +319,12 @@ def _muon_items(params, grads, momenta, lr, decay, scale):
     for p, g, m in zip(params, grads, momenta):
         if not p.numel():
             continue
-        _check_size(p, "params")
         p3, m3 = _stack(p, "params"), None if m is None else _stack(m, "momenta")
         g3 = g.reshape(-1, *g.shape[-2:]) if g.dim() > 3 else _stack(g, "grads")  # a copy where the leading axes ask for one
-        held += [p3, g3, m3]
+        held += (p3, g3, m3)
         count, rows, cols = p3.shape
+        if rows * cols > 1 << 22:  # (a smaller one fits whatever its sides)
+            _check_size(p, "params")
         by = math.sqrt(max(1.0, rows / cols)) if scale is None else scale
         items.append(_ITEM.pack(p3.data_ptr(), g3.data_ptr(), 0 if m is None else m3.data_ptr(), *p3.stride(), *g3.stride(),
                                 *((0, 0, 0) if m is None else m3.stride()), count, rows, cols, _TYPES[p.dtype], _TYPES[g.dtype],

@@ -456,3 +456,9 @@ def test_a_state_without_a_momentum_is_loaded():
     w.grad = torch.randn(3, 4)
     again.step()
     assert again.state[w]["momentum"].shape == (3, 4)
+
+
+def test_a_list_with_a_weight_that_is_too_large_is_refused():
+    small, wide = torch.zeros(3, 4), torch.empty(1, (1 << 22) + 1)
+    with pytest.raises(ValueError, match="params: sides up to"):
+        train_ops._muon_items([small, wide], [small, wide], [None, None], 0.1, 1.0, None)
