@@ -22,9 +22,9 @@
 // errors of the small singular values' part of A would then grow by a^2 a step instead of a.)  A matrix that fits one workgroup's LDS
 // goes through all steps in one launch (mu_small_kernel).
 // Measured, where a library product of 8192 x 8192 float16 reaches 1.09 PFLOP/s: a 4096 x 4096 float32 weight 3.9 ms = 1.05
-// PFLOP/s of its three products (B X alone 1.17); a layer's four weights (2048 x 2048 twice, 5461 x 2048, 2048 x 5461,
-// bfloat16) 2.96 ms, of them 0.15 for the momentum and the splitting, at 4.6 and 5.3 TB/s; 8 x 1024 x 2048 0.98 ms;
-// 1025 x 511 169 us (26 launches that wait for each other); 128 x 168 50 us.
+// PFLOP/s of its three products (B X alone 1.14); a layer's four weights (2048 x 2048 twice, 5461 x 2048, 2048 x 5461,
+// bfloat16) 3.99 ms, of them 0.17 for the momentum and the splitting, at 4.5 and 5.5 TB/s; 8 x 1024 x 2048 1.31 ms;
+// 1025 x 511 158 us (23 launches that wait for each other); 128 x 168 51 us.
 #include <limits.h>
 #include <math.h>
 #include <string.h>
@@ -588,10 +588,10 @@ __host__ __device__ inline int mu_by_xcd(int xcd, int rank, int n)
 // row (four of hi, four of lo) lie at chunk ^ ((row >> 1) & 7), which spreads the 16 rows that a quarter wave reads over all
 // 64 banks.  The loads go from global memory to LDS directly, one stage ahead of the products (three for the smallest tile).
 // Bound: the matrix cores for the 256-tile (B X of 4096 x 4096: 352 us = 1.17 PFLOP/s; the chip lowers its clock under this
-// load: on zeros the whole call takes 2.9 ms, on numbers 3.9).  The 128-tile reaches 0.95 (four symmetric products of 2048: 115
-// us): it reads LDS twice as often for a product and has its loads only one shorter stage ahead.  Eight waves of 64 x 32 hide
-// that better than four of 64 x 64 (a layer's four weights 3.10 against 3.19 ms; two of 128 x 64: 3.38; eight with four stages:
-// 3.27).  The 64-tile is bound by its loads (eight symmetric products of 1024: 47 us).
+// load: on zeros the whole call takes 2.9 ms, on numbers 3.9).  The 128-tile reaches 0.85 to 0.95 (four symmetric products of 2048:
+// 115 to 121 us): it reads LDS twice as often for a product and has its loads only one shorter stage ahead.  Eight waves of 64 x 32 hide
+// that better than four of 64 x 64 (a layer's four weights, when blocks of steps were taken, 3.10 against 3.19 ms; two of 128 x 64:
+// 3.38; eight with four stages: 3.27).  The 64-tile is bound by its loads (eight symmetric products of 1024: 47 us).
 template <int T, int WM, int WN, int MODE>
 __global__ __launch_bounds__(64 * WM * WN) void mu_product_kernel(mu_args a)
 {

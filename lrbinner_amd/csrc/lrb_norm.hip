@@ -15,7 +15,7 @@
 // w and b are loaded once per thread and the weight's gradient is summed in registers: one partial row per workgroup is
 // written and a second kernel adds the partial rows in a fixed order (no atomics: the same bits run after run).
 // Everything between load and store is float32.
-// Measured (32,768 x 4096 bfloat16): forward 97 us = 5.5 TB/s, backward 164 us = 4.9 TB/s and 12 us for the join (a copy: 5.1).
+// Measured (32,768 x 4096 bfloat16): forward 97.5 us = 5.5 TB/s, backward 160 us = 5.0 TB/s and 12 us for the join (a copy: 5.1).
 #include <limits.h>
 #include <math.h>
 
@@ -44,7 +44,7 @@ struct ln_args {
 // any address.  Where a row ends inside the V, the thread takes the row's last V instead: it then computes some elements that
 // its neighbour computes too, from the same operands in the same order, and both store the same bits; only what is summed
 // over the row has to leave them out (ln_chunk::own).  So no load or store is made element by element, which for rows of
-// 4095 16-bit elements cost as much as the rest (a forward pass over 8191 of them: 48 us, so 27).  Rows of fewer than V
+// 4095 16-bit elements cost as much as the rest (a forward pass over 8191 of them: 48 us, so 25).  Rows of fewer than V
 // columns (LN_TINY) go element by element.  Rows of a multiple of V columns (LN_EVEN) have no such thread and are spared the
 // selections (32,768 x 4096 bfloat16 forward: 97 us, with them 114).  A thread whose columns all lie past the end reads the
 // row's last V too and stores nothing: with a branch between the loads of a row the same pass takes 129 us.
@@ -390,7 +390,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_bwd_kernel(ln_args a
     }
 }
 
-// Rows too long for the registers of a workgroup: the row is read again for each of its passes (it fits the L2).
+// Rows too long for the registers of a workgroup: the row is read again for each of its passes, element by element, mostly from beyond
+// the L2 (two workgroups a CU of an XCD, with x and dy of 16,384 float32, are 8 MB against its 4).  Measured (float32): forward
+// 1678 x 20,001 102 us, backward 2048 x 16,384 109 us and 49 us for dw and db: twice what the bytes take.
 template <typename T, bool ACT> __device__ __forceinline__ float ln_at(const ln_args &a, const T *x, long long row, int col, float &f)
 {
     const float v = (float)x[col];
