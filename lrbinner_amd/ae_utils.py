@@ -305,7 +305,7 @@ class VAE(nn.Module):
                         self._train_step(data, static_idx, optimizer, sums)
                     graphs[batch_size] = (g, static_idx)
                 except Exception as e:  # capture unsupported: stay eager, say so
-                    logger.debug(f"HIP graph capture of the VAE step failed ({e}); running eagerly")
+                    logger.warning(f"HIP graph capture of the VAE step failed ({e}); running eagerly")
                     use_graph = False
                     torch.cuda.synchronize()
             if use_graph and batch_size in graphs:

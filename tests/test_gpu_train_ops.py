@@ -869,3 +869,18 @@ def test_a_refused_step_leaves_no_state(monkeypatch):
     with pytest.raises(RuntimeError, match="before the capture"):
         opt.step()
     assert not opt.state_dict()["state"]
+
+
+def test_a_failed_capture_is_said(monkeypatch, caplog):
+    def refuses(graph):
+        raise RuntimeError("no capture today")
+
+    torch.manual_seed(0)
+    data = torch.rand(1000, 168, device="cuda")
+    vae = ae_utils.VAE(32, 136, norm="layer", device="cuda")
+    before = [p.detach().clone() for p in vae.parameters()]
+    monkeypatch.setattr(torch.cuda, "graph", refuses)
+    with caplog.at_level("WARNING", logger="LRBinner"):
+        vae.trainmodel(data, nepochs=2, batchsteps=[], batch_size=100)
+    assert sum("no capture today" in r.message for r in caplog.records) == 1
+    assert all(bool(torch.isfinite(p).all()) and not torch.equal(p, q) for p, q in zip(vae.parameters(), before))
